@@ -508,6 +508,58 @@ int mfnet_up_final_bwd_f32(const float* dlogits, float* dx, int64_t ldx, int64_t
 int mfnet_adapter_mix_bwd_f32(const float* dh, const float* ada, const float* wx, const float* wy, float* dada, float* dw, int64_t M,
                               int64_t D, hipStream_t stream);
 
+/* ---- 8-bit activation checkpoints (not in the reference, which keeps every activation in fp32). A row of C elements is held in blocks
+ * of 32 consecutive elements (the last of a row may be shorter): int8 codes [rows, C] and one exponent byte per block, exps
+ * [rows, ceil(C / 32)]. With amax the block's largest magnitude, e is the smallest integer in [-126, 121] with amax <= 127 * 2^e (121 if
+ * none), code = rint(x * 2^-e) clamped to +-127, the byte is e + 127; byte 255 marks a block that holds an infinity or NaN, all of whose
+ * elements stand for NaN. code * 2^e is exact in bf16. Any C >= 1 and any row stride >= C; rows whose C, strides and addresses allow
+ * 16-byte accesses (C % 8 == 0) take the fast kernels. codes / exps are dense. rows = 0 is allowed everywhere (nothing is launched). */
+int mfnet_ckpt8_pack(const void* x, int x_dtype, int64_t ldx, void* codes, void* exps, int64_t rows, int64_t C, hipStream_t stream);
+int mfnet_ckpt8_unpack(const void* codes, const void* exps, void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t C, hipStream_t stream);
+/* act = GELU(x) (erf form, nn.GELU) and the checkpoint of x; x and act of one dtype. */
+int mfnet_gelu_fwd_ckpt8(const void* x, int dtype, int64_t ldx, void* act, int64_t ldact, void* codes, void* exps, int64_t rows, int64_t C,
+                         hipStream_t stream);
+/* dx = dy * GELU'(x8), x8 the checkpoint's values; act (optional, row stride lddx) = GELU(x8). dy, dx, act of one dtype. */
+int mfnet_gelu_bwd_ckpt8(const void* codes, const void* exps, const void* dy, int dtype, int64_t lddy, void* dx, void* act, int64_t lddx,
+                         int64_t rows, int64_t C, hipStream_t stream);
+/* LayerNorm with its input kept in 8 bits: y bf16 [rows, C], mean / rstd [rows] of the exact x, checkpoint of x. C % 32 == 0, C <= 2048. */
+int mfnet_layernorm_fwd_ckpt8(const void* x, int x_dtype, int64_t ldx, const float* gamma, const float* beta, void* y, float* mean,
+                              float* rstd, void* codes, void* exps, int64_t rows, int64_t C, float eps, hipStream_t stream);
+/* With xh = (x8 - mean) rstd and t = dy gamma: dx = rstd (t - mean(t) - xh mean(t xh)) (+ dres), written as fp32 (dx) and / or bf16
+ * (dx_bf16), all dense [rows, C]; y (optional, needs beta) = bf16(xh gamma + beta), the LayerNorm output again; dgamma = sum dy xh and
+ * dbeta = sum dy (both or neither; overwritten; ws of mfnet_layernorm_ckpt8_workspace_floats). Deterministic: no atomics. */
+int mfnet_layernorm_bwd_ckpt8(const void* dy, int dy_dtype, int64_t lddy, const void* codes, const void* exps, const float* mean,
+                              const float* rstd, const float* gamma, const float* beta, const float* dres, float* dx, void* dx_bf16, void* y,
+                              float* dgamma, float* dbeta, float* ws, int64_t ws_floats, int64_t rows, int64_t C, hipStream_t stream);
+int64_t mfnet_layernorm_ckpt8_workspace_floats(int64_t rows, int64_t C);
+
+/* ---- A pool of n low-rank adapters beside one frozen projection: row m takes adapter ids[m] (int32 on the device; none if it lies
+ * outside [0, n)), the rows of a call in any order (loralib/layers.py:149-165 has one adapter per modality and call).
+ * Factors are bf16 images padded to RP = 16, 32 or 64 ranks: a "down" image [n][RP][C] (the product contracts over C) and an "up" image
+ * [n][C][RP] (it contracts over the ranks); pack writes either or both from A [n][r][C] (long_first = 0) or B [n][C][r]
+ * (long_first = 1), fp32 or bf16. All long axes are multiples of 8, rows 16-byte aligned with strides that are multiples of 8;
+ * M < 2^31 - 256, n <= 65535. No call synchronises, allocates or uses atomics; the same inputs give the same bits. */
+int mfnet_lora_pool_pack(const void* src, int dtype, int long_first, int64_t n, int64_t C, int r, int RP, void* down, void* up,
+                         hipStream_t stream);
+/* Rows grouped by adapter, ascending inside each: offs [n + 1], perm [M], and chunks of rows for the backward sums: base [n + 1], table
+ * [4 * mfnet_lora_pool_chunks(M, n)] int32 (16-byte aligned). Depends on ids alone: one per batch serves all of its layers. */
+int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* offs, int* perm, int* base, int* table, hipStream_t stream);
+int64_t mfnet_lora_pool_chunks(int64_t M, int64_t n);
+/* out [M, RP] fp32 = scale[i] * down_i x_m (zeros for rows without an adapter). */
+int mfnet_lora_pool_down(const void* X, int64_t ldx, const void* down, const float* scale, const int* ids, int64_t n, int RP, float* out,
+                         int64_t M, int64_t K, hipStream_t stream);
+/* out = X W^T (+ bias) (+ up_i D_m, with D the fp32 [M, RP] of mfnet_lora_pool_down); W bf16 [N, K], out bf16 | fp32 [M, N].
+ * D = NULL: the projection alone. */
+int mfnet_lora_pool_gemm(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* D, const void* up,
+                         const int* ids, int64_t n, int RP, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K,
+                         hipStream_t stream);
+/* Per adapter the sum over its rows of y_m U_m^T, y bf16 (Y) or an 8-bit checkpoint (codes, exps; dense), U fp32 [M, RP]: out fp32
+ * [n][C][r], or [n][r][C] with rank_major. Overwritten; adapters without rows get zeros. ws of mfnet_lora_pool_tn_workspace_floats. */
+int mfnet_lora_pool_tn(const void* Y, int64_t ldy, const void* codes, const void* exps, const float* U, int RP, const int* perm,
+                       const int* base, const int* table, int64_t M, int64_t n, int64_t C, int r, int rank_major, float* out, float* ws,
+                       int64_t ws_floats, hipStream_t stream);
+int64_t mfnet_lora_pool_tn_workspace_floats(int64_t M, int64_t n, int64_t C, int RP);
+
 #ifdef __cplusplus
 }
 #endif

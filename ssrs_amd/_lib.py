@@ -128,6 +128,26 @@ _SIGS = {
     "mfnet_gla_attn_bwd_f32": [P, P, P, P, P, I64, I64, I64, I64, I64, I64, F, P],
     "mfnet_up_final_bwd_f32": [P, P, I64, I64, I64, I64, I64, I64, P],
     "mfnet_adapter_mix_bwd_f32": [P, P, P, P, P, P, I64, I64, P],
+    # ---- 8-bit activation checkpoints (csrc/ckpt8.hip)
+    "mfnet_ckpt8_pack": [P, I, I64, P, P, I64, I64, P],
+    "mfnet_ckpt8_unpack": [P, P, P, I, I64, I64, I64, P],
+    "mfnet_gelu_fwd_ckpt8": [P, I, I64, P, I64, P, P, I64, I64, P],
+    "mfnet_gelu_bwd_ckpt8": [P, P, P, I, I64, P, P, I64, I64, I64, P],
+    "mfnet_layernorm_fwd_ckpt8": [P, I, I64, P, P, P, P, P, P, P, I64, I64, F, P],
+    "mfnet_layernorm_bwd_ckpt8": [P, I, I64, P, P, P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, P],
+    # ---- pooled low-rank adapters (csrc/lora_pool.hip)
+    "mfnet_lora_pool_pack": [P, I, I, I64, I64, I, I, P, P, P],
+    "mfnet_lora_pool_plan": [P, I64, I64, P, P, P, P, P],
+    "mfnet_lora_pool_down": [P, I64, P, P, P, I64, I, P, I64, I64, P],
+    "mfnet_lora_pool_gemm": [P, I64, P, I64, P, P, P, P, I64, I, P, I, I64, I64, I64, I64, P],
+    "mfnet_lora_pool_tn": [P, I64, P, P, P, I, P, P, P, I64, I64, I64, I, I, P, P, I64, P],
+}
+
+# host-side size helpers: name -> (restype, argtypes)
+_HELPERS = {
+    "mfnet_layernorm_ckpt8_workspace_floats": (c_int64, [I64, I64]),
+    "mfnet_lora_pool_chunks": (c_int64, [I64, I64]),
+    "mfnet_lora_pool_tn_workspace_floats": (c_int64, [I64, I64, I64, I]),
 }
 
 
@@ -155,6 +175,8 @@ def lib():
         L.mfnet_attn_bwd_workspace_floats.argtypes = [c_int64, c_int64, c_int64, c_int64, c_int64]
         L.mfnet_attn_f32_bwd_workspace_floats.restype = c_int64
         L.mfnet_attn_f32_bwd_workspace_floats.argtypes = [c_int64, c_int64, c_int64, c_int64, c_int64]
+        for name, (res, sig) in _HELPERS.items():
+            getattr(L, name).restype, getattr(L, name).argtypes = res, sig
         for name, sig in _SIGS.items():
             fn = getattr(L, name, None)
             if fn is None:
@@ -167,7 +189,7 @@ def lib():
 
 def exported_symbols():
     return ["mfnet_version", "mfnet_last_error", "mfnet_skinny_tn_workspace_floats", "mfnet_gemm_tn_splits", "mfnet_colreduce_workspace_floats",
-            "mfnet_attn_bwd_workspace_floats", "mfnet_lora_side_splits", "mfnet_attn_f32_bwd_workspace_floats"] + list(_SIGS)
+            "mfnet_attn_bwd_workspace_floats", "mfnet_lora_side_splits", "mfnet_attn_f32_bwd_workspace_floats"] + list(_HELPERS) + list(_SIGS)
 
 
 def call(name: str, *args):
