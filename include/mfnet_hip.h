@@ -536,29 +536,29 @@ int64_t mfnet_layernorm_ckpt8_workspace_floats(int64_t rows, int64_t C);
 /* ---- A pool of n low-rank adapters beside one frozen projection: row m takes adapter ids[m] (int32 on the device; none if it lies
  * outside [0, n)), the rows of a call in any order (loralib/layers.py:149-165 has one adapter per modality and call).
  * Factors are bf16 images padded to RP = 16, 32 or 64 ranks: a "down" image [n][RP][C] (the product contracts over C) and an "up" image
- * [n][C][RP] (it contracts over the ranks); pack writes either or both from A [n][r][C] (long_first = 0) or B [n][C][r]
- * (long_first = 1), fp32 or bf16. All long axes are multiples of 8, rows 16-byte aligned with strides that are multiples of 8;
- * M < 2^31 - 256, n <= 65535. No call synchronises, allocates or uses atomics; the same inputs give the same bits. */
-int mfnet_lora_pool_pack(const void* src, int dtype, int long_first, int64_t n, int64_t C, int r, int RP, void* down, void* up,
-                         hipStream_t stream);
+ * [n][C][RP] (it contracts over the ranks) of each; pack writes all four from A [n][r][K] and B [n][N][r], fp32 or bf16. K and N are
+ * multiples of 8, rows 16-byte aligned with strides that are multiples of 8; M < 2^31 - 256, n <= 65535. No call synchronises,
+ * allocates or uses atomics; the same inputs give the same bits. An adapter's or a row's infinities and NaN reach only the rows of that
+ * adapter, or that row, and their gradients. */
+int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, int64_t n, int64_t K, int64_t N, int r, int RP, void* a_down, void* a_up,
+                         void* b_down, void* b_up, hipStream_t stream);
 /* Rows grouped by adapter, ascending inside each: offs [n + 1], perm [M], and chunks of rows for the backward sums: base [n + 1], table
  * [4 * mfnet_lora_pool_chunks(M, n)] int32 (16-byte aligned). Depends on ids alone: one per batch serves all of its layers. */
 int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* offs, int* perm, int* base, int* table, hipStream_t stream);
 int64_t mfnet_lora_pool_chunks(int64_t M, int64_t n);
-/* out [M, RP] fp32 = scale[i] * down_i x_m (zeros for rows without an adapter). */
-int mfnet_lora_pool_down(const void* X, int64_t ldx, const void* down, const float* scale, const int* ids, int64_t n, int RP, float* out,
-                         int64_t M, int64_t K, hipStream_t stream);
-/* out = X W^T (+ bias) (+ up_i D_m, with D the fp32 [M, RP] of mfnet_lora_pool_down); W bf16 [N, K], out bf16 | fp32 [M, N].
- * D = NULL: the projection alone. */
-int mfnet_lora_pool_gemm(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* D, const void* up,
-                         const int* ids, int64_t n, int RP, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K,
-                         hipStream_t stream);
-/* Per adapter the sum over its rows of y_m U_m^T, y bf16 (Y) or an 8-bit checkpoint (codes, exps; dense), U fp32 [M, RP]: out fp32
- * [n][C][r], or [n][r][C] with rank_major. Overwritten; adapters without rows get zeros. ws of mfnet_lora_pool_tn_workspace_floats. */
-int mfnet_lora_pool_tn(const void* Y, int64_t ldy, const void* codes, const void* exps, const float* U, int RP, const int* perm,
-                       const int* base, const int* table, int64_t M, int64_t n, int64_t C, int r, int rank_major, float* out, float* ws,
-                       int64_t ws_floats, hipStream_t stream);
-int64_t mfnet_lora_pool_tn_workspace_floats(int64_t M, int64_t n, int64_t C, int RP);
+/* down [M, RP] fp32 = scale[i] * A_i x_m (zeros for rows without an adapter; the backward pass reads it),
+ * out [M, N] bf16 | fp32 = x W^T (+ bias) + B_i down; X bf16 [M, K], W bf16 [N, K], bias fp32 [N] or NULL. */
+int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* scale, const void* a_down,
+                        const void* b_up, const int* ids, int64_t n, int RP, float* down, void* out, int out_dtype, int64_t ldo, int64_t M,
+                        int64_t N, int64_t K, hipStream_t stream);
+/* With p_m = scale[i] * B_i^T dy_m: dx [M, K] bf16 = dy Wt^T + A_i^T p (Wt bf16 [K, N]; dx = NULL: left out), dA [n][r][K] = sum over the
+ * adapter's rows of p x^T, dB [n][N][r] = sum of dy down^T, fp32, overwritten; adapters without rows get zeros. x is the forward's input
+ * as bf16 rows (X) or its 8-bit checkpoint (codes, exps; dense), one of the two. */
+int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, int64_t ldx, const void* codes, const void* exps, const void* Wt, int64_t ldwt,
+                        const float* scale, const void* b_down, const void* a_up, const int* ids, const int* perm, const int* base,
+                        const int* table, int64_t n, int r, int RP, const float* down, void* dx, int64_t lddx, float* dA, float* dB, float* ws,
+                        int64_t ws_floats, int64_t M, int64_t N, int64_t K, hipStream_t stream);
+int64_t mfnet_lora_pool_bwd_workspace_floats(int64_t M, int64_t n, int64_t K, int64_t N, int RP);
 
 #ifdef __cplusplus
 }

@@ -136,18 +136,17 @@ _SIGS = {
     "mfnet_layernorm_fwd_ckpt8": [P, I, I64, P, P, P, P, P, P, P, I64, I64, F, P],
     "mfnet_layernorm_bwd_ckpt8": [P, I, I64, P, P, P, P, P, P, P, P, P, P, P, P, P, I64, I64, I64, P],
     # ---- pooled low-rank adapters (csrc/lora_pool.hip)
-    "mfnet_lora_pool_pack": [P, I, I, I64, I64, I, I, P, P, P],
+    "mfnet_lora_pool_pack": [P, P, I, I64, I64, I64, I, I, P, P, P, P, P],
     "mfnet_lora_pool_plan": [P, I64, I64, P, P, P, P, P],
-    "mfnet_lora_pool_down": [P, I64, P, P, P, I64, I, P, I64, I64, P],
-    "mfnet_lora_pool_gemm": [P, I64, P, I64, P, P, P, P, I64, I, P, I, I64, I64, I64, I64, P],
-    "mfnet_lora_pool_tn": [P, I64, P, P, P, I, P, P, P, I64, I64, I64, I, I, P, P, I64, P],
+    "mfnet_lora_pool_fwd": [P, I64, P, I64, P, P, P, P, P, I64, I, P, P, I, I64, I64, I64, I64, P],
+    "mfnet_lora_pool_bwd": [P, I64, P, I64, P, P, P, I64, P, P, P, P, P, P, P, I64, I, I, P, P, I64, P, P, P, I64, I64, I64, I64, P],
 }
 
 # host-side size helpers: name -> (restype, argtypes)
 _HELPERS = {
     "mfnet_layernorm_ckpt8_workspace_floats": (c_int64, [I64, I64]),
     "mfnet_lora_pool_chunks": (c_int64, [I64, I64]),
-    "mfnet_lora_pool_tn_workspace_floats": (c_int64, [I64, I64, I64, I]),
+    "mfnet_lora_pool_bwd_workspace_floats": (c_int64, [I64, I64, I64, I64, I]),
 }
 
 
@@ -193,7 +192,7 @@ def exported_symbols():
 
 
 def call(name: str, *args):
-    L = lib()
+    L = _lib or lib()
     rc = getattr(L, name)(*args)
     if rc != 0:
         raise MfnetError(f"{name} failed ({rc}): {L.mfnet_last_error().decode()}")

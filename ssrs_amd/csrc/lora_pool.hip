@@ -14,6 +14,8 @@
 // A workgroup that meets rows of several adapters multiplies all its rows with each adapter in turn and SELECTS the rows it belongs to:
 // a sum of zeros would let one adapter's infinities and NaN into another request's rows.
 #include "ckpt8.h"
+#include <math.h>
+#include <type_traits>
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* gbl_ptr_t;
@@ -52,31 +54,31 @@ __device__ __forceinline__ int next_id(int cand) {
 #define NO_ID 0x7fffffff
 
 // ------------------------------------------------------------------------------------------------ images
-// long_first: src [n][C][r] (B), else src [n][r][C] (A). One thread per (adapter, position on the long axis).
-template <typename T, bool LONG_FIRST>
-__global__ __launch_bounds__(256) void pool_pack_kernel(const T* __restrict__ src, int C, int r, int RP, bf16_t* __restrict__ down, bf16_t* __restrict__ up) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
+// One thread per (adapter, position on the long axis) writes both images of a factor: blockIdx.z 0: A [n][r][K], 1: B [n][N][r].
+struct PoolPack { const void* src[2]; bf16_t* down[2]; bf16_t* up[2]; int C[2], r, RP; };
+template <typename T>
+__global__ __launch_bounds__(256) void pool_pack_kernel(const PoolPack p) {
+  const int z = blockIdx.z, c = blockIdx.x * 256 + threadIdx.x, C = p.C[z], r = p.r, RP = p.RP;
   const int64_t i = blockIdx.y;
   if (c >= C) return;
-  const T* s = src + i * (int64_t)C * r;
+  const T* s = (const T*)p.src[z] + i * (int64_t)C * r;
   for (int j0 = 0; j0 < RP; j0 += 8) {
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int k = j0 + j;
+      v[j] = 0.f;
       if (k < r) {
-        const T t = LONG_FIRST ? s[(int64_t)c * r + k] : s[(int64_t)k * C + c];
+        const T t = z ? s[(int64_t)c * r + k] : s[(int64_t)k * C + c];
         if constexpr (sizeof(T) == 4) v[j] = t; else v[j] = bf16_to_f32(t);
-      } else v[j] = 0.f;
+      }
     }
     Frag f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) f.w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-    if (up) *reinterpret_cast<u32x4_t*>(up + (i * C + c) * RP + j0) = f.q;
-    if (down) {
+    *reinterpret_cast<u32x4_t*>(p.up[z] + (i * C + c) * RP + j0) = f.q;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) down[(i * RP + j0 + j) * C + c] = (bf16_t)(f.w[j >> 1] >> (16 * (j & 1)));
-    }
+    for (int j = 0; j < 8; ++j) p.down[z][(i * RP + j0 + j) * C + c] = (bf16_t)(f.w[j >> 1] >> (16 * (j & 1)));
   }
 }
 
@@ -138,7 +140,7 @@ __global__ __launch_bounds__(256) void pool_chunks_kernel(const int* __restrict_
 }
 
 // ------------------------------------------------------------------------------------------------ down: s_i F_i y_m
-// 16 rows per workgroup, the four waves take every fourth 32-wide k-step. The factor is the MFMA's "A" operand, the rows its "B"
+// 16 rows per workgroup, the four waves take every fourth 128-wide piece of K. The factor is the MFMA's "A" operand, the rows its "B"
 // operand, so a lane ends with four consecutive ranks of row fr. Bound by reading the rows once (the factors come from L2).
 template <int NR>      // RP / 16
 __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
@@ -153,7 +155,6 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
   f32x4_t sel[NR];
 #pragma unroll
   for (int f = 0; f < NR; ++f) sel[f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  const int nks = (K + 31) / 32;
   for (int last = -1;;) {
     const int cur = next_id(id > last ? id : NO_ID);
     if (cur == NO_ID) break;
@@ -162,15 +163,20 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
     f32x4_t acc[NR];
 #pragma unroll
     for (int f = 0; f < NR; ++f) acc[f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int ks = wave; ks < nks; ks += 4) {
-      Frag x, a[NR];
-      const bool on = 32 * ks + 8 * fq < K;               // chunks behind the last column are zeros on both sides
-      x.q = on ? *reinterpret_cast<const u32x4_t*>(xp + 32 * ks) : (u32x4_t){0u, 0u, 0u, 0u};
+    for (int k0 = 128 * wave; k0 < K; k0 += 512) {          // four k-steps in flight
+      Frag x[4], a[4][NR];
 #pragma unroll
-      for (int f = 0; f < NR; ++f) a[f].q = on ? *reinterpret_cast<const u32x4_t*>(fp + (int64_t)16 * f * K + 32 * ks) : (u32x4_t){0u, 0u, 0u, 0u};
+      for (int j = 0; j < 4; ++j) {
+        const int k = k0 + 32 * j;
+        const bool on = k + 8 * fq < K;                     // chunks behind the last column are zeros on both sides
+        x[j].q = on ? *reinterpret_cast<const u32x4_t*>(xp + k) : (u32x4_t){0u, 0u, 0u, 0u};
 #pragma unroll
-      for (int f = 0; f < NR; ++f) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[f].v, x.v, acc[f], 0, 0, 0);
+        for (int f = 0; f < NR; ++f) a[j][f].q = on ? *reinterpret_cast<const u32x4_t*>(fp + (int64_t)16 * f * K + k) : (u32x4_t){0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int f = 0; f < NR; ++f) acc[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][f].v, x[j].v, acc[f], 0, 0, 0);
     }
 #pragma unroll
     for (int f = 0; f < NR; ++f)
@@ -194,6 +200,40 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
   }
 }
 
+// Few rows, an adapter each as it may be: one row per workgroup, RP / 4 ranks per wave, 8 elements per lane and request. All requests of
+// a row are independent of each other, where the kernel above would take the adapters of its 16 rows one after the other.
+template <int NR>
+__global__ __launch_bounds__(256) void pool_down_row_kernel(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
+                                                            const int* __restrict__ ids, int n, float* __restrict__ out, int K) {
+  constexpr int R = 4 * NR;                                  // ranks of a wave
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t m = blockIdx.x;
+  const int id = ids[m];
+  float s[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) s[j] = 0.f;
+  const bool on = (unsigned)id < (unsigned)n;
+  if (on) {
+    const bf16_t* f = F + ((int64_t)id * 16 * NR + R * wave) * K;
+    for (int c = 8 * lane; c < K; c += 512) {
+      const u32x4_t x = *reinterpret_cast<const u32x4_t*>(X + m * ldx + c);
+      u32x4_t a[R];
+#pragma unroll
+      for (int j = 0; j < R; ++j) a[j] = *reinterpret_cast<const u32x4_t*>(f + (int64_t)j * K + c);
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[j] = fmaf(bf16_lo(x[q]), bf16_lo(a[j][q]), fmaf(bf16_hi(x[q]), bf16_hi(a[j][q]), s[j]));
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < R; ++j) s[j] = wave_sum(s[j]);
+  float v = 0.f;
+#pragma unroll
+  for (int j = 0; j < R; ++j) v = lane == j ? s[j] : v;
+  if (lane < R) out[m * (16 * NR) + R * wave + lane] = on ? scale[id] * v : 0.f;
+}
+
 // ------------------------------------------------------------------------------------------------ out = X W^T + bias + Up_i down
 struct PoolGemm {
   const bf16_t* X; int64_t ldx; const bf16_t* W; int64_t ldw; const float* bias;
@@ -202,9 +242,201 @@ struct PoolGemm {
   int64_t M; int N, K, tiles_m, tiles_n;
 };
 
-// chunk XOR of W row o of a wave's columns: conflict-free ds_read_b128 for the permuted row sets (G fragments per group)
-template <int G> __device__ __forceinline__ int pool_swz_w(int o) {
-  return G == 4 ? ((((o >> 4) & 3) << 1) | ((o >> 1) & 1)) : ((((o >> 3) & 3) << 1) | ((o >> 1) & 1));
+// Column order inside a wave's 16 G columns: fragment i, operand row fr <-> column 4 G (fr >> 2) + 4 i + (fr & 3), so that a lane ends
+// with 4 G consecutive columns. Chunk XOR of that column's LDS row: the 16 rows of a fragment fall on 16 different 16-byte slots.
+template <int G> __device__ __forceinline__ int pool_col(int fr, int i) { return 4 * G * (fr >> 2) + 4 * i + (fr & 3); }
+template <int G> __device__ __forceinline__ int pool_swz_w(int o) { return ((o / (4 * G)) << 1) | ((o >> 1) & 1); }
+
+// Low-rank update, bias and store of a wave's tile: the lane owns rows m0 + r0 + 16 b and columns ncol + 4 G fq .. + 4 G - 1 (rows past
+// the end repeat the last one and are not stored). The update is MFMA k-steps of 32 slots: RP = 16: ranks 0..15 of the factor's part hi,
+// then of its part lo; wider: 32 ranks of one part. A bf16 result needs 16 bits of the fp32 factor (hi + lo), an fp32 one a third part.
+template <int XF, int G>
+__device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[G][XF], int64_t m0, int r0, int ncol, int fr, int fq) {
+  const int mlim = p.M - m0 - 1 < r0 + 16 * XF ? (int)(p.M - m0) - 1 : r0 + 16 * XF;       // last row of the matrix, from m0
+  if (p.D) {
+    const int* ids = p.ids + m0;
+    const int RP = p.RP;
+    const float* D = p.D + m0 * RP;
+    int id[XF];
+#pragma unroll
+    for (int b = 0; b < XF; ++b) {
+      const int r = r0 + 16 * b;
+      id[b] = ids[r < mlim ? r : mlim];
+      if ((unsigned)id[b] >= (unsigned)p.n) id[b] = -1;
+    }
+    const bool wide = RP > 16;
+    const int parts = p.out_f32 ? 3 : 2, steps = wide ? parts * (RP / 32) : parts - 1;
+    for (int s = 0; s < steps; ++s) {
+      const int rk = wide ? 32 * (s / parts) + 8 * fq : 8 * (fq & 1);
+      const int part = wide ? s % parts : 2 * s + (fq >> 1);               // 3: none
+      Frag u[XF];
+#pragma unroll
+      for (int b = 0; b < XF; ++b) {
+        const int r = r0 + 16 * b;
+        const float4* d = reinterpret_cast<const float4*>(D + ((r < mlim ? r : mlim) * RP + rk));
+        const float4 d0 = d[0], d1 = d[1];
+        const float x[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned int hi = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+          const float e0 = x[2 * i] - bf16_lo(hi), e1 = x[2 * i + 1] - bf16_hi(hi);
+          const unsigned int lo = pack_bf16x2(e0, e1), l2 = pack_bf16x2(e0 - bf16_lo(lo), e1 - bf16_hi(lo));
+          u[b].w[i] = part == 0 ? hi : (part == 1 ? lo : (part == 2 ? l2 : 0u));
+        }
+      }
+      for (int last = -1;;) {
+        int cand = NO_ID;
+#pragma unroll
+        for (int b = 0; b < XF; ++b) cand = id[b] > last && id[b] < cand ? id[b] : cand;
+        const int cur = next_id(cand);
+        if (cur == NO_ID) break;
+        last = cur;
+        const bf16_t* up = p.Up + (int64_t)cur * p.N * RP;
+        Frag f[G];
+#pragma unroll
+        for (int a = 0; a < G; ++a) {
+          const int c = ncol + pool_col<G>(fr, a);
+          f[a].q = *reinterpret_cast<const u32x4_t*>(up + ((int64_t)(c < p.N ? c : p.N - 1) * RP + rk));
+        }
+#pragma unroll
+        for (int b = 0; b < XF; ++b)
+#pragma unroll
+          for (int a = 0; a < G; ++a) {
+            const f32x4_t t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[a].v, u[b].v, acc[a][b], 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[a][b][r] = id[b] == cur ? t[r] : acc[a][b][r];
+          }
+      }
+    }
+  }
+  const int cb = ncol + 4 * G * fq;
+  float bv[4 * G];
+#pragma unroll
+  for (int a = 0; a < G; ++a) {
+    const float4 b4 = p.bias && cb + 4 * a < p.N ? *reinterpret_cast<const float4*>(p.bias + cb + 4 * a) : make_float4(0.f, 0.f, 0.f, 0.f);
+    bv[4 * a] = b4.x; bv[4 * a + 1] = b4.y; bv[4 * a + 2] = b4.z; bv[4 * a + 3] = b4.w;
+  }
+  if (p.out_f32) {
+    float* out = (float*)p.out + (m0 + r0) * p.ldo + cb;
+#pragma unroll
+    for (int b = 0; b < XF; ++b) {
+      if (r0 + 16 * b > mlim) continue;
+      float* o = out + 16 * b * p.ldo;
+#pragma unroll
+      for (int a = 0; a < G; ++a)
+        if (cb + 4 * a < p.N)
+          *reinterpret_cast<float4*>(o + 4 * a) = make_float4(acc[a][b][0] + bv[4 * a], acc[a][b][1] + bv[4 * a + 1], acc[a][b][2] + bv[4 * a + 2], acc[a][b][3] + bv[4 * a + 3]);
+    }
+  } else {
+    bf16_t* out = (bf16_t*)p.out + (m0 + r0) * p.ldo + cb;
+#pragma unroll
+    for (int b = 0; b < XF; ++b) {
+      if (r0 + 16 * b > mlim) continue;
+      bf16_t* o = out + 16 * b * p.ldo;
+      u32x2_t w[G];
+#pragma unroll
+      for (int a = 0; a < G; ++a) {
+        w[a].x = pack_bf16x2(acc[a][b][0] + bv[4 * a], acc[a][b][1] + bv[4 * a + 1]);
+        w[a].y = pack_bf16x2(acc[a][b][2] + bv[4 * a + 2], acc[a][b][3] + bv[4 * a + 3]);
+      }
+      if (G & 1) {                                           // 24 bytes per lane: 8-byte pieces
+#pragma unroll
+        for (int a = 0; a < G; ++a)
+          if (cb + 4 * a < p.N) *reinterpret_cast<u32x2_t*>(o + 4 * a) = w[a];
+      } else {
+#pragma unroll
+        for (int a = 0; a + 1 < G; a += 2)
+          if (cb + 4 * a < p.N) *reinterpret_cast<u32x4_t*>(o + 4 * a) = (u32x4_t){w[a].x, w[a].y, w[a + 1].x, w[a + 1].y};
+      }
+    }
+  }
+}
+
+// Few rows (M <= 16 XF): 16 columns per workgroup, the four waves take every fourth 64-wide piece of K and add up through LDS: the
+// weight is streamed once and every request of a wave is independent. Bound by latency. The low-rank update needs no matrix
+// instruction here: a lane owns one row and four columns, whose RP factors lie in one piece; they are requested before the products.
+template <int XF>
+__global__ __launch_bounds__(256) void pool_gemm_rows_kernel(const PoolGemm p) {
+  __shared__ f32x4_t red[4][XF][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int fr = lane & 15, fq = lane >> 4;
+  const int n0 = blockIdx.x * 16, K = p.K, M = (int)p.M;
+  const int mf = 16 * wave + fr, cb = n0 + 4 * fq;           // the row and columns this lane finishes (waves below XF)
+  const bool fin = wave < XF && mf < M && cb < p.N;
+  float add[4] = {0.f, 0.f, 0.f, 0.f};
+  if (fin && p.bias) {
+    const float4 b = *reinterpret_cast<const float4*>(p.bias + cb);
+    add[0] = b.x; add[1] = b.y; add[2] = b.z; add[3] = b.w;
+  }
+  if (fin && p.D) {
+    const int id = p.ids[mf];
+    if ((unsigned)id < (unsigned)p.n) {
+      const int RP = p.RP;
+      const bf16_t* up = p.Up + ((int64_t)id * p.N + cb) * RP;
+      const float* d = p.D + (int64_t)mf * RP;
+      float lr[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < RP; j += 8) {
+        const float4 d0 = *reinterpret_cast<const float4*>(d + j), d1 = *reinterpret_cast<const float4*>(d + j + 4);
+        const float x[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const u32x4_t u = *reinterpret_cast<const u32x4_t*>(up + (int64_t)c * RP + j);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) lr[c] = fmaf(x[2 * q], bf16_lo(u[q]), fmaf(x[2 * q + 1], bf16_hi(u[q]), lr[c]));
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) add[c] += lr[c];
+    }
+  }
+  const bf16_t* w = p.W + (int64_t)(n0 + fr < p.N ? n0 + fr : p.N - 1) * p.ldw + 8 * fq;
+  const bf16_t* x[XF];
+#pragma unroll
+  for (int b = 0; b < XF; ++b) x[b] = p.X + (int64_t)(16 * b + fr < M ? 16 * b + fr : M - 1) * p.ldx + 8 * fq;
+  f32x4_t acc[XF];
+#pragma unroll
+  for (int b = 0; b < XF; ++b) acc[b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  const u32x4_t zero = (u32x4_t){0u, 0u, 0u, 0u};
+  for (int k0 = 64 * wave; k0 < K; k0 += 256 * 2) {          // two pieces of 64 in flight
+    Frag wf[4], xf[4][XF];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + 256 * (j >> 1) + 32 * (j & 1);
+      const bool on = k + 8 * fq < K;                        // chunks behind column K: zeros on both sides
+      wf[j].q = on ? *reinterpret_cast<const u32x4_t*>(w + k) : zero;
+#pragma unroll
+      for (int b = 0; b < XF; ++b) xf[j][b].q = on ? *reinterpret_cast<const u32x4_t*>(x[b] + k) : zero;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int b = 0; b < XF; ++b) acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j].v, xf[j][b].v, acc[b], 0, 0, 0);
+  }
+#pragma unroll
+  for (int b = 0; b < XF; ++b) red[wave][b][lane] = acc[b];
+  __syncthreads();
+  if (!fin) return;
+  const f32x4_t t = (red[0][wave][lane] + red[1][wave][lane]) + (red[2][wave][lane] + red[3][wave][lane]);
+  const int64_t at = (int64_t)mf * p.ldo + cb;
+  if (p.out_f32) *reinterpret_cast<float4*>((float*)p.out + at) = make_float4(t[0] + add[0], t[1] + add[1], t[2] + add[2], t[3] + add[3]);
+  else {
+    u32x2_t o;
+    o.x = pack_bf16x2(t[0] + add[0], t[1] + add[1]);
+    o.y = pack_bf16x2(t[2] + add[2], t[3] + add[3]);
+    *reinterpret_cast<u32x2_t*>((bf16_t*)p.out + at) = o;
+  }
+}
+
+// Workgroup -> tile. Workgroup ids go round-robin over the 8 XCDs: each XCD takes a contiguous run of tiles, and a run walks down 4
+// tile rows before it moves to the next column, so that the 32 tiles an XCD holds at a time share 4 + 8 panels in its L2 (32 tiles of
+// one tile row: 1 + 32).
+__device__ __forceinline__ void pool_tile(const PoolGemm& p, int* tm, int* tn) {
+  const int nwg = p.tiles_m * p.tiles_n, orig = blockIdx.x, xcd = orig & 7, q = nwg >> 3, r = nwg & 7;
+  const int wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (orig >> 3);
+  const int per = 4 * p.tiles_n, g = wg / per, rem = wg - g * per;
+  const int rows = p.tiles_m - 4 * g < 4 ? p.tiles_m - 4 * g : 4;
+  *tm = 4 * g + rem % rows;
+  *tn = rem / rows;
 }
 
 // WM x WN waves, each 16 XF rows x 16 G columns; k-tiles of 64 in two LDS buffers filled by global_load_lds. The W rows are the MFMA's
@@ -218,14 +450,8 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void pool_gemm_kernel(
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int fr = lane & 15, fq = lane >> 4;
-  // XCD-aware: workgroup ids go round-robin over the 8 XCDs; each XCD walks a contiguous run of tiles
-  const int nwg = p.tiles_m * p.tiles_n;
-  int wg;
-  {
-    const int orig = blockIdx.x, xcd = orig & 7, q = nwg >> 3, r = nwg & 7;
-    wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (orig >> 3);
-  }
-  const int tm = wg / p.tiles_n, tn = wg - tm * p.tiles_n;
+  int tm, tn;
+  pool_tile(p, &tm, &tn);
   const int64_t m0 = (int64_t)tm * BM;
   const int n0 = tn * BN;
 
@@ -262,7 +488,7 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void pool_gemm_kernel(
   x_sw = fr & 7;
 #pragma unroll
   for (int i = 0; i < G; ++i) {
-    const int o = 4 * G * (fr >> 2) + 4 * i + (fr & 3);
+    const int o = pool_col<G>(fr, i);
     w_off[i] = (BM + wn * 16 * G + o) * 128;
     w_sw[i] = pool_swz_w<G>(o);
   }
@@ -299,97 +525,198 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void pool_gemm_kernel(
     asm volatile("" ::: "memory");
   }
 
-  // ---- epilogue: lane owns rows m0 + wm*16*XF + 16 b + fr and columns cb .. cb + 4G - 1
-  const int64_t mw = m0 + wm * 16 * XF + fr;
-  const int ncol = n0 + wn * 16 * G;
-  if (p.D) {
-    int id[XF];
+  pool_epilogue<XF, G>(p, acc, m0, wm * 16 * XF + fr, n0 + wn * 16 * G, fr, fq);
+}
+
+// The same product for many rows: 8 waves as 2 (rows) x 4 (columns), wave tile 16 XF x 16 G, two k-tiles of 64 in LDS. A k-tile is
+// four phases, one quadrant of the wave's tile each (half the row fragments x half the column fragments x both k-steps):
+//
+//   phase 0  reads x-lo, w-lo     multiplies x-lo w-lo      requests x-hi of tile t + 1
+//   phase 1  reads w-hi           multiplies x-lo w-hi      requests x-lo of tile t + 2
+//   phase 2  reads x-hi           multiplies x-hi w-hi      requests half of W of tile t + 2
+//   phase 3                       multiplies x-hi w-lo      requests the rest of W of tile t + 2
+//
+// Each phase is a read slot and a multiply slot with a barrier behind each; the waves of the second row half run one slot late, so
+// that on every SIMD one of its two waves multiplies while the other reads. A request overwrites only what both halves have read (waited
+// for by lgkmcnt(0) inside the read slot, published by its barrier) at least one slot earlier. vmcnt counts in order: at the end of
+// phase 3's read slot the requests younger than W of tile t + 1 may be in flight, at the end of phase 1's those younger than x-hi of
+// this tile. Addresses: a fragment's LDS address is one of four lane addresses plus a constant, a request's global one a constant
+// 32-bit offset beside a scalar that advances by 128 bytes a tile, so that the loop has next to no vector instructions beside the MFMAs.
+template <int XF, int G>
+__global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_kernel(const PoolGemm p) {
+  constexpr int BM = 32 * XF, BN = 64 * G, STAGE = (BM + BN) * 128;
+  constexpr int XH = XF / 2, GL = (G + 1) / 2;               // fragments of a row half; column fragments of the first half
+  constexpr int XP = XF / 4, WP = G, W0 = (G + 1) / 2;       // requests per wave: a row half, all of W, its first part
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3;
+  const int fr = lane & 15, fq = lane >> 4;
+  int tm, tn;
+  pool_tile(p, &tm, &tn);
+  const int64_t m0 = (int64_t)tm * BM;
+  const int n0 = tn * BN;
+
+  // Requests: 1-KB pieces of 8 rows; byte offsets from the tile's first row fit 31 bits (row strides up to 2^22 elements). A row half
+  // (lo / hi) holds rows wm * 16 XF + half * 8 XF ... of both wave rows: 2 XF pieces, XP per wave. W: 8 G pieces, G per wave.
+  const int mlim = p.M - m0 < BM ? (int)(p.M - m0) - 1 : BM - 1, nlim = p.N - n0 < BN ? p.N - n0 - 1 : BN - 1;
+  const bf16_t* xbase = p.X + m0 * p.ldx;
+  const bf16_t* wbase = p.W + (int64_t)n0 * p.ldw;
+#if defined(__HIP_DEVICE_COMPILE__)                          // (buffer resources are a type of the device pass only)
+  const __amdgpu_buffer_rsrc_t xres = __builtin_amdgcn_make_buffer_rsrc((void*)xbase, 0, (int)(mlim * (2 * p.ldx) + 2 * p.K), 0x00020000);
+  const __amdgpu_buffer_rsrc_t wres = __builtin_amdgcn_make_buffer_rsrc((void*)wbase, 0, (int)(nlim * (2 * p.ldw) + 2 * p.K), 0x00020000);
+  int xo[2][XP], wo[WP];
 #pragma unroll
-    for (int b = 0; b < XF; ++b) {
-      const int64_t m = mw + 16 * b;
-      id[b] = m < p.M ? p.ids[m] : -1;
-      if ((unsigned)id[b] >= (unsigned)p.n) id[b] = -1;
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < XP; ++i) {
+      const int j = wave + 8 * i, row = (j / XF) * 16 * XF + h * 8 * XF + (j % XF) * 8 + (lane >> 3);       // piece of the half: XF of them per wave row
+      xo[h][i] = (row < mlim ? row : mlim) * (int)(2 * p.ldx) + (((lane & 7) ^ (row & 7)) << 4);
     }
-    const int RP = p.RP, wide = RP > 16;
-    // k-slots of one MFMA: RP = 16: ranks 0..15 of part hi, then of part lo; wider: 32 ranks of one part
-    const int parts = p.out_f32 ? 3 : 2;                   // a bf16 result needs 16 bits of the product's fp32 factor, an fp32 one all
-    for (int last = -1;;) {
-      int cand = NO_ID;
 #pragma unroll
-      for (int b = 0; b < XF; ++b) cand = id[b] > last && id[b] < cand ? id[b] : cand;
-      const int cur = next_id(cand);
-      if (cur == NO_ID) break;
-      last = cur;
-      bool same = true;
+  for (int i = 0; i < WP; ++i) {
+    const int row = (wave + 8 * i) * 8 + (lane >> 3);
+    wo[i] = (row < nlim ? row : nlim) * (int)(2 * p.ldw) + (((lane & 7) ^ pool_swz_w<G>(row % (16 * G))) << 4);
+  }
+  const int nt = p.K / 64, ragged = p.K & 63;                // whole k-tiles; columns behind them
+  auto req_x = [&](int h, int kt) __attribute__((always_inline)) {
 #pragma unroll
-      for (int b = 0; b < XF; ++b) same = same && (id[b] == cur || mw + 16 * b >= p.M);
-      const bool uniform = __all(same);
-      for (int s = 0; s < (wide ? parts * (RP / 32) : parts - 1); ++s) {
-        const int rk = wide ? 32 * (s / parts) + 8 * fq : 8 * (fq & 1);
-        const int part = wide ? s % parts : 2 * s + (fq >> 1);      // (RP = 16, s = 1: parts 2 and 3; the fourth is left out)
-        Frag up[G];
-#pragma unroll
-        for (int a = 0; a < G; ++a) {
-          int c = ncol + 4 * G * (fr >> 2) + 4 * a + (fr & 3);
-          c = c < p.N ? c : p.N - 1;
-          up[a].q = *reinterpret_cast<const u32x4_t*>(p.Up + ((int64_t)cur * p.N + c) * RP + rk);
-        }
-#pragma unroll
-        for (int b = 0; b < XF; ++b) {
-          const int64_t m = mw + 16 * b < p.M ? mw + 16 * b : p.M - 1;
-          const float4 u0 = *reinterpret_cast<const float4*>(p.D + m * RP + rk), u1 = *reinterpret_cast<const float4*>(p.D + m * RP + rk + 4);
-          const float x[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-          Frag u;
-          if (part == 0) u.v = split_part(x, 0);
-          else if (part == 1) u.v = split_part(x, 1);
-          else if (part == 2) u.v = split_part(x, 2);
-          else u.q = (u32x4_t){0u, 0u, 0u, 0u};
-          if (uniform) {
-#pragma unroll
-            for (int a = 0; a < G; ++a) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(up[a].v, u.v, acc[a][b], 0, 0, 0);
-          } else {
-#pragma unroll
-            for (int a = 0; a < G; ++a) {
-              const f32x4_t t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(up[a].v, u.v, acc[a][b], 0, 0, 0);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) acc[a][b][r] = id[b] == cur ? t[r] : acc[a][b][r];
-            }
-          }
-        }
-      }
+    for (int i = 0; i < XP; ++i) {
+      const int j = wave + 8 * i, row0 = (j / XF) * 16 * XF + h * 8 * XF + (j % XF) * 8;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xres, (lds_ptr_t)(lds + (kt & 1) * STAGE + row0 * 128), 16, xo[h][i], kt * 128, 0, 0);
     }
-  }
-  const int cb = ncol + 4 * G * fq;
-  float bv[4 * G];
+  };
+  auto req_w = [&](int i0, int i1, int kt) __attribute__((always_inline)) {
 #pragma unroll
-  for (int a = 0; a < G; ++a) {
-    const float4 b4 = p.bias && cb + 4 * a < p.N ? *reinterpret_cast<const float4*>(p.bias + cb + 4 * a) : make_float4(0.f, 0.f, 0.f, 0.f);
-    bv[4 * a] = b4.x; bv[4 * a + 1] = b4.y; bv[4 * a + 2] = b4.z; bv[4 * a + 3] = b4.w;
-  }
+    for (int i = 0; i < WP; ++i)
+      if (i >= i0 && i < i1)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(wres, (lds_ptr_t)(lds + (kt & 1) * STAGE + (BM + (wave + 8 * i) * 8) * 128), 16, wo[i], kt * 128, 0, 0);
+  };
+
+  // fragment addresses: both swizzles depend on the lane alone, so a fragment is a constant offset from one address per k-step
+  unsigned int xa[2], wa[2];
 #pragma unroll
-  for (int b = 0; b < XF; ++b) {
-    const int64_t m = mw + 16 * b;
-    if (m >= p.M) continue;
-    if (p.out_f32) {
-      float* o = (float*)p.out + m * p.ldo + cb;
+  for (int ks = 0; ks < 2; ++ks) {
+    const unsigned int l0 = (unsigned int)(uintptr_t)(lds_ptr_t)lds;
+    xa[ks] = l0 + (wm * 16 * XF + fr) * 128 + (((fq + 4 * ks) ^ (fr & 7)) << 4);
+    wa[ks] = l0 + (BM + wn * 16 * G + pool_col<G>(fr, 0)) * 128 + (((fq + 4 * ks) ^ pool_swz_w<G>(pool_col<G>(fr, 0))) << 4);
+  }
+  f32x4_t acc[G][XF];
+#pragma unroll
+  for (int a = 0; a < G; ++a)
+#pragma unroll
+    for (int b = 0; b < XF; ++b) acc[a][b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  bf16x8_t xf[XH][2], wf[G][2];
+  typedef const __attribute__((address_space(3))) bf16x8_t* frag_ptr_t;
+  auto read_x = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < XH; ++i) xf[i][ks] = *(frag_ptr_t)(uintptr_t)(xa[ks] + (h * XH + i) * 2048);
+  };
+  auto read_w = [&](int i0, int i1) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+        if (i >= i0 && i < i1) wf[i][ks] = *(frag_ptr_t)(uintptr_t)(wa[ks] + i * 512);
+  };
+  auto mul = [&](int h, int i0, int i1) __attribute__((always_inline)) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int a = 0; a < G; ++a)
-        if (cb + 4 * a < p.N)
-          *reinterpret_cast<float4*>(o + 4 * a) = make_float4(acc[a][b][0] + bv[4 * a], acc[a][b][1] + bv[4 * a + 1], acc[a][b][2] + bv[4 * a + 2], acc[a][b][3] + bv[4 * a + 3]);
-    } else {
-      bf16_t* o = (bf16_t*)p.out + m * p.ldo + cb;
+        if (a >= i0 && a < i1) {
 #pragma unroll
-      for (int h = 0; h < G / 2; ++h)
-        if (cb + 8 * h < p.N) {
-          u32x4_t w;
-          w.x = pack_bf16x2(acc[2 * h][b][0] + bv[8 * h], acc[2 * h][b][1] + bv[8 * h + 1]);
-          w.y = pack_bf16x2(acc[2 * h][b][2] + bv[8 * h + 2], acc[2 * h][b][3] + bv[8 * h + 3]);
-          w.z = pack_bf16x2(acc[2 * h + 1][b][0] + bv[8 * h + 4], acc[2 * h + 1][b][1] + bv[8 * h + 5]);
-          w.w = pack_bf16x2(acc[2 * h + 1][b][2] + bv[8 * h + 6], acc[2 * h + 1][b][3] + bv[8 * h + 7]);
-          *reinterpret_cast<u32x4_t*>(o + 8 * h) = w;
+          for (int b = 0; b < XH; ++b) acc[a][h * XH + b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[a][ks], xf[b][ks], acc[a][h * XH + b], 0, 0, 0);
         }
-    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  // end of a read slot: this wave's fragments are in registers; end of either slot: barrier
+  auto end_read = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto end_mul = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  if (nt > 0) {
+    req_x(0, 0); req_w(0, WP, 0); req_x(1, 0);
   }
+  if (nt > 1) {
+    req_x(0, 1); req_w(0, WP, 1);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP + WP) : "memory");
+  } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  if (wm) __builtin_amdgcn_s_barrier();                      // the second row half runs one slot late
+  // MORE: two further tiles exist
+  auto tile = [&](auto more, int t) __attribute__((always_inline)) {
+    constexpr bool MORE = decltype(more)::value;
+    read_x(0);
+    read_w(0, GL);
+    if (MORE || t + 1 < nt) req_x(1, t + 1);
+    end_read();
+    mul(0, 0, GL);
+    end_mul();
+    read_w(GL, G);
+    if (MORE) {
+      req_x(0, t + 2);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * XP + WP) : "memory");
+    } else if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    end_read();
+    mul(0, GL, G);
+    end_mul();
+    read_x(1);
+    if (MORE) req_w(0, W0, t + 2);
+    end_read();
+    mul(1, GL, G);
+    end_mul();
+    if (MORE) {
+      req_w(W0, WP, t + 2);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * XP + WP) : "memory");
+    } else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP) : "memory");
+    end_read();
+    mul(1, 0, GL);
+    end_mul();
+  };
+  auto flip = [&](int t) __attribute__((always_inline)) {      // to the other buffer
+    const unsigned int d = t & 1 ? (unsigned int)-STAGE : (unsigned int)STAGE;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) { xa[ks] += d; wa[ks] += d; }
+  };
+  int t = 0;
+  for (; t + 2 < nt; ++t) { tile(std::true_type{}, t); flip(t); }
+  for (; t < nt; ++t) { tile(std::false_type{}, t); flip(t); }
+  if (!wm) __builtin_amdgcn_s_barrier();
+  if (ragged) {                                              // the columns behind the last whole k-tile; zeros behind column K on both sides
+    __syncthreads();
+    for (int i = 0; i < (BM + BN) / 64; ++i) {
+      const int row0 = (wave + 8 * i) * 8, row = row0 + (lane >> 3), o = row - BM;
+      const int c = ((lane & 7) ^ (row < BM ? row & 7 : pool_swz_w<G>(o % (16 * G)))) << 3;
+      const bf16_t* s = row < BM ? xbase + (int64_t)(row < mlim ? row : mlim) * p.ldx : wbase + (int64_t)(o < nlim ? o : nlim) * p.ldw;
+      s = c < ragged ? s + nt * 64 + c : reinterpret_cast<const bf16_t*>(g_pool_zero);
+      __builtin_amdgcn_global_load_lds((gbl_ptr_t)s, (lds_ptr_t)(lds + row0 * 128), 16, 0, 0);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (nt & 1) flip(1);                                     // the chunks went to buffer 0
+    read_w(0, G);
+    read_x(0);
+    mul(0, 0, G);
+    read_x(1);
+    mul(1, 0, G);
+  }
+  pool_epilogue<XF, G>(p, acc, m0, wm * 16 * XF + fr, n0 + wn * 16 * G, fr, fq);
+#endif
 }
 
 // ------------------------------------------------------------------------------------------------ dA / dB: sums over an adapter's rows
@@ -403,14 +730,10 @@ struct PoolTn {
 };
 #define TN_MAX_CH 512
 template <int NR, bool CKPT, bool RANK_MAJOR>
-__global__ __launch_bounds__(256, 2) void pool_tn_kernel(const PoolTn p) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4][4][32 * 128];
-  __shared__ int rows[TN_MAX_CH];
-  const int4 ck = p.table[blockIdx.y];
-  if (ck.x < 0) return;
+__device__ __forceinline__ void pool_tn_body(unsigned char (*lds)[4][32 * 128], int* rows, const PoolTn& p, const int4 ck, int strip) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int fr = lane & 15, fq = lane >> 4;
-  const int cw = blockIdx.x * 256, C = p.C, len = ck.z - ck.y;
+  const int cw = strip * 256, C = p.C, len = ck.z - ck.y;
   const int j0 = 16 * NR * blockIdx.z;                               // first rank of this workgroup
   for (int i = threadIdx.x; i < len; i += 256) rows[i] = p.perm[ck.y + i];
   __syncthreads();
@@ -521,31 +844,54 @@ __global__ __launch_bounds__(256, 2) void pool_tn_kernel(const PoolTn p) {
   }
 }
 
+// both sums of a layer in one launch: the first strips_a workgroups of a chunk row take dA, the others dB
+template <int NR, bool CKPT>
+__global__ __launch_bounds__(256, 2) void pool_tn_kernel(const PoolTn a, const PoolTn b, int strips_a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[4][4][32 * 128];
+  __shared__ int rows[TN_MAX_CH];
+  const int4 ck = a.table[blockIdx.y];
+  if (ck.x < 0) return;
+  if ((int)blockIdx.x < strips_a) pool_tn_body<NR, CKPT, true>(lds, rows, a, ck, blockIdx.x);
+  else pool_tn_body<NR, false, false>(lds, rows, b, ck, blockIdx.x - strips_a);
+}
+
 // out[i] = sum over the chunks of adapter i, in order; part entries [d0][ld] -> out [d0][d1] (the padded ranks are dropped). No rows: zeros.
-__global__ __launch_bounds__(256) void pool_sum_kernel(const float* __restrict__ part, const int* __restrict__ base, int64_t per, int ld, int d0, int d1, float* __restrict__ out) {
+struct PoolSum { const float* part; float* out; int64_t per; int ld, d0, d1; };
+__global__ __launch_bounds__(256) void pool_sum_kernel(const PoolSum a, const PoolSum b, const int* __restrict__ base) {
+  const PoolSum p = blockIdx.z ? b : a;
   const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= (int64_t)d0 * d1) return;
+  if (e >= (int64_t)p.d0 * p.d1) return;
   const int i = blockIdx.y;
-  const int64_t src = (e / d1) * ld + e % d1;
+  const float* src = p.part + (e / p.d1) * p.ld + e % p.d1;
   float s = 0.f;
-  for (int k = base[i]; k < base[i + 1]; ++k) s += part[k * per + src];
-  out[(int64_t)i * d0 * d1 + e] = s;
+  const int k1 = base[i + 1];
+#pragma unroll 8
+  for (int k = base[i]; k < k1; ++k) s += src[k * p.per];
+  p.out[(int64_t)i * p.d0 * p.d1 + e] = s;
 }
 
 // ------------------------------------------------------------------------------------------------ host
 static bool pool_rp(int RP) { return RP == 16 || RP == 32 || RP == 64; }
+static bool pool_counts(int64_t M, int64_t n) { return M >= 0 && M < (1ll << 31) - 256 && n >= 1 && n <= 65535; }
+// a matrix whose rows are read in 16-byte pieces
+static bool pool_rows(const void* t, int64_t ld, int64_t C) { return C >= 8 && C % 8 == 0 && C < (1 << 24) && ld >= C && ld % 8 == 0 && (uintptr_t)t % 16 == 0; }
+#define POOL_CHECK_ROWS(name, T_, ld_, C_)                                                                                              \
+  MF_CHECK_ARG(pool_rows(T_, ld_, C_), name ": rows must hold a multiple of 8 elements, 16-byte aligned, row stride a multiple of 8 (C=%lld ld=%lld)", \
+               (long long)(C_), (long long)(ld_))
 
-extern "C" int mfnet_lora_pool_pack(const void* src, int dtype, int long_first, int64_t n, int64_t C, int r, int RP, void* down, void* up, hipStream_t stream) {
-  MF_CHECK_ARG(src && (down || up), "lora_pool_pack: null pointer");
+extern "C" int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, int64_t n, int64_t K, int64_t N, int r, int RP, void* a_down, void* a_up,
+                                    void* b_down, void* b_up, hipStream_t stream) {
+  MF_CHECK_ARG(A && B && a_down && a_up && b_down && b_up, "lora_pool_pack: null pointer");
   MF_CHECK_ARG(dtype == MFNET_F32 || dtype == MFNET_BF16, "lora_pool_pack: bad dtype");
-  MF_CHECK_ARG(n >= 1 && n <= 65535 && C >= 8 && C % 8 == 0 && C < (1 << 24) && r >= 1 && r <= RP && pool_rp(RP), "lora_pool_pack: bad sizes (n=%lld C=%lld r=%d RP=%d)",
-               (long long)n, (long long)C, r, RP);
-  MF_CHECK_ARG((uintptr_t)src % (dtype == MFNET_F32 ? 4 : 2) == 0 && (uintptr_t)up % 16 == 0 && (uintptr_t)down % 16 == 0, "lora_pool_pack: misaligned tensor");
-  const dim3 grid((unsigned)ceil_div64(C, 256), (unsigned)n);
-#define PP(T_, L_) hipLaunchKernelGGL((pool_pack_kernel<T_, L_>), grid, dim3(256), 0, stream, (const T_*)src, (int)C, r, RP, (bf16_t*)down, (bf16_t*)up)
-  if (dtype == MFNET_F32) { if (long_first) PP(float, true); else PP(float, false); }
-  else { if (long_first) PP(bf16_t, true); else PP(bf16_t, false); }
-#undef PP
+  MF_CHECK_ARG(n >= 1 && n <= 65535 && pool_rows(a_down, K, K) && pool_rows(b_down, N, N) && r >= 1 && r <= RP && pool_rp(RP),
+               "lora_pool_pack: bad sizes (n=%lld K=%lld N=%lld r=%d RP=%d)", (long long)n, (long long)K, (long long)N, r, RP);
+  MF_CHECK_ARG(((uintptr_t)A | (uintptr_t)B) % (dtype == MFNET_F32 ? 4 : 2) == 0 && ((uintptr_t)a_up | (uintptr_t)b_up) % 16 == 0, "lora_pool_pack: misaligned tensor");
+  PoolPack p;
+  p.src[0] = A; p.src[1] = B; p.down[0] = (bf16_t*)a_down; p.down[1] = (bf16_t*)b_down; p.up[0] = (bf16_t*)a_up; p.up[1] = (bf16_t*)b_up;
+  p.C[0] = (int)K; p.C[1] = (int)N; p.r = r; p.RP = RP;
+  const dim3 grid((unsigned)ceil_div64(K > N ? K : N, 256), (unsigned)n, 2);
+  if (dtype == MFNET_F32) hipLaunchKernelGGL(pool_pack_kernel<float>, grid, dim3(256), 0, stream, p);
+  else hipLaunchKernelGGL(pool_pack_kernel<bf16_t>, grid, dim3(256), 0, stream, p);
   MF_LAUNCH_CHECK("lora_pool_pack");
   return MFNET_OK;
 }
@@ -557,7 +903,7 @@ extern "C" int64_t mfnet_lora_pool_chunks(int64_t M, int64_t n) {
 }
 
 extern "C" int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* offs, int* perm, int* base, int* table, hipStream_t stream) {
-  MF_CHECK_ARG(M >= 0 && M < (1ll << 31) - 256 && n >= 1 && n <= 65535, "lora_pool_plan: bad sizes (M=%lld n=%lld)", (long long)M, (long long)n);
+  MF_CHECK_ARG(pool_counts(M, n), "lora_pool_plan: bad sizes (M=%lld n=%lld)", (long long)M, (long long)n);
   MF_CHECK_ARG(offs && base && (M == 0 || (ids && perm && table)), "lora_pool_plan: null pointer");
   MF_CHECK_ARG((uintptr_t)table % 16 == 0, "lora_pool_plan: table must be 16-byte aligned");
   hipLaunchKernelGGL(pool_plan_kernel, dim3((unsigned)n + 1), dim3(256), 0, stream, ids, (int)M, (int)n, offs, perm);
@@ -567,83 +913,117 @@ extern "C" int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* o
   return MFNET_OK;
 }
 
-#define POOL_CHECK_ROWS(name, T_, ld_, C_)                                                                                          \
-  MF_CHECK_ARG((C_) >= 8 && (C_) % 8 == 0 && (C_) < (1 << 24) && (ld_) >= (C_) && (ld_) % 8 == 0 && (uintptr_t)(T_) % 16 == 0,      \
-               name ": rows must hold a multiple of 8 elements, 16-byte aligned, row stride a multiple of 8 (C=%lld ld=%lld)", (long long)(C_), (long long)(ld_))
-
-extern "C" int mfnet_lora_pool_down(const void* X, int64_t ldx, const void* down, const float* scale, const int* ids, int64_t n, int RP,
-                                    float* out, int64_t M, int64_t K, hipStream_t stream) {
-  MF_CHECK_ARG(M >= 0 && M < (1ll << 31) - 256 && n >= 1 && n <= 65535 && pool_rp(RP), "lora_pool_down: bad sizes (M=%lld n=%lld RP=%d)", (long long)M, (long long)n, RP);
-  if (M == 0) return MFNET_OK;
-  MF_CHECK_ARG(X && down && scale && ids && out, "lora_pool_down: null pointer");
-  POOL_CHECK_ROWS("lora_pool_down", X, ldx, K);
-  MF_CHECK_ARG(((uintptr_t)down | (uintptr_t)out) % 16 == 0, "lora_pool_down: misaligned tensor");
-  const dim3 grid((unsigned)ceil_div64(M, 16));
-#define PD(NR_) hipLaunchKernelGGL((pool_down_kernel<NR_>), grid, dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)down, scale, ids, (int)n, out, M, (int)K)
+static int pool_down(const void* X, int64_t ldx, const void* image, const float* scale, const int* ids, int64_t n, int RP, float* out, int64_t M, int64_t K, hipStream_t stream) {
+  // up to 256 rows a workgroup per row is quicker than 16 rows and their adapters in turn
+#define PD(NR_) do { if (M <= 256) hipLaunchKernelGGL((pool_down_row_kernel<NR_>), dim3((unsigned)M), dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)image, scale, ids, (int)n, out, (int)K); \
+    else hipLaunchKernelGGL((pool_down_kernel<NR_>), dim3((unsigned)ceil_div64(M, 16)), dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)image, scale, ids, (int)n, out, M, (int)K); } while (0)
   if (RP == 16) PD(1); else if (RP == 32) PD(2); else PD(4);
 #undef PD
-  MF_LAUNCH_CHECK("lora_pool_down");
+  MF_LAUNCH_CHECK("lora_pool (down)");
   return MFNET_OK;
 }
 
-extern "C" int mfnet_lora_pool_gemm(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* D, const void* up,
-                                    const int* ids, int64_t n, int RP, void* out, int out_dtype, int64_t ldo, int64_t M, int64_t N, int64_t K,
-                                    hipStream_t stream) {
-  MF_CHECK_ARG(M >= 0 && M < (1ll << 31) - 256, "lora_pool_gemm: bad row count");
-  MF_CHECK_ARG(out_dtype == MFNET_BF16 || out_dtype == MFNET_F32, "lora_pool_gemm: bad out dtype");
+static int pool_gemm(PoolGemm& p, hipStream_t stream) {
+  const int64_t M = p.M, N = p.N;
+  const double iters = (p.K + 63) / 64;
+  auto tiles = [&](int bm, int bn) { p.tiles_m = (int)ceil_div64(M, bm); p.tiles_n = (int)ceil_div64(N, bn); return (int64_t)p.tiles_m * p.tiles_n; };
+#define PR(XF_) hipLaunchKernelGGL((pool_gemm_rows_kernel<XF_>), dim3((unsigned)ceil_div64(N, 16)), dim3(256), 0, stream, p)
+  if (M <= 16) PR(1);
+  else if (M <= 32) PR(2);
+  else if (M <= 64) PR(4);
+#undef PR
+  else {
+    // The tile is the one with the least modelled time: rounds of the 256 CUs x (k-tiles x time of one + what a tile costs beside them),
+    // in us, as measured at K = 768 .. 8192 (256 x 256: 0.72 us and 10; 128 x 192, two workgroups per CU: 0.6 and 7; 64 x 64, up to four:
+    // 0.25 and 3 alone).
+    const bool ld_ok = p.ldx <= (1 << 22) && p.ldw <= (1 << 22);         // the phased kernel's 32-bit offsets
+    const double r84 = ceil(ceil_div64(M, 256) * (double)ceil_div64(N, 256) / 256), c84 = r84 * (iters * 1.45 + 11);
+    const double r43 = ceil(ceil_div64(M, 128) * (double)ceil_div64(N, 192) / 256), c43 = r43 * (iters * 0.63 + 7);
+    const double t64 = ceil_div64(M, 64) * (double)ceil_div64(N, 64), c64 = (t64 <= 512 ? 1.0 : t64 / 512) * iters * 0.5 + 4;
+    const int64_t nwg = !ld_ok || (c64 <= c84 && c64 <= c43) ? tiles(64, 64) : c84 <= c43 ? tiles(256, 256) : tiles(128, 192);
+    MF_CHECK_ARG(nwg < (1ll << 31), "lora_pool: too many tiles");
+    if (!ld_ok || (c64 <= c84 && c64 <= c43)) hipLaunchKernelGGL((pool_gemm_kernel<2, 2, 2, 2>), dim3((unsigned)nwg), dim3(256), 0, stream, p);
+    else if (c84 <= c43) hipLaunchKernelGGL((pool_gemm_phased_kernel<8, 4>), dim3((unsigned)nwg), dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((pool_gemm_phased_kernel<4, 3>), dim3((unsigned)nwg), dim3(512), 0, stream, p);
+  }
+  MF_LAUNCH_CHECK("lora_pool (product)");
+  return MFNET_OK;
+}
+
+extern "C" int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* scale, const void* a_down,
+                                   const void* b_up, const int* ids, int64_t n, int RP, float* down, void* out, int out_dtype, int64_t ldo, int64_t M,
+                                   int64_t N, int64_t K, hipStream_t stream) {
+  MF_CHECK_ARG(pool_counts(M, n) && pool_rp(RP), "lora_pool_fwd: bad sizes (M=%lld n=%lld RP=%d)", (long long)M, (long long)n, RP);
+  MF_CHECK_ARG(out_dtype == MFNET_BF16 || out_dtype == MFNET_F32, "lora_pool_fwd: bad out dtype");
   if (M == 0) return MFNET_OK;
-  MF_CHECK_ARG(X && W && out && (!D || (up && ids)), "lora_pool_gemm: null pointer");
-  MF_CHECK_ARG(!D || (n >= 1 && n <= 65535 && pool_rp(RP)), "lora_pool_gemm: bad pool (n=%lld RP=%d)", (long long)n, RP);
-  POOL_CHECK_ROWS("lora_pool_gemm", X, ldx, K);
-  POOL_CHECK_ROWS("lora_pool_gemm (weight)", W, ldw, K);
-  POOL_CHECK_ROWS("lora_pool_gemm (out)", out, ldo, N);
-  MF_CHECK_ARG(((uintptr_t)bias | (uintptr_t)D | (uintptr_t)up) % 16 == 0, "lora_pool_gemm: misaligned tensor");
+  MF_CHECK_ARG(X && W && scale && a_down && b_up && ids && down && out, "lora_pool_fwd: null pointer");
+  POOL_CHECK_ROWS("lora_pool_fwd", X, ldx, K);
+  POOL_CHECK_ROWS("lora_pool_fwd (weight)", W, ldw, K);
+  POOL_CHECK_ROWS("lora_pool_fwd (out)", out, ldo, N);
+  MF_CHECK_ARG(((uintptr_t)bias | (uintptr_t)down | (uintptr_t)a_down | (uintptr_t)b_up) % 16 == 0, "lora_pool_fwd: misaligned tensor");
+  const int rc = pool_down(X, ldx, a_down, scale, ids, n, RP, down, M, K, stream);
+  if (rc) return rc;
   PoolGemm p;
   p.X = (const bf16_t*)X; p.ldx = ldx; p.W = (const bf16_t*)W; p.ldw = ldw; p.bias = bias;
-  p.D = D; p.Up = (const bf16_t*)up; p.ids = ids; p.n = (int)n; p.RP = RP;
+  p.D = down; p.Up = (const bf16_t*)b_up; p.ids = ids; p.n = (int)n; p.RP = RP;
   p.out = out; p.ldo = ldo; p.out_f32 = out_dtype == MFNET_F32;
   p.M = M; p.N = (int)N; p.K = (int)K;
-#define PG(WM_, WN_, XF_, G_) do { p.tiles_m = (int)ceil_div64(M, 16 * XF_ * WM_); p.tiles_n = (int)ceil_div64(N, 16 * G_ * WN_); \
-    MF_CHECK_ARG((int64_t)p.tiles_m * p.tiles_n < (1ll << 31), "lora_pool_gemm: too many tiles"); \
-    hipLaunchKernelGGL((pool_gemm_kernel<WM_, WN_, XF_, G_>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(64 * WM_ * WN_), 0, stream, p); } while (0)
-  if (ceil_div64(M, 256) * ceil_div64(N, 256) >= 200) PG(2, 4, 8, 4);
-  else if (ceil_div64(M, 128) * ceil_div64(N, 128) >= 200) PG(2, 2, 4, 4);
-  else PG(2, 2, 2, 2);
-#undef PG
-  MF_LAUNCH_CHECK("lora_pool_gemm");
-  return MFNET_OK;
+  return pool_gemm(p, stream);
 }
 
-// floats of workspace of mfnet_lora_pool_tn
-extern "C" int64_t mfnet_lora_pool_tn_workspace_floats(int64_t M, int64_t n, int64_t C, int RP) { return mfnet_lora_pool_chunks(M, n) * C * RP; }
+// floats of workspace of mfnet_lora_pool_bwd: p [M, RP] and the partial sums of dA and dB
+extern "C" int64_t mfnet_lora_pool_bwd_workspace_floats(int64_t M, int64_t n, int64_t K, int64_t N, int RP) {
+  return M <= 0 ? 0 : M * RP + mfnet_lora_pool_chunks(M, n) * (K + N) * RP;
+}
 
-extern "C" int mfnet_lora_pool_tn(const void* Y, int64_t ldy, const void* codes, const void* exps, const float* U, int RP, const int* perm, const int* base,
-                                  const int* table, int64_t M, int64_t n, int64_t C, int r, int rank_major, float* out, float* ws, int64_t ws_floats, hipStream_t stream) {
-  MF_CHECK_ARG(M >= 0 && M < (1ll << 31) - 256 && n >= 1 && n <= 65535 && pool_rp(RP) && r >= 1 && r <= RP, "lora_pool_tn: bad sizes");
-  MF_CHECK_ARG(out && base, "lora_pool_tn: null pointer");
-  MF_CHECK_ARG(C >= 8 && C % 8 == 0 && C < (1 << 24), "lora_pool_tn: C=%lld must be a multiple of 8", (long long)C);
+extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, int64_t ldx, const void* codes, const void* exps, const void* Wt, int64_t ldwt,
+                                   const float* scale, const void* b_down, const void* a_up, const int* ids, const int* perm, const int* base, const int* table,
+                                   int64_t n, int r, int RP, const float* down, void* dx, int64_t lddx, float* dA, float* dB, float* ws, int64_t ws_floats,
+                                   int64_t M, int64_t N, int64_t K, hipStream_t stream) {
+  MF_CHECK_ARG(pool_counts(M, n) && pool_rp(RP) && r >= 1 && r <= RP, "lora_pool_bwd: bad sizes (M=%lld n=%lld r=%d RP=%d)", (long long)M, (long long)n, r, RP);
+  MF_CHECK_ARG(K >= 8 && K % 8 == 0 && K < (1 << 24) && N >= 8 && N % 8 == 0 && N < (1 << 24), "lora_pool_bwd: K=%lld and N=%lld must be multiples of 8", (long long)K, (long long)N);
+  MF_CHECK_ARG(dA && dB && base, "lora_pool_bwd: null pointer");
   const int64_t chunks = mfnet_lora_pool_chunks(M, n);
+  float* part_a = ws + M * RP;
+  float* part_b = part_a + chunks * K * RP;
   if (M > 0) {
-    MF_CHECK_ARG(U && perm && table && ((Y != nullptr) != (codes != nullptr)) && (!codes || exps), "lora_pool_tn: null pointer (rows as bf16 or as a checkpoint)");
-    if (Y) POOL_CHECK_ROWS("lora_pool_tn", Y, ldy, C);
-    MF_CHECK_ARG((uintptr_t)codes % 8 == 0 && (uintptr_t)table % 16 == 0 && (uintptr_t)U % 4 == 0, "lora_pool_tn: misaligned tensor");
-    MF_CHECK_ARG(ws && ws_floats >= chunks * C * RP, "lora_pool_tn: workspace too small");
-    MF_CHECK_ARG(chunks <= 65535, "lora_pool_tn: too many chunks of rows (%lld)", (long long)chunks);
-    PoolTn p;
-    p.Y = (const bf16_t*)Y; p.ldy = ldy; p.codes = (const signed char*)codes; p.exps = (const unsigned char*)exps;
-    p.U = U; p.RP = RP; p.perm = perm; p.table = (const int4*)table; p.part = ws; p.C = (int)C;
-    const dim3 grid((unsigned)ceil_div64(C, 256), (unsigned)chunks, RP == 64 ? 2 : 1);
-#define PT(NR_, CK_, RM_) hipLaunchKernelGGL((pool_tn_kernel<NR_, CK_, RM_>), grid, dim3(256), 0, stream, p)
-#define PT2(NR_, CK_) do { if (rank_major) PT(NR_, CK_, true); else PT(NR_, CK_, false); } while (0)
-    if (RP == 16) { if (codes) PT2(1, true); else PT2(1, false); }
-    else { if (codes) PT2(2, true); else PT2(2, false); }
-#undef PT2
+    MF_CHECK_ARG(dy && scale && b_down && ids && perm && table && down && ws && (!dx || (Wt && a_up)), "lora_pool_bwd: null pointer");
+    MF_CHECK_ARG((X != nullptr) != (codes != nullptr) && (!codes || exps), "lora_pool_bwd: the input either as bf16 rows or as a checkpoint");
+    POOL_CHECK_ROWS("lora_pool_bwd (dy)", dy, lddy, N);
+    if (X) POOL_CHECK_ROWS("lora_pool_bwd (x)", X, ldx, K);
+    if (dx) POOL_CHECK_ROWS("lora_pool_bwd (weight)", Wt, ldwt, N);
+    if (dx) POOL_CHECK_ROWS("lora_pool_bwd (dx)", dx, lddx, K);
+    MF_CHECK_ARG((uintptr_t)codes % 8 == 0 && ((uintptr_t)table | (uintptr_t)down | (uintptr_t)ws | (uintptr_t)b_down | (uintptr_t)a_up) % 16 == 0, "lora_pool_bwd: misaligned tensor");
+    MF_CHECK_ARG(ws_floats >= mfnet_lora_pool_bwd_workspace_floats(M, n, K, N, RP), "lora_pool_bwd: workspace too small");
+    MF_CHECK_ARG(chunks <= 65535, "lora_pool_bwd: too many chunks of rows (%lld)", (long long)chunks);
+    int rc = pool_down(dy, lddy, b_down, scale, ids, n, RP, ws, M, N, stream);
+    if (rc) return rc;
+    if (dx) {
+      PoolGemm p;
+      p.X = (const bf16_t*)dy; p.ldx = lddy; p.W = (const bf16_t*)Wt; p.ldw = ldwt; p.bias = nullptr;
+      p.D = ws; p.Up = (const bf16_t*)a_up; p.ids = ids; p.n = (int)n; p.RP = RP;
+      p.out = dx; p.ldo = lddx; p.out_f32 = 0;
+      p.M = M; p.N = (int)K; p.K = (int)N;
+      rc = pool_gemm(p, stream);
+      if (rc) return rc;
+    }
+    PoolTn a, b;
+    a.Y = (const bf16_t*)X; a.ldy = ldx; a.codes = (const signed char*)codes; a.exps = (const unsigned char*)exps;
+    a.U = ws; a.RP = RP; a.perm = perm; a.table = (const int4*)table; a.part = part_a; a.C = (int)K;
+    b = a;
+    b.Y = (const bf16_t*)dy; b.ldy = lddy; b.U = down; b.part = part_b; b.C = (int)N;
+    const int strips_a = (int)ceil_div64(K, 256), strips_b = (int)ceil_div64(N, 256);
+    const dim3 grid((unsigned)(strips_a + strips_b), (unsigned)chunks, RP == 64 ? 2 : 1);
+#define PT(NR_, CK_) hipLaunchKernelGGL((pool_tn_kernel<NR_, CK_>), grid, dim3(256), 0, stream, a, b, strips_a)
+    if (RP == 16) { if (codes) PT(1, true); else PT(1, false); }
+    else { if (codes) PT(2, true); else PT(2, false); }
 #undef PT
-    MF_LAUNCH_CHECK("lora_pool_tn");
+    MF_LAUNCH_CHECK("lora_pool_bwd (sums over rows)");
   }
-  const int d0 = rank_major ? r : (int)C, d1 = rank_major ? (int)C : r;
-  hipLaunchKernelGGL(pool_sum_kernel, dim3((unsigned)ceil_div64((int64_t)d0 * d1, 256), (unsigned)n), dim3(256), 0, stream, ws, base, C * RP,
-                     rank_major ? (int)C : RP, d0, d1, out);
-  MF_LAUNCH_CHECK("lora_pool_tn (sums)");
+  PoolSum sa, sb;
+  sa.part = part_a; sa.out = dA; sa.per = K * RP; sa.ld = (int)K; sa.d0 = r; sa.d1 = (int)K;
+  sb.part = part_b; sb.out = dB; sb.per = N * RP; sb.ld = RP; sb.d0 = (int)N; sb.d1 = r;
+  hipLaunchKernelGGL(pool_sum_kernel, dim3((unsigned)ceil_div64((K > N ? K : N) * r, 256), (unsigned)n, 2), dim3(256), 0, stream, sa, sb, base);
+  MF_LAUNCH_CHECK("lora_pool_bwd (sums of chunks)");
   return MFNET_OK;
 }

@@ -1594,213 +1594,225 @@ def gather(pairs, accumulate=False):
 
 
 # ------------------------------------------------------------------------------------------ 8-bit activation checkpoints
-class _on:
-    """The kernels of a call run on the device its tensors live on, whichever device is current."""
-
-    def __init__(self, t):
-        self.dev = t.device.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.prev != self.dev:
-            torch.cuda.set_device(self.prev)
-        return False
+# The wrappers below are called with tensors of a few microseconds' work: their checks are written to cost about one (device indices
+# instead of device objects, messages formatted only when raised, one allocation for what belongs together).
+_raw_stream = torch._C._cuda_getCurrentRawStream        # torch.cuda.current_stream(device).cuda_stream without the Stream object
 
 
-def _one_device(name, *ts):
-    """all tensors on one ROCm device (a kernel would read another device's memory as its own)"""
-    dev = None
+def _bad(name, what):
+    raise MfnetError(f"{name}: {what}")
+
+
+def _device_of(name, *ts):
+    """index of the one ROCm device all the tensors are on (a kernel would read another device's memory as its own)"""
+    dev = -2
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()
+        if d < 0:
             _chk(t)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise MfnetError(f"{name}: tensors on {dev} and {t.device}")
+        if dev == -2:
+            dev = d
+        elif d != dev:
+            _bad(name, f"tensors on devices {dev} and {d}")
+    return dev
 
 
-def _need(cond, name, what):
-    if not cond:
-        raise MfnetError(f"{name}: {what}")
+def _launch(name, dev, nbytes, flops, *args):
+    """the entry point on the current stream of device dev, whichever device is current"""
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return tcall(name, nbytes, flops, *args, _raw_stream(dev))
+    if KERNEL_TRACE is None:
+        return call(name, *args, _raw_stream(dev))
+    return tcall(name, nbytes, flops, *args, _raw_stream(dev))
 
 
 def _rows_any(name, t):
     """(tensor, rows, C, row stride) of [..., C] with a unit last stride and leading dimensions that collapse to one stride; a view
     that has no such form is copied"""
-    _need(t.dim() >= 1 and t.shape[-1] >= 1, name, f"needs at least one element per row, got shape {tuple(t.shape)}")
-    C = t.shape[-1]
-    if t.dim() == 2 and (t.stride(1) == 1 or C == 1) and (t.shape[0] <= 1 or t.stride(0) >= C):
-        return t, t.shape[0], C, t.stride(0) if t.shape[0] > 1 else C
-    t2 = t.contiguous().view(-1, C)
-    return t2, t2.shape[0], C, C
+    shape = t.shape
+    if not shape or not shape[-1]:
+        _bad(name, f"needs at least one element per row, got shape {tuple(shape)}")
+    C = shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // C, C, C
+    if t.dim() == 2 and (t.stride(1) == 1 or C == 1) and (shape[0] <= 1 or t.stride(0) >= C):
+        return t, shape[0], C, t.stride(0) if shape[0] > 1 else C
+    return t.contiguous(), t.numel() // C, C, C
 
 
 class Ckpt8:
-    """A tensor held in 8 bits: int8 codes of its shape [..., C] and one exponent byte per 32 consecutive elements of a row. `shape`
-    is the tensor's; `nbytes` what it occupies. Made by ckpt8_pack / gelu_fwd_ckpt8 / layernorm_fwd_ckpt8, read by ckpt8_unpack and the
-    backward kernels."""
-    __slots__ = ("codes", "exps", "shape")
+    """A tensor held in 8 bits: int8 codes of its shape [..., C] and one exponent byte per 32 consecutive elements of a row, in one
+    buffer. `shape` is the tensor's, `nbytes` what it occupies. Made by ckpt8_pack / gelu_fwd_ckpt8 / layernorm_fwd_ckpt8, read by
+    ckpt8_unpack and the backward kernels."""
+    __slots__ = ("buf", "shape", "rows", "C", "at_exps")
 
-    def __init__(self, codes, exps, shape):
-        self.codes, self.exps, self.shape = codes, exps, tuple(shape)
-
-    @classmethod
-    def empty(cls, shape, device):
-        C = shape[-1]
-        return cls(torch.empty(shape, dtype=torch.int8, device=device),
-                   torch.empty(tuple(shape[:-1]) + ((C + 31) // 32,), dtype=torch.uint8, device=device), shape)
-
-    @property
-    def device(self):
-        return self.codes.device
-
-    @property
-    def nbytes(self):
-        return self.codes.numel() + self.exps.numel()
-
-    def _check(self, name):
-        C = self.shape[-1]
-        _need(self.codes.dtype == torch.int8 and self.exps.dtype == torch.uint8 and self.codes.is_contiguous() and self.exps.is_contiguous()
-              and tuple(self.codes.shape) == self.shape and tuple(self.exps.shape) == self.shape[:-1] + ((C + 31) // 32,), name,
-              "a Ckpt8 needs dense int8 codes and one uint8 exponent per 32 elements of a row")
+    def __init__(self, shape, device):
+        self.shape = tuple(shape)
+        self.C = C = self.shape[-1]
         rows = 1
         for d in self.shape[:-1]:
             rows *= d
-        return rows, C
+        self.rows = rows
+        self.at_exps = (rows * C + 15) // 16 * 16
+        self.buf = torch.empty(self.at_exps + rows * ((C + 31) // 32), dtype=torch.uint8, device=device)
+
+    @property
+    def device(self):
+        return self.buf.device
+
+    @property
+    def nbytes(self):
+        return self.buf.numel()
+
+    @property
+    def codes(self):
+        return self.buf[:self.rows * self.C].view(torch.int8).view(self.shape)
+
+    @property
+    def exps(self):
+        return self.buf[self.at_exps:].view(self.shape[:-1] + ((self.C + 31) // 32,))
+
+    def _ptrs(self):
+        p = self.buf.data_ptr()
+        return p, p + self.at_exps
 
 
 def _ck_dtype(name, t):
-    _need(t.dtype in _DT, name, f"dtype {t.dtype}: float32 or bfloat16")
-    return _DT[t.dtype]
+    dt = _DT.get(t.dtype)
+    if dt is None:
+        _bad(name, f"dtype {t.dtype}: float32 or bfloat16")
+    return dt
 
 
 def ckpt8_pack(x) -> Ckpt8:
     """x [..., C] fp32 | bf16 -> its 8-bit checkpoint."""
-    _one_device("ckpt8_pack", x)
+    dev = _device_of("ckpt8_pack", x)
     dt = _ck_dtype("ckpt8_pack", x)
     x2, rows, C, ldx = _rows_any("ckpt8_pack", x)
-    c = Ckpt8.empty(x.shape, x.device)
-    with _on(x):
-        tcall("mfnet_ckpt8_pack", x.numel() * (x.element_size() + 1) + c.exps.numel(), 0, x2.data_ptr(), dt, ldx, c.codes.data_ptr(),
-              c.exps.data_ptr(), rows, C, _stream(x))
+    c = Ckpt8(x.shape, x.device)
+    codes, exps = c._ptrs()
+    _launch("mfnet_ckpt8_pack", dev, rows * C * (2 if dt else 4) + c.nbytes, 0, x2.data_ptr(), dt, ldx, codes, exps, rows, C)
     return c
 
 
 def ckpt8_unpack(c: Ckpt8, dtype=torch.bfloat16):
     """the values a checkpoint stands for (exact in bf16 and fp32)."""
-    _one_device("ckpt8_unpack", c.codes, c.exps)
-    rows, C = c._check("ckpt8_unpack")
-    _need(dtype in _DT, "ckpt8_unpack", f"dtype {dtype}: float32 or bfloat16")
-    x = torch.empty(c.shape, dtype=dtype, device=c.device)
-    with _on(x):
-        tcall("mfnet_ckpt8_unpack", x.numel() * (x.element_size() + 1) + c.exps.numel(), 0, c.codes.data_ptr(), c.exps.data_ptr(), x.data_ptr(),
-              _DT[dtype], C, rows, C, _stream(x))
+    dev = _device_of("ckpt8_unpack", c.buf)
+    if dtype not in _DT:
+        _bad("ckpt8_unpack", f"dtype {dtype}: float32 or bfloat16")
+    x = torch.empty(c.shape, dtype=dtype, device=c.buf.device)
+    codes, exps = c._ptrs()
+    _launch("mfnet_ckpt8_unpack", dev, x.numel() * x.element_size() + c.nbytes, 0, codes, exps, x.data_ptr(), _DT[dtype], c.C, c.rows, c.C)
     return x
 
 
 def gelu_fwd_ckpt8(x):
     """x [..., C] fp32 | bf16 -> (GELU(x) of its dtype, the checkpoint of x)."""
-    _one_device("gelu_fwd_ckpt8", x)
-    dt = _ck_dtype("gelu_fwd_ckpt8", x)
-    x2, rows, C, ldx = _rows_any("gelu_fwd_ckpt8", x)
+    name = "gelu_fwd_ckpt8"
+    dev = _device_of(name, x)
+    dt = _ck_dtype(name, x)
+    x2, rows, C, ldx = _rows_any(name, x)
     act = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    c = Ckpt8.empty(x.shape, x.device)
-    with _on(x):
-        tcall("mfnet_gelu_fwd_ckpt8", x.numel() * (2 * x.element_size() + 1) + c.exps.numel(), 0, x2.data_ptr(), dt, ldx, act.data_ptr(), C,
-              c.codes.data_ptr(), c.exps.data_ptr(), rows, C, _stream(x))
+    c = Ckpt8(x.shape, x.device)
+    codes, exps = c._ptrs()
+    _launch("mfnet_gelu_fwd_ckpt8", dev, rows * C * (4 if dt else 8) + c.nbytes, 0, x2.data_ptr(), dt, ldx, act.data_ptr(), C, codes, exps, rows, C)
     return act, c
 
 
 def gelu_bwd_ckpt8(c: Ckpt8, dy, want_act=False):
     """dy [..., C] -> dx = dy * GELU'(x8) of dy's dtype; with want_act (dx, GELU(x8)): the activation the next layer's weight gradient needs."""
-    _one_device("gelu_bwd_ckpt8", c.codes, c.exps, dy)
-    rows, C = c._check("gelu_bwd_ckpt8")
-    dt = _ck_dtype("gelu_bwd_ckpt8", dy)
-    _need(tuple(dy.shape) == c.shape, "gelu_bwd_ckpt8", f"dy {tuple(dy.shape)} does not match the checkpoint {c.shape}")
-    d2, _, _, ldd = _rows_any("gelu_bwd_ckpt8", dy)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    name = "gelu_bwd_ckpt8"
+    dev = _device_of(name, c.buf, dy)
+    dt = _ck_dtype(name, dy)
+    if dy.shape != c.shape:
+        _bad(name, f"dy {tuple(dy.shape)} does not match the checkpoint {c.shape}")
+    d2, rows, C, ldd = _rows_any(name, dy)
+    dx = torch.empty(c.shape, dtype=dy.dtype, device=dy.device)
     act = torch.empty_like(dx) if want_act else None
-    with _on(dy):
-        tcall("mfnet_gelu_bwd_ckpt8", dy.numel() * ((3 if want_act else 2) * dy.element_size() + 1) + c.exps.numel(), 0, c.codes.data_ptr(),
-              c.exps.data_ptr(), d2.data_ptr(), dt, ldd, dx.data_ptr(), _p(act), C, rows, C, _stream(dy))
+    codes, exps = c._ptrs()
+    _launch("mfnet_gelu_bwd_ckpt8", dev, rows * C * (3 if want_act else 2) * (2 if dt else 4) + c.nbytes, 0, codes, exps, d2.data_ptr(), dt, ldd,
+            dx.data_ptr(), _p(act), C, rows, C)
     return (dx, act) if want_act else dx
 
 
 def _vec_f32(name, what, t, n):
-    _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n, name, f"{what} must be {n} dense fp32 values, got {tuple(t.shape)} {t.dtype}")
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n:
+        _bad(name, f"{what} must be {n} dense fp32 values, got {tuple(t.shape)} {t.dtype}")
 
 
-def _aligned(t, nbytes=16):
-    """t, or a copy of it where its storage offset breaks the kernels' alignment"""
-    return t if t is None or t.data_ptr() % nbytes == 0 else t.clone()
+def _aligned(t):
+    """t, or a copy of it where its storage offset breaks the kernels' 16-byte alignment"""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _ln_rows(name, t):
+    t2, rows, C, ld = _rows_any(name, t)
+    if C % 32 or C > 2048:
+        _bad(name, f"C={C} must be a multiple of 32, at most 2048")
+    if ld % 4 or t2.data_ptr() % 16:
+        t2, ld = t2.clone(memory_format=torch.contiguous_format), C
+    return t2, rows, C, ld
 
 
 def layernorm_fwd_ckpt8(x, gamma, beta, eps):
     """x [..., C] fp32 | bf16 -> (LayerNorm(x) bf16, mean, rstd, the checkpoint of x). C a multiple of 32, at most 2048."""
     name = "layernorm_fwd_ckpt8"
-    _one_device(name, x, gamma, beta)
+    dev = _device_of(name, x, gamma, beta)
     dt = _ck_dtype(name, x)
-    x2, rows, C, ldx = _rows_any(name, x)
-    _need(C % 32 == 0 and C <= 2048, name, f"C={C} must be a multiple of 32, at most 2048")
+    x2, rows, C, ldx = _ln_rows(name, x)
     _vec_f32(name, "gamma", gamma, C)
     _vec_f32(name, "beta", beta, C)
-    if ldx % 4 or x2.data_ptr() % 16:
-        x2, ldx = x2.clone(memory_format=torch.contiguous_format), C
     gamma, beta = _aligned(gamma), _aligned(beta)
     y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    c = Ckpt8.empty(x.shape, x.device)
-    with _on(x):
-        tcall("mfnet_layernorm_fwd_ckpt8", x.numel() * (x.element_size() + 3) + c.exps.numel() + 8 * rows, 0, x2.data_ptr(), dt, ldx, gamma.data_ptr(),
-              beta.data_ptr(), y.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(), c.codes.data_ptr(), c.exps.data_ptr(), rows, C, float(eps), _stream(x))
-    return y, stats[0], stats[1], c
+    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
+    c = Ckpt8(x.shape, x.device)
+    codes, exps = c._ptrs()
+    _launch("mfnet_layernorm_fwd_ckpt8", dev, rows * C * (4 if dt else 6) + c.nbytes + 8 * rows, 0, x2.data_ptr(), dt, ldx, gamma.data_ptr(), beta.data_ptr(),
+            y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exps, rows, C, float(eps))
+    return y, mean, rstd, c
 
 
 def layernorm_bwd_ckpt8(dy, c: Ckpt8, mean, rstd, gamma, beta=None, dres=None, want_f32=True, want_bf16=False, want_y=False, want_weights=False):
     """dx = LN'(dy) (+ dres) from the checkpoint of the LayerNorm's input. Returns the fp32 dx (want_f32), its bf16 copy (want_bf16), the
     LayerNorm output again (want_y: bf16, needs beta) and dgamma, dbeta (want_weights), those asked for, in this order (one alone as it is)."""
     name = "layernorm_bwd_ckpt8"
-    _one_device(name, dy, c.codes, c.exps, mean, rstd, gamma, beta, dres)
-    rows, C = c._check(name)
+    dev = _device_of(name, dy, c.buf, mean, rstd, gamma, beta, dres)
     dt = _ck_dtype(name, dy)
-    _need(C % 32 == 0 and C <= 2048, name, f"C={C} must be a multiple of 32, at most 2048")
-    _need(tuple(dy.shape) == c.shape, name, f"dy {tuple(dy.shape)} does not match the checkpoint {c.shape}")
-    _need(want_f32 or want_bf16, name, "dx is wanted in neither dtype")
-    _need(not want_y or beta is not None, name, "want_y needs beta")
+    if dy.shape != c.shape:
+        _bad(name, f"dy {tuple(dy.shape)} does not match the checkpoint {c.shape}")
+    d2, rows, C, ldd = _ln_rows(name, dy)
+    if not (want_f32 or want_bf16):
+        _bad(name, "dx is wanted in neither dtype")
+    if want_y and beta is None:
+        _bad(name, "want_y needs beta")
     _vec_f32(name, "mean", mean, rows)
     _vec_f32(name, "rstd", rstd, rows)
     _vec_f32(name, "gamma", gamma, C)
     if beta is not None:
         _vec_f32(name, "beta", beta, C)
-    d2, _, _, ldd = _rows_any(name, dy)
-    if ldd % 4 or d2.data_ptr() % 16:
-        d2, ldd = d2.clone(memory_format=torch.contiguous_format), C
     if dres is not None:
-        _need(dres.dtype == torch.float32 and tuple(dres.shape) == c.shape, name, f"dres must be fp32 {c.shape}")
+        if dres.dtype != torch.float32 or dres.shape != c.shape:
+            _bad(name, f"dres must be fp32 {c.shape}")
         dres = _aligned(dres.contiguous())
     gamma, beta = _aligned(gamma), _aligned(beta)
-    dev = dy.device
-    dx = torch.empty(c.shape, dtype=torch.float32, device=dev) if want_f32 else None
-    dxb = torch.empty(c.shape, dtype=torch.bfloat16, device=dev) if want_bf16 else None
-    y = torch.empty(c.shape, dtype=torch.bfloat16, device=dev) if want_y else None
-    dgb = ws = None
+    device = dy.device
+    dx = torch.empty(c.shape, dtype=torch.float32, device=device) if want_f32 else None
+    dxb = torch.empty(c.shape, dtype=torch.bfloat16, device=device) if want_bf16 else None
+    y = torch.empty(c.shape, dtype=torch.bfloat16, device=device) if want_y else None
+    dg = db = ws = None
     nws = 0
     if want_weights:
-        nws = int(_lib.lib().mfnet_layernorm_ckpt8_workspace_floats(rows, C))
-        dgb = torch.empty((2, C), dtype=torch.float32, device=dev)
-        ws = torch.empty(nws, dtype=torch.float32, device=dev)
-    per_el = dy.element_size() + 1 + (4 if dres is not None else 0) + (4 if want_f32 else 0) + (2 if want_bf16 else 0) + (2 if want_y else 0)
-    with _on(dy):
-        tcall("mfnet_layernorm_bwd_ckpt8", dy.numel() * per_el + c.exps.numel() + 8 * rows, 0, d2.data_ptr(), dt, ldd, c.codes.data_ptr(), c.exps.data_ptr(),
-              mean.data_ptr(), rstd.data_ptr(), gamma.data_ptr(), _p(beta), _p(dres), _p(dx), _p(dxb), _p(y), _p(dgb[0]) if want_weights else None,
-              _p(dgb[1]) if want_weights else None, _p(ws), nws, rows, C, _stream(dy))
-    out = [t for t in (dx, dxb, y) if t is not None] + ([dgb[0], dgb[1]] if want_weights else [])
+        nws = _lib.lib().mfnet_layernorm_ckpt8_workspace_floats(rows, C)
+        dg, db = torch.empty((2, C), dtype=torch.float32, device=device).unbind(0)
+        ws = torch.empty(nws, dtype=torch.float32, device=device)
+    per_el = (2 if dt else 4) + (4 if dres is not None else 0) + (4 if want_f32 else 0) + (2 if want_bf16 else 0) + (2 if want_y else 0)
+    codes, exps = c._ptrs()
+    _launch("mfnet_layernorm_bwd_ckpt8", dev, rows * C * per_el + c.nbytes + 8 * rows, 0, d2.data_ptr(), dt, ldd, codes, exps, mean.data_ptr(),
+            rstd.data_ptr(), gamma.data_ptr(), _p(beta), _p(dres), _p(dx), _p(dxb), _p(y), _p(dg), _p(db), _p(ws), nws, rows, C)
+    out = [t for t in (dx, dxb, y, dg, db) if t is not None]
     return out[0] if len(out) == 1 else tuple(out)
 
 
@@ -1808,41 +1820,41 @@ def layernorm_bwd_ckpt8(dy, c: Ckpt8, mean, rstd, gamma, beta=None, dres=None, w
 class LoraPool:
     """n low-rank adapters of one layer, laid out for the kernels (lora_pool): bf16 images of A [n, r, K] and B [n, N, r] padded to
     RP = 16, 32 or 64 ranks, one per direction of use. A copy: later changes of A and B do not reach it."""
-    __slots__ = ("n", "r", "K", "N", "RP", "scale", "a_down", "a_up", "b_down", "b_up")
-
-    @property
-    def device(self):
-        return self.a_down.device
+    __slots__ = ("n", "r", "K", "N", "RP", "scale", "buf", "a_down", "a_up", "b_down", "b_up")
 
 
 def lora_pool(A, B, scale=None) -> LoraPool:
-    """A [n, r, K], B [n, N, r] fp32 | bf16 (fp32 factors are rounded to bf16: the MFMA operands), scale [n] fp32 (None: ones);
-    1 <= r <= 64, K and N multiples of 8."""
+    """A [n, r, K], B [n, N, r], both fp32 or both bf16 (fp32 factors are rounded to bf16: the MFMA operands), scale [n] fp32 (None:
+    ones); 1 <= r <= 64, K and N multiples of 8."""
     name = "lora_pool"
-    _one_device(name, A, B, scale)
-    _need(A.dim() == 3 and B.dim() == 3 and A.shape[0] == B.shape[0] and A.shape[1] == B.shape[2], name,
-          f"A [n, r, K] and B [n, N, r] expected, got {tuple(A.shape)} and {tuple(B.shape)}")
+    dev = _device_of(name, A, B, scale)
+    if A.dim() != 3 or B.dim() != 3 or A.shape[0] != B.shape[0] or A.shape[1] != B.shape[2]:
+        _bad(name, f"A [n, r, K] and B [n, N, r] expected, got {tuple(A.shape)} and {tuple(B.shape)}")
     n, r, K = A.shape
     N = B.shape[1]
-    _need(1 <= n <= 65535 and 1 <= r <= 64, name, f"{n} adapters of rank {r}: 1 .. 65535 adapters of rank 1 .. 64")
-    _need(8 <= K < 1 << 24 and 8 <= N < 1 << 24 and K % 8 == 0 and N % 8 == 0, name, f"K={K} and N={N} must be multiples of 8 below 2^24")
-    _ck_dtype(name, A)
-    _ck_dtype(name, B)
+    if not (1 <= n <= 65535 and 1 <= r <= 64):
+        _bad(name, f"{n} adapters of rank {r}: 1 .. 65535 adapters of rank 1 .. 64")
+    if not (8 <= K < 1 << 24 and 8 <= N < 1 << 24) or K % 8 or N % 8:
+        _bad(name, f"K={K} and N={N} must be multiples of 8 below 2^24")
+    dt = _ck_dtype(name, A)
+    if B.dtype != A.dtype:
+        _bad(name, f"A is {A.dtype}, B is {B.dtype}")
     p = LoraPool()
     p.n, p.r, p.K, p.N = n, r, K, N
-    p.RP = 16 if r <= 16 else 32 if r <= 32 else 64
+    p.RP = RP = 16 if r <= 16 else 32 if r <= 32 else 64
     A, B = A.detach().contiguous(), B.detach().contiguous()
     if scale is None:
         p.scale = torch.ones(n, dtype=torch.float32, device=A.device)
     else:
         _vec_f32(name, "scale", scale, n)
         p.scale = scale.detach().clone()
-    def image(*shape):
-        return torch.empty(shape, dtype=torch.bfloat16, device=A.device)
-    p.a_down, p.a_up, p.b_down, p.b_up = image(n, p.RP, K), image(n, K, p.RP), image(n, p.RP, N), image(n, N, p.RP)
-    with _on(A):
-        call("mfnet_lora_pool_pack", A.data_ptr(), _DT[A.dtype], 0, n, K, r, p.RP, p.a_down.data_ptr(), p.a_up.data_ptr(), _stream(A))
-        call("mfnet_lora_pool_pack", B.data_ptr(), _DT[B.dtype], 1, n, N, r, p.RP, p.b_down.data_ptr(), p.b_up.data_ptr(), _stream(A))
+    p.buf = torch.empty(2 * n * RP * (K + N), dtype=torch.bfloat16, device=A.device)
+    p.a_down = p.buf.data_ptr()                           # device addresses of the four images: every one a multiple of 16 bytes
+    p.a_up = p.a_down + 2 * n * RP * K
+    p.b_down = p.a_up + 2 * n * RP * K
+    p.b_up = p.b_down + 2 * n * RP * N
+    _launch("mfnet_lora_pool_pack", dev, A.element_size() * n * r * (K + N) + 2 * p.buf.numel(), 0, A.data_ptr(), B.data_ptr(), dt, n, K, N, r, RP,
+            p.a_down, p.a_up, p.b_down, p.b_up)
     return p
 
 
@@ -1853,54 +1865,37 @@ class LoraPlan:
 
 
 def _check_ids(name, ids, M):
-    _need(ids.dtype == torch.int32 and ids.dim() == 1 and ids.is_contiguous() and ids.shape[0] == M, name,
-          f"ids must be {M} dense int32 row indices, got {tuple(ids.shape)} {ids.dtype}")
+    if ids.dtype != torch.int32 or ids.dim() != 1 or ids.shape[0] != M or not ids.is_contiguous():
+        _bad(name, f"ids must be {M} dense int32 row indices, got {tuple(ids.shape)} {ids.dtype}")
 
 
 def lora_pool_plan(ids, n) -> LoraPlan:
     """ids int32 [M]: the adapter of every row (none if outside [0, n))."""
     name = "lora_pool_plan"
-    _one_device(name, ids)
-    _need(ids.dim() == 1, name, f"ids must be one-dimensional, got {tuple(ids.shape)}")
-    _check_ids(name, ids, ids.shape[0])
-    _need(1 <= n <= 65535, name, f"n={n}: 1 .. 65535 adapters")
+    dev = _device_of(name, ids)
+    _check_ids(name, ids, ids.shape[0] if ids.dim() else -1)
+    if not 1 <= n <= 65535:
+        _bad(name, f"n={n}: 1 .. 65535 adapters")
     p = LoraPlan()
     p.ids, p.M, p.n = ids, ids.shape[0], n
-    chunks = int(_lib.lib().mfnet_lora_pool_chunks(p.M, n))
+    chunks = _lib.lib().mfnet_lora_pool_chunks(p.M, n)
     p.table = torch.empty((max(chunks, 1), 4), dtype=torch.int32, device=ids.device)
-    p.offs, p.base = torch.empty((2, n + 1), dtype=torch.int32, device=ids.device)
+    p.offs, p.base = torch.empty((2, n + 1), dtype=torch.int32, device=ids.device).unbind(0)
     p.perm = torch.empty(max(p.M, 1), dtype=torch.int32, device=ids.device)
-    with _on(ids):
-        call("mfnet_lora_pool_plan", ids.data_ptr(), p.M, n, p.offs.data_ptr(), p.perm.data_ptr(), p.base.data_ptr(), p.table.data_ptr(), _stream(ids))
+    _launch("mfnet_lora_pool_plan", dev, 8 * p.M, 0, ids.data_ptr(), p.M, n, p.offs.data_ptr(), p.perm.data_ptr(), p.base.data_ptr(), p.table.data_ptr())
     return p
 
 
-def _bf16_rows(name, what, t, cols):
-    """(tensor, rows, stride) of a bf16 matrix whose rows the kernels read in 16-byte pieces; other layouts are copied"""
-    _need(t.dtype == torch.bfloat16 and t.dim() == 2 and t.shape[1] == cols, name, f"{what} must be a bf16 matrix of {cols} columns, got {tuple(t.shape)} {t.dtype}")
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < cols or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else cols
-
-
-def _pool_gemm(name, x, w, bias, down, up, ids, pool, out_dtype):
-    M, K = x.shape
-    N = w.shape[0]
-    x, _, ldx = _bf16_rows(name, "the rows", x, K)
-    w, _, ldw = _bf16_rows(name, "the weight", w, K)
-    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
-    tcall("mfnet_lora_pool_gemm", 2 * (M * K + N * K) + M * N * out.element_size(), 2.0 * M * N * K + 2.0 * M * N * pool.r, x.data_ptr(), ldx, w.data_ptr(), ldw,
-          _p(bias), _p(down), up.data_ptr(), ids.data_ptr(), pool.n, pool.RP, out.data_ptr(), _DT[out_dtype], N, M, N, K, _stream(x))
-    return out
-
-
-def _pool_down(name, x, image, ids, pool):
-    M, C = x.shape
-    x, _, ldx = _bf16_rows(name, "the rows", x, C)
-    d = torch.empty((M, pool.RP), dtype=torch.float32, device=x.device)
-    tcall("mfnet_lora_pool_down", 2 * M * C + 4 * M * pool.RP, 2.0 * M * C * pool.r, x.data_ptr(), ldx, image.data_ptr(), pool.scale.data_ptr(), ids.data_ptr(),
-          pool.n, pool.RP, d.data_ptr(), M, C, _stream(x))
-    return d
+def _bf16_rows(name, what, t, rows, cols):
+    """(tensor, stride) of a bf16 [rows, cols] matrix whose rows the kernels read in 16-byte pieces; other layouts are copied"""
+    if t.dtype != torch.bfloat16 or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        _bad(name, f"{what} must be a bf16 [{rows}, {cols}] matrix, got {tuple(t.shape)} {t.dtype}")
+    ld, inner = t.stride()
+    if rows <= 1:
+        ld = cols
+    if inner != 1 or ld % 8 or ld < cols or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format), cols
+    return t, ld
 
 
 def lora_pool_fwd(x, w, bias, pool: LoraPool, ids, out_dtype=torch.bfloat16, want_down=False):
@@ -1908,33 +1903,23 @@ def lora_pool_fwd(x, w, bias, pool: LoraPool, ids, out_dtype=torch.bfloat16, wan
     x [M, K] bf16 and w [N, K] bf16 (any row stride), bias [N] fp32 or None, ids int32 [M]. want_down: (out, down), the fp32 [M, RP]
     product s_i A_i x that lora_pool_bwd reads."""
     name = "lora_pool_fwd"
-    _one_device(name, x, w, bias, pool.a_down, ids)
-    _need(x.dim() == 2 and x.shape[1] == pool.K and w.dim() == 2 and tuple(w.shape) == (pool.N, pool.K), name,
-          f"x [M, {pool.K}] and w [{pool.N}, {pool.K}] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
-    _need(out_dtype in _DT, name, f"out_dtype {out_dtype}: float32 or bfloat16")
-    _check_ids(name, ids, x.shape[0])
+    dev = _device_of(name, x, w, bias, pool.buf, ids)
+    M, K, N = x.shape[0] if x.dim() else 0, pool.K, pool.N
+    x, ldx = _bf16_rows(name, "x", x, M, K)
+    w, ldw = _bf16_rows(name, "w", w, N, K)
+    od = _DT.get(out_dtype)
+    if od is None:
+        _bad(name, f"out_dtype {out_dtype}: float32 or bfloat16")
+    _check_ids(name, ids, M)
     if bias is not None:
-        _vec_f32(name, "bias", bias, pool.N)
+        _vec_f32(name, "bias", bias, N)
         bias = _aligned(bias)
-    with _on(x):
-        down = _pool_down(name, x, pool.a_down, ids, pool)
-        out = _pool_gemm(name, x, w, bias, down, pool.b_up, ids, pool, out_dtype)
+    down = torch.empty((M, pool.RP), dtype=torch.float32, device=x.device)
+    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    _launch("mfnet_lora_pool_fwd", dev, 2 * (M * K + N * K + pool.n * pool.r * (K + N)) + M * N * (2 if od else 4), 2.0 * M * (N * K + pool.r * (N + K)),
+            x.data_ptr(), ldx, w.data_ptr(), ldw, _p(bias), pool.scale.data_ptr(), pool.a_down, pool.b_up, ids.data_ptr(), pool.n, pool.RP, down.data_ptr(),
+            out.data_ptr(), od, N, M, N, K)
     return (out, down) if want_down else out
-
-
-def _pool_tn(name, y, u, plan, pool, C, rank_major):
-    M, n = plan.M, plan.n
-    out = torch.empty((n, pool.r, C) if rank_major else (n, C, pool.r), dtype=torch.float32, device=u.device)
-    nws = int(_lib.lib().mfnet_lora_pool_tn_workspace_floats(M, n, C, pool.RP))
-    ws = torch.empty(max(nws, 1), dtype=torch.float32, device=u.device)
-    if isinstance(y, Ckpt8):
-        src, nbytes = (None, 0, y.codes.data_ptr(), y.exps.data_ptr()), y.nbytes
-    else:
-        y, _, ldy = _bf16_rows(name, "the rows", y, C)
-        src, nbytes = (y.data_ptr(), ldy, None, None), 2 * M * C
-    tcall("mfnet_lora_pool_tn", nbytes + 4 * M * pool.RP + 4 * out.numel(), 2.0 * M * C * pool.r, *src, u.data_ptr(), pool.RP, plan.perm.data_ptr(),
-          plan.base.data_ptr(), plan.table.data_ptr(), M, n, C, pool.r, 1 if rank_major else 0, out.data_ptr(), ws.data_ptr(), nws, _stream(u))
-    return out
 
 
 def lora_pool_bwd(dy, x, w_t, pool: LoraPool, plan: LoraPlan, down, want_dx=True):
@@ -1943,19 +1928,33 @@ def lora_pool_bwd(dy, x, w_t, pool: LoraPool, plan: LoraPlan, down, want_dx=True
     plan of the same row indices. Adapters without rows get zero gradients; the result does not depend on the run."""
     name = "lora_pool_bwd"
     ck = isinstance(x, Ckpt8)
-    _one_device(name, dy, *((x.codes, x.exps) if ck else (x,)), w_t if want_dx else None, pool.a_down, plan.perm, down)
-    M = plan.M
-    _need(dy.dim() == 2 and tuple(dy.shape) == (M, pool.N), name, f"dy [{M}, {pool.N}] expected, got {tuple(dy.shape)}")
+    dev = _device_of(name, dy, x.buf if ck else x, w_t if want_dx else None, pool.buf, plan.perm, down)
+    M, n, K, N, RP = plan.M, pool.n, pool.K, pool.N, pool.RP
+    dy, lddy = _bf16_rows(name, "dy", dy, M, N)
     if ck:
-        x._check(name)
-    _need(len(x.shape) == 2 and tuple(x.shape) == (M, pool.K), name, f"x [{M}, {pool.K}] expected, got {tuple(x.shape)}")
-    _need(plan.n == pool.n, name, f"the plan counts {plan.n} adapters, the pool holds {pool.n}")
-    _need(tuple(down.shape) == (M, pool.RP) and down.dtype == torch.float32 and down.is_contiguous(), name, f"down must be the forward's fp32 [{M}, {pool.RP}]")
+        if x.shape != (M, K):
+            _bad(name, f"x [{M}, {K}] expected, got the checkpoint of {x.shape}")
+        src = (None, 0) + x._ptrs()
+    else:
+        x, ldx = _bf16_rows(name, "x", x, M, K)
+        src = (x.data_ptr(), ldx, None, None)
+    if plan.n != n:
+        _bad(name, f"the plan counts {plan.n} adapters, the pool holds {n}")
+    if down.shape != (M, RP) or down.dtype != torch.float32 or not down.is_contiguous():
+        _bad(name, f"down must be the forward's fp32 [{M}, {RP}]")
+    ldw, dx = 0, None
+    device = dy.device
     if want_dx:
-        _need(w_t is not None and w_t.dim() == 2 and tuple(w_t.shape) == (pool.K, pool.N), name, f"w_t [{pool.K}, {pool.N}] expected")
-    with _on(dy):
-        p = _pool_down(name, dy, pool.b_down, plan.ids, pool)
-        dx = _pool_gemm(name, dy, w_t, None, p, pool.a_up, plan.ids, pool, torch.bfloat16) if want_dx else None
-        dA = _pool_tn(name, x, p, plan, pool, pool.K, True)
-        dB = _pool_tn(name, dy, down, plan, pool, pool.N, False)
+        if w_t is None:
+            _bad(name, "dx needs w_t")
+        w_t, ldw = _bf16_rows(name, "w_t", w_t, K, N)
+        dx = torch.empty((M, K), dtype=torch.bfloat16, device=device)
+    dA = torch.empty((n, pool.r, K), dtype=torch.float32, device=device)
+    dB = torch.empty((n, N, pool.r), dtype=torch.float32, device=device)
+    nws = _lib.lib().mfnet_lora_pool_bwd_workspace_floats(M, n, K, N, RP)
+    ws = torch.empty(nws, dtype=torch.float32, device=device)
+    _launch("mfnet_lora_pool_bwd", dev, 2 * M * (N + (2 * K if want_dx else 0)) + 4 * (dA.numel() + dB.numel()) + (2 * N * K if want_dx else 0),
+            2.0 * M * ((N * K if want_dx else 0) + pool.r * (2 * N + 2 * K)), dy.data_ptr(), lddy, *src, w_t.data_ptr() if want_dx else None, ldw,
+            pool.scale.data_ptr(), pool.b_down, pool.a_up, plan.ids.data_ptr(), plan.perm.data_ptr(), plan.base.data_ptr(), plan.table.data_ptr(), n, pool.r, RP,
+            down.data_ptr(), _p(dx), K, dA.data_ptr(), dB.data_ptr(), _p(ws), nws, M, N, K)
     return dx, dA, dB

@@ -30,19 +30,23 @@ def test_entry_points_refuse_bad_arguments_before_a_launch():
     a = list(bwd)
     a[13] = a[14] = 16
     assert L.mfnet_layernorm_bwd_ckpt8(*a) == -1 and b"workspace" in E()
-    assert L.mfnet_lora_pool_pack(16, 0, 0, 2, 64, 20, 16, 16, 16, None) == -1 and b"sizes" in E()
-    assert L.mfnet_lora_pool_pack(16, 0, 0, 2, 60, 4, 16, 16, 16, None) == -1
-    assert L.mfnet_lora_pool_pack(16, 0, 0, 2, 64, 4, 24, 16, 16, None) == -1
+    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 64, 64, 20, 16, 16, 16, 16, 16, None) == -1 and b"sizes" in E()          # rank above its padding
+    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 60, 64, 4, 16, 16, 16, 16, 16, None) == -1
+    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 64, 64, 4, 24, 16, 16, 16, 16, None) == -1
+    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 64, 64, 4, 16, 16, 16, None, 16, None) == -1 and b"null" in E()
+    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 64, 64, 4, 16, 16, 24, 16, 16, None) == -1 and b"misaligned" in E()
     assert L.mfnet_lora_pool_plan(16, 1 << 31, 2, 16, 16, 16, 16, None) == -1 and b"sizes" in E()
     assert L.mfnet_lora_pool_plan(None, 8, 2, 16, 16, 16, 16, None) == -1 and b"null" in E()
-    assert L.mfnet_lora_pool_down(16, 60, 16, 16, 16, 2, 16, 16, 8, 64, None) == -1 and b"stride" in E()
-    assert L.mfnet_lora_pool_down(16, 64, 16, 16, 16, 2, 17, 16, 8, 64, None) == -1 and b"sizes" in E()
-    assert L.mfnet_lora_pool_gemm(16, 64, 16, 64, None, 16, None, None, 2, 16, 16, 1, 64, 8, 64, 64, None) == -1 and b"null" in E()
-    assert L.mfnet_lora_pool_gemm(16, 64, 24, 64, None, None, None, None, 0, 0, 16, 1, 64, 8, 64, 64, None) == -1 and b"weight" in E()
-    assert L.mfnet_lora_pool_gemm(16, 64, 16, 64, None, None, None, None, 0, 0, 16, 1, 64, 8, 60, 64, None) == -1 and b"out" in E()
-    assert L.mfnet_lora_pool_tn(16, 64, 16, 16, 16, 16, 16, 16, 16, 8, 2, 64, 4, 0, 16, 16, 1 << 20, None) == -1 and b"null" in E()     # rows twice
-    assert L.mfnet_lora_pool_tn(16, 64, None, None, 16, 16, 16, 16, 16, 8, 2, 64, 4, 0, 16, 16, 8, None) == -1 and b"workspace" in E()
-    assert L.mfnet_lora_pool_tn(16, 64, None, None, 16, 16, 16, 16, 16, 8, 2, 64, 17, 0, 16, 16, 1 << 20, None) == -1
+    fwd = dict(X=16, ldx=64, W=16, ldw=64, bias=None, scale=16, a_down=16, b_up=16, ids=16, n=2, RP=16, down=16, out=16, dt=1, ldo=64, M=8, N=64, K=64, s=None)
+    for key, v, msg in (("ldx", 60, b"row stride"), ("K", 60, b"multiple of 8"), ("X", 24, b"16-byte"), ("W", None, b"null"), ("ldw", 56, b"weight"), ("ldo", 62, b"out"),
+                        ("RP", 17, b"sizes"), ("n", 0, b"sizes"), ("M", 1 << 31, b"sizes"), ("dt", 2, b"dtype"), ("down", None, b"null"), ("b_up", 24, b"misaligned"), ("ids", None, b"null")):
+        assert L.mfnet_lora_pool_fwd(*dict(fwd, **{key: v}).values()) == -1 and msg in E(), key
+    assert L.mfnet_lora_pool_fwd(*dict(fwd, M=0).values()) == 0
+    bwd = dict(dy=16, lddy=64, X=16, ldx=64, codes=None, exps=None, Wt=16, ldwt=64, scale=16, b_down=16, a_up=16, ids=16, perm=16, base=16, table=16, n=2, r=4, RP=16, down=16,
+               dx=16, lddx=64, dA=16, dB=16, ws=16, nws=1 << 20, M=8, N=64, K=64, s=None)
+    for key, v, msg in (("codes", 16, b"either"), ("X", None, b"either"), ("lddy", 60, b"dy"), ("ldx", 60, b"(x)"), ("ldwt", 56, b"weight"), ("lddx", 60, b"dx"), ("r", 17, b"sizes"),
+                        ("nws", 100, b"workspace"), ("dA", None, b"null"), ("table", 24, b"misaligned"), ("K", 68, b"multiples of 8"), ("Wt", None, b"null"), ("down", None, b"null")):
+        assert L.mfnet_lora_pool_bwd(*dict(bwd, **{key: v}).values()) == -1 and msg in E(), key
 
 
 def test_sizes():
@@ -56,7 +60,7 @@ def test_sizes():
             one_each = min(n, M)
             worst = (one_each - 1) + -(-(M - one_each + 1) // ch)
             assert c >= worst
-            assert L.mfnet_lora_pool_tn_workspace_floats(M, n, 64, 32) == c * 64 * 32
+            assert L.mfnet_lora_pool_bwd_workspace_floats(M, n, 64, 72, 32) == M * 32 + c * (64 + 72) * 32
 
 
 def test_wrappers_refuse_host_tensors():
