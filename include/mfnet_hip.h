@@ -535,8 +535,9 @@ int64_t mfnet_layernorm_ckpt8_workspace_floats(int64_t rows, int64_t C);
 
 /* ---- A pool of n low-rank adapters beside one frozen projection: row m takes adapter ids[m] (int32 on the device; none if it lies
  * outside [0, n)), the rows of a call in any order (loralib/layers.py:149-165 has one adapter per modality and call).
- * Factors are bf16 images padded to RP = 16, 32 or 64 ranks: a "down" image [n][RP][C] (the product contracts over C) and an "up" image
- * [n][C][RP] (it contracts over the ranks) of each; pack writes all four from A [n][r][K] and B [n][N][r], fp32 or bf16. K and N are
+ * Factors are bf16 images padded to RP = 16, 32 or 64 ranks: of each a "down" image of n * mfnet_lora_pool_image_elements(C, RP)
+ * elements, in MFMA operand order (the product contracts over C), and an "up" image [n][C][RP] (it contracts over the ranks); pack
+ * writes all four from A [n][r][K] and B [n][N][r], fp32 or bf16. K and N are
  * multiples of 8, rows 16-byte aligned with strides that are multiples of 8; M < 2^31 - 256, n <= 65535. No call synchronises,
  * allocates or uses atomics; the same inputs give the same bits. An adapter's or a row's infinities and NaN reach only the rows of that
  * adapter, or that row, and their gradients. */
@@ -546,6 +547,7 @@ int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, int64_t n, int
  * [4 * mfnet_lora_pool_chunks(M, n)] int32 (16-byte aligned). Depends on ids alone: one per batch serves all of its layers. */
 int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* offs, int* perm, int* base, int* table, hipStream_t stream);
 int64_t mfnet_lora_pool_chunks(int64_t M, int64_t n);
+int64_t mfnet_lora_pool_image_elements(int64_t C, int RP);
 /* down [M, RP] fp32 = scale[i] * A_i x_m (zeros for rows without an adapter; the backward pass reads it),
  * out [M, N] bf16 | fp32 = x W^T (+ bias) + B_i down; X bf16 [M, K], W bf16 [N, K], bias fp32 [N] or NULL. */
 int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* scale, const void* a_down,

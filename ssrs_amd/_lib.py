@@ -146,6 +146,7 @@ _SIGS = {
 _HELPERS = {
     "mfnet_layernorm_ckpt8_workspace_floats": (c_int64, [I64, I64]),
     "mfnet_lora_pool_chunks": (c_int64, [I64, I64]),
+    "mfnet_lora_pool_image_elements": (c_int64, [I64, I]),
     "mfnet_lora_pool_bwd_workspace_floats": (c_int64, [I64, I64, I64, I64, I]),
 }
 

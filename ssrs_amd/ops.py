@@ -1848,11 +1848,12 @@ def lora_pool(A, B, scale=None) -> LoraPool:
     else:
         _vec_f32(name, "scale", scale, n)
         p.scale = scale.detach().clone()
-    p.buf = torch.empty(2 * n * RP * (K + N), dtype=torch.bfloat16, device=A.device)
+    K64, N64 = (K + 63) // 64 * 64, (N + 63) // 64 * 64    # the down images end in zeros up to a multiple of 64 columns
+    p.buf = torch.empty(n * RP * (K64 + K + N64 + N), dtype=torch.bfloat16, device=A.device)
     p.a_down = p.buf.data_ptr()                           # device addresses of the four images: every one a multiple of 16 bytes
-    p.a_up = p.a_down + 2 * n * RP * K
+    p.a_up = p.a_down + 2 * n * RP * K64
     p.b_down = p.a_up + 2 * n * RP * K
-    p.b_up = p.b_down + 2 * n * RP * N
+    p.b_up = p.b_down + 2 * n * RP * N64
     _launch("mfnet_lora_pool_pack", dev, A.element_size() * n * r * (K + N) + 2 * p.buf.numel(), 0, A.data_ptr(), B.data_ptr(), dt, n, K, N, r, RP,
             p.a_down, p.a_up, p.b_down, p.b_up)
     return p
