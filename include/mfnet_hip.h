@@ -527,7 +527,8 @@ int mfnet_layernorm_fwd_ckpt8(const void* x, int x_dtype, int64_t ldx, const flo
                               float* rstd, void* codes, void* exps, int64_t rows, int64_t C, float eps, hipStream_t stream);
 /* With xh = (x8 - mean) rstd and t = dy gamma: dx = rstd (t - mean(t) - xh mean(t xh)) (+ dres), written as fp32 (dx) and / or bf16
  * (dx_bf16), all dense [rows, C]; y (optional, needs beta) = bf16(xh gamma + beta), the LayerNorm output again; dgamma = sum dy xh and
- * dbeta = sum dy (both or neither; overwritten; ws of mfnet_layernorm_ckpt8_workspace_floats). Deterministic: no atomics. */
+ * dbeta = sum dy (both or neither; overwritten; ws of mfnet_layernorm_ckpt8_workspace_floats). Deterministic: no atomics. dy = NULL with
+ * neither dx: y alone. */
 int mfnet_layernorm_bwd_ckpt8(const void* dy, int dy_dtype, int64_t lddy, const void* codes, const void* exps, const float* mean,
                               const float* rstd, const float* gamma, const float* beta, const float* dres, float* dx, void* dx_bf16, void* y,
                               float* dgamma, float* dbeta, float* ws, int64_t ws_floats, int64_t rows, int64_t C, hipStream_t stream);
@@ -537,12 +538,12 @@ int64_t mfnet_layernorm_ckpt8_workspace_floats(int64_t rows, int64_t C);
  * outside [0, n)), the rows of a call in any order (loralib/layers.py:149-165 has one adapter per modality and call).
  * Factors are bf16 images padded to RP = 16, 32 or 64 ranks: of each a "down" image of n * mfnet_lora_pool_image_elements(C, RP)
  * elements, in MFMA operand order (the product contracts over C), and an "up" image [n][C][RP] (it contracts over the ranks); pack
- * writes all four from A [n][r][K] and B [n][N][r], fp32 or bf16. K and N are
+ * writes all four from A [n][r][K] and B [n][N][r], fp32 or bf16, and copies scale [n] (NULL: ones). K and N are
  * multiples of 8, rows 16-byte aligned with strides that are multiples of 8; M < 2^31 - 256, n <= 65535. No call synchronises,
  * allocates or uses atomics; the same inputs give the same bits. An adapter's or a row's infinities and NaN reach only the rows of that
  * adapter, or that row, and their gradients. */
-int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, int64_t n, int64_t K, int64_t N, int r, int RP, void* a_down, void* a_up,
-                         void* b_down, void* b_up, hipStream_t stream);
+int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, const float* scale, int64_t n, int64_t K, int64_t N, int r, int RP,
+                         void* a_down, void* a_up, void* b_down, void* b_up, float* scale_out, hipStream_t stream);
 /* Rows grouped by adapter, ascending inside each: offs [n + 1], perm [M], and chunks of rows for the backward sums: base [n + 1], table
  * [4 * mfnet_lora_pool_chunks(M, n)] int32 (16-byte aligned). Depends on ids alone: one per batch serves all of its layers. */
 int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* offs, int* perm, int* base, int* table, hipStream_t stream);

@@ -279,7 +279,7 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void ln_bwd_ckpt8_kernel(const T* _
     for (int j = 0; j < NV; ++j) {
       const int c = 4 * (lane + 64 * j);
       const bool on = c < C;
-      d[j] = on ? load4(dy + row * lddy + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      d[j] = on && dy ? load4(dy + row * lddy + c) : make_float4(0.f, 0.f, 0.f, 0.f);
       w[j] = on ? *reinterpret_cast<const unsigned int*>(codes + row * C + c) : 0u;
       by[j] = on ? exps[row * (C >> 5) + (c >> 5)] : 0u;
       if (dres) r[j] = on ? *reinterpret_cast<const float4*>(dres + row * C + c) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -485,12 +485,13 @@ extern "C" int mfnet_layernorm_bwd_ckpt8(const void* dy, int dy_dtype, int64_t l
   MF_CHECK_ARG(ck_dtype(dy_dtype), "layernorm_bwd_ckpt8: bad dtype");
   MF_CHECK_ARG((dgamma == nullptr) == (dbeta == nullptr), "layernorm_bwd_ckpt8: dgamma and dbeta go together");
   const bool wg = dgamma != nullptr;
-  MF_CHECK_ARG(rows == 0 || (dy && codes && exps && mean && rstd && gamma && (dx || dx_bf16)), "layernorm_bwd_ckpt8: null pointer");
+  MF_CHECK_ARG(rows == 0 || (codes && exps && mean && rstd && gamma && (dy ? dx || dx_bf16 : y && !dx && !dx_bf16 && !wg)),
+               "layernorm_bwd_ckpt8: null pointer (dy with dx, or y alone)");
   MF_CHECK_ARG(!y || beta, "layernorm_bwd_ckpt8: y needs beta");
   const int64_t n = rows ? ln_ck_wgs(rows) : 0;
   MF_CHECK_ARG(!wg || n == 0 || (ws && ws_floats >= n * 2 * C), "layernorm_bwd_ckpt8: workspace too small");
   if (rows) {
-    MF_CHECK_ARG(lddy >= C && lddy % 4 == 0, "layernorm_bwd_ckpt8: lddy must be >= C and a multiple of 4");
+    MF_CHECK_ARG(!dy || (lddy >= C && lddy % 4 == 0), "layernorm_bwd_ckpt8: lddy must be >= C and a multiple of 4");
     MF_CHECK_ARG(((uintptr_t)gamma | (uintptr_t)beta | (uintptr_t)dres | (uintptr_t)dx) % 16 == 0 && (uintptr_t)dy % (dy_dtype == MFNET_F32 ? 16 : 8) == 0 &&
                  ((uintptr_t)dx_bf16 | (uintptr_t)y) % 8 == 0 && (uintptr_t)codes % 4 == 0, "layernorm_bwd_ckpt8: misaligned tensor");
 #define LNB(T_, NV_, W_) hipLaunchKernelGGL((ln_bwd_ckpt8_kernel<T_, NV_, W_>), dim3((unsigned)n), dim3(64 * LNB_WAVES), W_ ? 2 * (size_t)C * 4 : 0, stream, (const T_*)dy, lddy, \

@@ -56,7 +56,7 @@ __device__ __forceinline__ int next_id(int cand) {
 // The "down" image is kept in MFMA operand order: [n][k-step of 32][RP / 16][lane][8], lane = (rank % 16) + 16 (k % 32 / 8), zeros behind
 // the last column up to a multiple of 64: a fragment is one dense KB. The "up" image is [n][C][RP].
 __device__ __host__ __forceinline__ int64_t pool_image(int64_t C, int RP) { return (C + 63) / 64 * 64 * RP; }      // elements of a down image per adapter
-struct PoolPack { const void* src[2]; bf16_t* down[2]; bf16_t* up[2]; int C[2], r, RP; };
+struct PoolPack { const void* src[2]; bf16_t* down[2]; bf16_t* up[2]; int C[2], r, RP; const float* scale; float* scale_out; };
 template <typename T>
 __global__ __launch_bounds__(256) void pool_pack_kernel(const PoolPack p) {
   const int z = blockIdx.z, C = p.C[z], r = p.r, RP = p.RP;                    // z = 0: A [n][r][K], 1: B [n][N][r]
@@ -67,6 +67,7 @@ __global__ __launch_bounds__(256) void pool_pack_kernel(const PoolPack p) {
     const T t = z ? s[(int64_t)c * r + k] : s[(int64_t)k * C + c];
     if constexpr (sizeof(T) == 4) return t; else return bf16_to_f32(t);
   };
+  if (z == 0 && blockIdx.x == 0 && threadIdx.x == 0) p.scale_out[i] = p.scale ? p.scale[i] : 1.f;
   const int chunks = (C + 63) / 64 * 8 * RP;                                   // 16-byte pieces of the down image, then of the up image
   const int t = blockIdx.x * 256 + threadIdx.x;
   float v[8];
@@ -975,16 +976,16 @@ static bool pool_rows(const void* t, int64_t ld, int64_t C) { return C >= 8 && C
 
 extern "C" int64_t mfnet_lora_pool_image_elements(int64_t C, int RP) { return C < 0 ? 0 : pool_image(C, RP); }
 
-extern "C" int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, int64_t n, int64_t K, int64_t N, int r, int RP, void* a_down, void* a_up,
-                                    void* b_down, void* b_up, hipStream_t stream) {
-  MF_CHECK_ARG(A && B && a_down && a_up && b_down && b_up, "lora_pool_pack: null pointer");
+extern "C" int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, const float* scale, int64_t n, int64_t K, int64_t N, int r, int RP,
+                                    void* a_down, void* a_up, void* b_down, void* b_up, float* scale_out, hipStream_t stream) {
+  MF_CHECK_ARG(A && B && a_down && a_up && b_down && b_up && scale_out, "lora_pool_pack: null pointer");
   MF_CHECK_ARG(dtype == MFNET_F32 || dtype == MFNET_BF16, "lora_pool_pack: bad dtype");
   MF_CHECK_ARG(n >= 1 && n <= 65535 && pool_rows(a_down, K, K) && pool_rows(b_down, N, N) && r >= 1 && r <= RP && pool_rp(RP),
                "lora_pool_pack: bad sizes (n=%lld K=%lld N=%lld r=%d RP=%d)", (long long)n, (long long)K, (long long)N, r, RP);
   MF_CHECK_ARG(((uintptr_t)A | (uintptr_t)B) % (dtype == MFNET_F32 ? 4 : 2) == 0 && ((uintptr_t)a_up | (uintptr_t)b_up) % 16 == 0, "lora_pool_pack: misaligned tensor");
   PoolPack p;
   p.src[0] = A; p.src[1] = B; p.down[0] = (bf16_t*)a_down; p.down[1] = (bf16_t*)b_down; p.up[0] = (bf16_t*)a_up; p.up[1] = (bf16_t*)b_up;
-  p.C[0] = (int)K; p.C[1] = (int)N; p.r = r; p.RP = RP;
+  p.C[0] = (int)K; p.C[1] = (int)N; p.r = r; p.RP = RP; p.scale = scale; p.scale_out = scale_out;
   const int64_t L = K > N ? K : N;
   const dim3 grid((unsigned)ceil_div64((ceil_div64(L, 64) * 64 + L) * RP / 8, 256), (unsigned)n, 2);
   if (dtype == MFNET_F32) hipLaunchKernelGGL(pool_pack_kernel<float>, grid, dim3(256), 0, stream, p);

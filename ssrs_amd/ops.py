@@ -1650,6 +1650,9 @@ class Ckpt8:
     __slots__ = ("buf", "shape", "rows", "C", "at_exps")
 
     def __init__(self, shape, device):
+        self.buf = torch.empty(self._place(shape), dtype=torch.uint8, device=device)
+
+    def _place(self, shape):
         self.shape = tuple(shape)
         self.C = C = self.shape[-1]
         rows = 1
@@ -1657,7 +1660,7 @@ class Ckpt8:
             rows *= d
         self.rows = rows
         self.at_exps = (rows * C + 15) // 16 * 16
-        self.buf = torch.empty(self.at_exps + rows * ((C + 31) // 32), dtype=torch.uint8, device=device)
+        return self.at_exps + rows * ((C + 31) // 32)
 
     @property
     def device(self):
@@ -1678,6 +1681,14 @@ class Ckpt8:
     def _ptrs(self):
         p = self.buf.data_ptr()
         return p, p + self.at_exps
+
+    @classmethod
+    def of(cls, buf, shape):
+        """the checkpoint whose buffer was kept by itself (autograd keeps tensors)"""
+        c = cls.__new__(cls)
+        c._place(shape)
+        c.buf = buf
+        return c
 
 
 def _ck_dtype(name, t):
@@ -1816,10 +1827,30 @@ def layernorm_bwd_ckpt8(dy, c: Ckpt8, mean, rstd, gamma, beta=None, dres=None, w
     return out[0] if len(out) == 1 else tuple(out)
 
 
+def layernorm_y_ckpt8(c: Ckpt8, mean, rstd, gamma, beta):
+    """the LayerNorm output again (bf16) from the checkpoint of its input: what layernorm_bwd_ckpt8(want_y=True) returns, alone."""
+    name = "layernorm_y_ckpt8"
+    dev = _device_of(name, c.buf, mean, rstd, gamma, beta)
+    C, rows = c.C, c.rows
+    if C % 32 or C > 2048:
+        _bad(name, f"C={C} must be a multiple of 32, at most 2048")
+    _vec_f32(name, "mean", mean, rows)
+    _vec_f32(name, "rstd", rstd, rows)
+    _vec_f32(name, "gamma", gamma, C)
+    _vec_f32(name, "beta", beta, C)
+    gamma, beta = _aligned(gamma), _aligned(beta)
+    y = torch.empty(c.shape, dtype=torch.bfloat16, device=c.buf.device)
+    codes, exps = c._ptrs()
+    _launch("mfnet_layernorm_bwd_ckpt8", dev, 2 * rows * C + c.nbytes + 8 * rows, 0, None, BF16, 0, codes, exps, mean.data_ptr(), rstd.data_ptr(),
+            gamma.data_ptr(), beta.data_ptr(), None, None, None, y.data_ptr(), None, None, None, 0, rows, C)
+    return y
+
+
 # ------------------------------------------------------------------------------------------ pooled low-rank adapters
 class LoraPool:
     """n low-rank adapters of one layer, laid out for the kernels (lora_pool): bf16 images of A [n, r, K] and B [n, N, r] padded to
-    RP = 16, 32 or 64 ranks, one per direction of use. A copy: later changes of A and B do not reach it."""
+    RP = 16, 32 or 64 ranks, one per direction of use, and
+    the scales. A copy: later changes of A, B and scale do not reach it."""
     __slots__ = ("n", "r", "K", "N", "RP", "scale", "buf", "a_down", "a_up", "b_down", "b_up")
 
 
@@ -1843,19 +1874,17 @@ def lora_pool(A, B, scale=None) -> LoraPool:
     p.n, p.r, p.K, p.N = n, r, K, N
     p.RP = RP = 16 if r <= 16 else 32 if r <= 32 else 64
     A, B = A.detach().contiguous(), B.detach().contiguous()
-    if scale is None:
-        p.scale = torch.ones(n, dtype=torch.float32, device=A.device)
-    else:
+    if scale is not None:
         _vec_f32(name, "scale", scale, n)
-        p.scale = scale.detach().clone()
     K64, N64 = (K + 63) // 64 * 64, (N + 63) // 64 * 64    # the down images end in zeros up to a multiple of 64 columns
-    p.buf = torch.empty(n * RP * (K64 + K + N64 + N), dtype=torch.bfloat16, device=A.device)
+    p.buf = torch.empty(n * RP * (K64 + K + N64 + N) + 2 * n, dtype=torch.bfloat16, device=A.device)
     p.a_down = p.buf.data_ptr()                           # device addresses of the four images: every one a multiple of 16 bytes
     p.a_up = p.a_down + 2 * n * RP * K64
     p.b_down = p.a_up + 2 * n * RP * K
     p.b_up = p.b_down + 2 * n * RP * N64
-    _launch("mfnet_lora_pool_pack", dev, A.element_size() * n * r * (K + N) + 2 * p.buf.numel(), 0, A.data_ptr(), B.data_ptr(), dt, n, K, N, r, RP,
-            p.a_down, p.a_up, p.b_down, p.b_up)
+    p.scale = p.b_up + 2 * n * RP * N                     # fp32 [n]
+    _launch("mfnet_lora_pool_pack", dev, A.element_size() * n * r * (K + N) + 2 * p.buf.numel(), 0, A.data_ptr(), B.data_ptr(), dt, _p(scale), n, K, N, r, RP,
+            p.a_down, p.a_up, p.b_down, p.b_up, p.scale)
     return p
 
 
@@ -1918,7 +1947,7 @@ def lora_pool_fwd(x, w, bias, pool: LoraPool, ids, out_dtype=torch.bfloat16, wan
     down = torch.empty((M, pool.RP), dtype=torch.float32, device=x.device)
     out = torch.empty((M, N), dtype=out_dtype, device=x.device)
     _launch("mfnet_lora_pool_fwd", dev, 2 * (M * K + N * K + pool.n * pool.r * (K + N)) + M * N * (2 if od else 4), 2.0 * M * (N * K + pool.r * (N + K)),
-            x.data_ptr(), ldx, w.data_ptr(), ldw, _p(bias), pool.scale.data_ptr(), pool.a_down, pool.b_up, ids.data_ptr(), pool.n, pool.RP, down.data_ptr(),
+            x.data_ptr(), ldx, w.data_ptr(), ldw, _p(bias), pool.scale, pool.a_down, pool.b_up, ids.data_ptr(), pool.n, pool.RP, down.data_ptr(),
             out.data_ptr(), od, N, M, N, K)
     return (out, down) if want_down else out
 
@@ -1956,6 +1985,6 @@ def lora_pool_bwd(dy, x, w_t, pool: LoraPool, plan: LoraPlan, down, want_dx=True
     ws = torch.empty(nws, dtype=torch.float32, device=device)
     _launch("mfnet_lora_pool_bwd", dev, 2 * M * (N + (2 * K if want_dx else 0)) + 4 * (dA.numel() + dB.numel()) + (2 * N * K if want_dx else 0),
             2.0 * M * ((N * K if want_dx else 0) + pool.r * (2 * N + 2 * K)), dy.data_ptr(), lddy, *src, w_t.data_ptr() if want_dx else None, ldw,
-            pool.scale.data_ptr(), pool.b_down, pool.a_up, plan.ids.data_ptr(), plan.perm.data_ptr(), plan.base.data_ptr(), plan.table.data_ptr(), n, pool.r, RP,
+            pool.scale, pool.b_down, pool.a_up, plan.ids.data_ptr(), plan.perm.data_ptr(), plan.base.data_ptr(), plan.table.data_ptr(), n, pool.r, RP,
             down.data_ptr(), _p(dx), K, dA.data_ptr(), dB.data_ptr(), _p(ws), nws, M, N, K)
     return dx, dA, dB

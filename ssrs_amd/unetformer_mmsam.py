@@ -281,13 +281,13 @@ class UNetFormer(nn.Module):
     """MFNet. Extra keyword arguments (not in the reference, all optional): `encoder` selects the SAM
     size ('vit_b' | 'vit_l' | 'vit_h'; the reference hard-codes 'vit_l' and is edited by hand,
     unetformer_mmsam.py:488-490; env MFNET_ENCODER overrides the default), `sam_checkpoint` the local
-    .pth, `args` a pre-parsed cfg namespace instead of sys.argv, `precision` 'bf16' | 'fp32' (see __init__)."""
+    .pth, `args` a pre-parsed cfg namespace instead of sys.argv, `precision` 'bf16' | 'fp32', `checkpoints` 'bf16' | 'int8' (see __init__)."""
 
     _CKPT = {"vit_b": "weights/sam_vit_b_01ec64.pth", "vit_l": "weights/sam_vit_l_0b3195.pth",
              "vit_h": "weights/sam_vit_h_4b8939.pth", "default": "weights/sam_vit_b_01ec64.pth"}
 
     def __init__(self, decode_channels=64, dropout=0.1, window_size=8, num_classes=6, *, encoder=None,
-                 sam_checkpoint=None, args=None, precision=None):
+                 sam_checkpoint=None, args=None, precision=None, checkpoints=None):
         super().__init__()
         # "bf16" (default): bf16 MFMA contractions with fp32 accumulation, training + inference, logits within 2e-2 of the fp32
         # reference. "fp32": every contraction on the fp32 MFMA, fp32 activations and gradients: logits within 1e-4, gradients
@@ -328,6 +328,27 @@ class UNetFormer(nn.Module):
         for n, p in self.image_encoder.named_parameters():
             p.requires_grad = token in n
         self.decoder = Decoder(ec, decode_channels, dropout, window_size, num_classes)
+        # what an MMLoRA encoder block keeps between its forward and its backward pass. "bf16" (default): the fp32 residual stream, the
+        # LayerNorm outputs, lin1's output and GELU of it. "int8": the residual stream and lin1's output in 8 bits (ops.Ckpt8), the rest
+        # is made again - 2.6x less memory per block, the same forward, gradients that see the rounded activations. Choose before the
+        # first training step; fp32 mode keeps everything.
+        self.checkpoints = checkpoints or "bf16"
+
+    @property
+    def checkpoints(self):
+        return self._checkpoints
+
+    @checkpoints.setter
+    def checkpoints(self, kind):
+        if kind not in ("bf16", "int8"):
+            raise ValueError(f"checkpoints {kind!r}: 'bf16' or 'int8'")
+        if kind == "int8" and self.mod != "sam_lora":
+            raise NotImplementedError("8-bit activation checkpoints exist for the MMLoRA encoder (mod 'sam_lora')")
+        if kind == "int8" and self.precision == "fp32":
+            raise ValueError("8-bit activation checkpoints are a bf16-mode option: precision 'fp32' keeps every activation")
+        self._checkpoints = kind
+        for blk in self.image_encoder.blocks:
+            blk.checkpoint8 = kind == "int8"
 
     def forward(self, x, y, mode='Train'):
         if x.shape[-2] % 32 or x.shape[-1] % 32:

@@ -170,6 +170,22 @@ def _attention_bwd(qkv, attn_mod, tb, o, dO, lse, G, Sh, Sw, heads, ws):
     return ops.attn_bwd(qkv, attn_mod.qkv.bias, tbl, tblT, o, dO, lse, G, Sh, Sw, heads, ws, Lh, Lw, hd ** -0.5)
 
 
+def _keeps8(blk, ctx):
+    """activations of this branch kept in 8 bits until the backward pass: asked for (UNetFormer(checkpoints="int8")), a backward pass may
+    come, bf16 mode, and a row length the kernels take"""
+    C = blk.norm1.weight.shape[0]
+    return getattr(blk, "checkpoint8", False) and not ops.FP32 and any(ctx.needs_input_grad) and C % 32 == 0 and C <= 2048
+
+
+def _down8(ln, A_x, A_y, half, wx=None, wy=None):
+    """(a, U) of a LayerNorm output that layernorm_fwd_ckpt8 made: the row-streaming kernel where it fits, the general products else"""
+    r, K = A_x.shape
+    if r in (4, 8) and half % 2 == 0 and K % 8 == 0 and K <= 4096 and 2 * r * K * 2 + 512 <= 96 * 1024 and ln.shape[0] == 2 * half:
+        return ops.lora_down_mix(ln, _stack2("A", A_x, A_y), wx, wy)
+    a = _down(ln, A_x, A_y, half)
+    return a, (ops.lora_mix_fwd(a, wx, wy) if wx is not None else None)
+
+
 @ops.keeps_precision
 class _LoraAttnBranch(torch.autograd.Function):
     """h -> h + proj(attn(qkv_lora(LN1(h))))  for the stacked token matrix (lora_block.py:64-82)."""
@@ -183,7 +199,11 @@ class _LoraAttnBranch(torch.autograd.Function):
         half = M // 2
         r = Ax.shape[0] // 2
         h2 = h.reshape(M, D)
-        if 2 * r in (4, 8) and half % 2 == 0 and _ln_lora_fits(2 * r, D):      # LayerNorm and the down-projection a = LN(h) @ A_g^T in one launch
+        ck = None
+        if _keeps8(blk, ctx):                    # h in 8 bits beside its statistics instead of h and LN(h)
+            ln, mean, rstd, ck = ops.layernorm_fwd_ckpt8(h2, blk.norm1.weight, blk.norm1.bias, blk.norm1.eps)
+            a = _down8(ln, Ax, Ay, half)[0]
+        elif 2 * r in (4, 8) and half % 2 == 0 and _ln_lora_fits(2 * r, D):      # LayerNorm and the down-projection a = LN(h) @ A_g^T in one launch
             ln, mean, rstd, a, _ = ops.layernorm_fwd_lora(h2, blk.norm1.weight, blk.norm1.bias, blk.norm1.eps, _stack2("A", Ax, Ay))
         else:
             ln, mean, rstd = ops.layernorm_fwd(h2, blk.norm1.weight, blk.norm1.bias, blk.norm1.eps)
@@ -193,7 +213,11 @@ class _LoraAttnBranch(torch.autograd.Function):
                        n_groups=2, lr_scale=1.0 / r)
         o, lse, tb = _attention(qkv, attn, 2 * B, Sh, Sw, heads, ws)
         out = ops.gemm(o, w_bf16(attn.proj.weight), bias=attn.proj.bias, residual=h2, out_dtype=torch.float32)
-        ctx.save_for_backward(h2, mean, rstd, ln, a, qkv, o, lse)          # (lse: None in fp32 mode)
+        if ck is not None:
+            ctx.save_for_backward(ck.buf, mean, rstd, None, a, qkv, o, lse)
+        else:
+            ctx.save_for_backward(h2, mean, rstd, ln, a, qkv, o, lse)      # (lse: None in fp32 mode)
+        ctx.kept8 = None if ck is None else ck.shape
         ctx.blk, ctx.geom, ctx.tb = blk, geom, tb
         ctx.params = (Ax, Ay, Bx, By)
         return out.view(h.shape)
@@ -204,7 +228,8 @@ class _LoraAttnBranch(torch.autograd.Function):
         blk, (B, Sh, Sw, heads, ws) = ctx.blk, ctx.geom
         Ax, Ay, Bx, By = ctx.params
         attn = blk.attn
-        M, D = h2.shape
+        ck = None if ctx.kept8 is None else ops.Ckpt8.of(h2, ctx.kept8)
+        M, D = h2.shape if ck is None else ck.shape
         half = M // 2
         r = Ax.shape[0] // 2
         hd = D // heads
@@ -213,6 +238,8 @@ class _LoraAttnBranch(torch.autograd.Function):
         dO = ops.gemm(d_bf, wT_bf16(attn.proj.weight))
         dqkv = _attention_bwd(qkv, attn, ctx.tb, o, dO, lse, 2 * B, Sh, Sw, heads, ws)
         s = 1.0 / r
+        if ck is not None:
+            ln = ops.layernorm_y_ckpt8(ck, mean, rstd, blk.norm1.weight, blk.norm1.bias)
         if 2 * r == 8 and not ops.FP32:
             # one pass over dqkv for d(xA^T) = dqkv . B (per modality) and dB = dqkv^T . a; one over ln for dA^T = ln^T . da
             dV, pp = ops.lora_side(dqkv, U=a, Vt=_qkv_lora_V(Bx, By, D, r, transposed=True), n_groups=2, scale=s)
@@ -227,10 +254,16 @@ class _LoraAttnBranch(torch.autograd.Function):
         rows_q, rows_v = slice(0, D), slice(D, 2 * D)
         grads = deliver((Ax, Ay, Bx, By), (dAx, dAy, [(rows_q, dVx[:D, :r]), (rows_v, dVx[2 * D:, r:])],
                                            [(rows_q, dVy[:D, :r]), (rows_v, dVy[2 * D:, r:])]))
+        if ck is not None:
+            del ln
+            ops.tn_flush()                       # a collected dA product would keep LN(h) in bf16 until the step's end
         if not ctx.needs_input_grad[0]:          # first block over a frozen patch embedding: nothing upstream wants dh
             return (None, None, None) + grads
         dln = ops.gemm(dqkv, wT_bf16(attn.qkv.weight), U=da, V=_stack2("A", Ax, Ay, transpose=True), rows_per_group=half, n_groups=2)
-        dh, dh_bf = ops.layernorm_bwd(dln, h2, mean, rstd, blk.norm1.weight, dres=d2, want_bf16=True)
+        if ck is not None:
+            dh, dh_bf = ops.layernorm_bwd_ckpt8(dln, ck, mean, rstd, blk.norm1.weight, dres=d2, want_bf16=True)
+        else:
+            dh, dh_bf = ops.layernorm_bwd(dln, h2, mean, rstd, blk.norm1.weight, dres=d2, want_bf16=True)
         ops.remember_bf16_twin(dh, dh_bf)
         return (dh.view(dout.shape), None, None) + grads
 
@@ -260,9 +293,20 @@ def _mix_linear_fwd(x_bf, lin, half, act, residual, aU=None):
 def _mix_linear_bwd(d_bf, x_bf, lin, saved, half, gelu_aux=None):
     """-> (dx bf16, (dAx, dAy, dBx, dBy, dwx, dwy) as strided views). d_bf: grad of the layer output (bf16,
     after any activation backward of the NEXT layer); gelu_aux: this layer's INPUT pre-activation if the
-    input was GELU(pre) (then dx is the grad w.r.t. pre)."""
+    input was GELU(pre) (then dx is the grad w.r.t. pre). x_bf may be a function instead: called with dx it
+    returns (dx of what lies before the input, the input) - an input that was kept in 8 bits."""
     a, U = saved
     r = a.shape[1]
+    if callable(x_bf):
+        da, dw, dV = _mix_linear_bwd_up(d_bf, lin, saved)
+        dx = ops.gemm(d_bf, wT_bf16(lin.weight), U=da, V=_stack2("A", lin.lora_Ax, lin.lora_Ay, transpose=True), rows_per_group=half, n_groups=2)
+        dx, x = x_bf(dx)
+        if 2 * r == 8:
+            dA = ops.lora_side(x, U=da, n_groups=2)[0]
+            dAx, dAy = dA[0].t(), dA[1].t()
+        else:
+            dAx, dAy = _tn_groups(x, da, half, True)
+        return dx, (dAx, dAy, dV[:, :r], dV[:, r:], dw[0:1], dw[1:2])
     if 2 * r == 8 and not ops.FP32:
         dV, pp = ops.lora_side(d_bf, U=U, Vt=_mix_V(lin, transposed=True))      # d_bf is read once for P = d . [Bx|By] and dB
         da, dw = ops.lora_mix_bwd(pp, a, lin.lora_wx, lin.lora_wy)
@@ -278,6 +322,18 @@ def _mix_linear_bwd(d_bf, x_bf, lin, saved, half, gelu_aux=None):
     return dx, (dAx, dAy, dV[:, :r], dV[:, r:], dw[0:1], dw[1:2])
 
 
+def _mix_linear_bwd_up(d_bf, lin, saved):
+    """the part of a lora.Linear backward that needs no input: (d(x A^T), d(wx, wy), d[Bx | By])"""
+    a, U = saved
+    if 2 * a.shape[1] == 8:
+        dV, pp = ops.lora_side(d_bf, U=U, Vt=_mix_V(lin, transposed=True))
+    else:
+        pp = ops.skinny_nt(d_bf, _mix_V(lin, transposed=True)).contiguous()
+        dV = ops.skinny_tn(d_bf, U, False, lazy=True)
+    da, dw = ops.lora_mix_bwd(pp, a, lin.lora_wx, lin.lora_wy)
+    return da, dw, dV
+
+
 @ops.keeps_precision
 class _LoraMlpBranch(torch.autograd.Function):
     """h -> h + lin2(gelu(lin1(LN2(h))))  with the cross-modal LoRA mix (lora_block.py:83-85,104-108)."""
@@ -289,6 +345,17 @@ class _LoraMlpBranch(torch.autograd.Function):
         half = M // 2
         h2 = h.reshape(M, D)
         l1 = blk.mlp.lin1
+        if _keeps8(blk, ctx):                    # kept in 8 bits: h (with its statistics) and lin1's output; not LN(h), not GELU(lin1)
+            l2 = blk.mlp.lin2
+            ln, mean, rstd, ck = ops.layernorm_fwd_ckpt8(h2, blk.norm2.weight, blk.norm2.bias, blk.norm2.eps)
+            s1 = _down8(ln, l1.lora_Ax, l1.lora_Ay, half, l1.lora_wx.detach(), l1.lora_wy.detach())
+            pre = _mix_linear_fwd(ln, l1, half, False, None, s1)[0]
+            act, ckp = ops.gelu_fwd_ckpt8(pre)
+            out, _, s2 = _mix_linear_fwd(act, l2, half, False, h2)
+            ctx.save_for_backward(ck.buf, mean, rstd, ckp.buf, None, None, *s1, *s2)
+            ctx.blk, ctx.kept8 = blk, (ck.shape, ckp.shape)
+            return out.view(h.shape)
+        ctx.kept8 = None
         if l1.lora_Ax.shape[0] in (4, 8) and half % 2 == 0 and _ln_lora_fits(l1.lora_Ax.shape[0], D):     # LayerNorm, lin1's down-projection and its cross-modal mix in one launch
             ln, mean, rstd, a1, U1 = ops.layernorm_fwd_lora(h2, blk.norm2.weight, blk.norm2.bias, blk.norm2.eps,
                                                             _stack2("A", l1.lora_Ax, l1.lora_Ay), l1.lora_wx.detach(), l1.lora_wy.detach())
@@ -306,6 +373,8 @@ class _LoraMlpBranch(torch.autograd.Function):
     def backward(ctx, dout):
         h2, mean, rstd, ln, act, pre, a1, U1, a2, U2 = ctx.saved_tensors
         blk = ctx.blk
+        if ctx.kept8 is not None:
+            return _LoraMlpBranch.backward8(blk, ops.Ckpt8.of(h2, ctx.kept8[0]), mean, rstd, ops.Ckpt8.of(ln, ctx.kept8[1]), (a1, U1), (a2, U2), dout)
         M, D = h2.shape
         half = M // 2
         d2 = dout.reshape(M, D).contiguous()
@@ -315,6 +384,25 @@ class _LoraMlpBranch(torch.autograd.Function):
         dh, dh_bf = ops.layernorm_bwd(dln, h2, mean, rstd, blk.norm2.weight, dres=d2, want_bf16=True)
         ops.remember_bf16_twin(dh, dh_bf)
         return (dh.view(dout.shape), None) + deliver(blk._mlp_params(), g1 + g2)     # order of LoraBlock._mlp_params()
+
+    @staticmethod
+    def backward8(blk, ck, mean, rstd, ckp, s1, s2, dout):
+        """the same from what was kept in 8 bits: GELU(lin1) and LN(h) are made again where their layer's dA needs them"""
+        M, D = ck.shape
+        half = M // 2
+        d2 = dout.reshape(M, D).contiguous()
+        norm = blk.norm2
+        dpre, g2 = _mix_linear_bwd(ops.bf16_of(d2), lambda dact: ops.gelu_bwd_ckpt8(ckp, dact, want_act=True), blk.mlp.lin2, s2, half)
+        kept = {}
+
+        def through_norm(dln):
+            kept["dh"], dh_bf, ln = ops.layernorm_bwd_ckpt8(dln, ck, mean, rstd, norm.weight, norm.bias, d2, want_bf16=True, want_y=True)
+            return dh_bf, ln
+        dh_bf, g1 = _mix_linear_bwd(dpre, through_norm, blk.mlp.lin1, s1, half)
+        dh = kept["dh"]
+        ops.remember_bf16_twin(dh, dh_bf)
+        ops.tn_flush()                           # the collected dA products would keep GELU(lin1) and LN(h) in bf16 until the step's end
+        return (dh.view(dout.shape), None) + deliver(blk._mlp_params(), g1 + g2)
 
 
 @ops.keeps_precision
@@ -493,6 +581,97 @@ class MergedLinear(nn.Linear, LoRALayer):
             out = ops.gemm(xb, w_bf16(self.weight), bias=self.bias, out_dtype=torch.float32)
         out = out.view(*h.shape[:-1], -1)
         return out[0], out[1]
+
+
+class PooledLinear(nn.Linear):
+    """One frozen projection with n low-rank adapters, the adapter of every row named by an index: many fine-tuned models' rows in one
+    call, for serving or for training them side by side (lora.Linear and lora.MergedLinear hold one adapter per modality).
+
+    forward(x, ids): x [..., in] fp32 or bf16, ids int32 - one per row (x.shape[:-1]) or one per entry of x's first dimension; an index
+    outside [0, n) takes the projection alone. -> [..., out] of x's dtype. lora_A [n, r, in] and lora_B [n, out, r] are trainable,
+    `scaling` [n] is a buffer; the factors are rounded to bf16 for the products, their gradients are fp32.
+    checkpoint8: keep the input in 8 bits until the backward pass (ops.Ckpt8; in multiples of 8). plan: ops.lora_pool_plan of the same
+    rows, to share one among the layers of a batch (None: the backward pass makes its own)."""
+
+    def __init__(self, in_features, out_features, n_adapters, r, lora_alpha=1, bias=True, checkpoint8=False):
+        super().__init__(in_features, out_features, bias=bias)
+        if not (1 <= int(r) <= 64 and 1 <= int(n_adapters) <= 65535):
+            raise ValueError(f"{n_adapters} adapters of rank {r}: 1 .. 65535 adapters of rank 1 .. 64")
+        if in_features % 8 or out_features % 8:
+            raise ValueError(f"in_features={in_features} and out_features={out_features} must be multiples of 8")
+        self.n_adapters, self.r, self.checkpoint8 = int(n_adapters), int(r), bool(checkpoint8)
+        self.weight.requires_grad = False
+        if self.bias is not None:
+            self.bias.requires_grad = False
+        self.lora_A = nn.Parameter(self.weight.new_zeros((n_adapters, r, in_features)))
+        self.lora_B = nn.Parameter(self.weight.new_zeros((n_adapters, out_features, r)))
+        self.register_buffer("scaling", torch.full((n_adapters,), lora_alpha / r, dtype=torch.float32))
+        for a in self.lora_A:
+            nn.init.kaiming_uniform_(a, a=math.sqrt(5))
+
+    @classmethod
+    def from_merged(cls, layers, checkpoint8=False):
+        """the pool of several fine-tuned lora.MergedLinear layers over the same frozen weight: adapters 2 i and 2 i + 1 are the x and y
+        modality of layers[i] (rank 2 r: r columns feed the q third of the output, r the v third)"""
+        first = layers[0]
+        r, D = first.r, first.out_features // 3
+        if any(m.r != r or m.weight.shape != first.weight.shape for m in layers):
+            raise ValueError("the layers of a pool share rank and shape")
+        if any(not torch.equal(m.weight, first.weight) or not torch.equal(m.bias, first.bias) for m in layers[1:]):
+            raise ValueError("the layers of a pool share their frozen weight and bias")
+        pool = cls(first.in_features, first.out_features, 2 * len(layers), 2 * r, bias=True, checkpoint8=checkpoint8).to(first.weight.device)
+        with torch.no_grad():
+            pool.weight.copy_(first.weight)
+            pool.bias.copy_(first.bias)
+            pool.lora_B.zero_()
+            pool.scaling.fill_(first.scaling)
+            for i, m in enumerate(layers):
+                for j, (A, B) in enumerate(((m.lora_Ax, m.lora_Bx), (m.lora_Ay, m.lora_By))):
+                    pool.lora_A[2 * i + j] = A
+                    pool.lora_B[2 * i + j, :D, :r] = B[:D]
+                    pool.lora_B[2 * i + j, 2 * D:, r:] = B[D:]
+        return pool
+
+    def forward(self, x, ids, plan=None):
+        if ops.FP32:
+            raise NotImplementedError("lora.PooledLinear runs on the bf16 MFMA: it has no fp32 mode")
+        rows = x.shape[:-1]
+        if tuple(ids.shape) != tuple(rows):
+            if ids.dim() != 1 or not rows or ids.shape[0] != rows[0]:
+                raise ValueError(f"ids {tuple(ids.shape)} for rows {tuple(rows)}: one index per row or per entry of the first dimension")
+            ids = ids.view(-1, *[1] * (len(rows) - 1)).expand(rows)
+        return _PooledLinear.apply(x, self, ids.reshape(-1), plan, self.lora_A, self.lora_B)
+
+
+@ops.keeps_precision
+class _PooledLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, lin, ids, plan, A, B):
+        x2 = x.reshape(-1, x.shape[-1])
+        xb = x2 if x2.dtype == BF else ops.cast(x2.contiguous().float(), BF)
+        pool = _cached(("pool",), (A, B, lin.scaling), lambda: ops.lora_pool(A, B, lin.scaling))
+        train = any(ctx.needs_input_grad)
+        out = ops.lora_pool_fwd(xb, w_bf16(lin.weight), lin.bias, pool, ids, out_dtype=BF if x.dtype == BF else torch.float32, want_down=train)
+        if train:
+            out, down = out
+            ctx.kept8 = tuple(xb.shape) if lin.checkpoint8 else None
+            ctx.save_for_backward(ops.ckpt8_pack(xb).buf if lin.checkpoint8 else xb, ids, down)
+            ctx.lin, ctx.pool, ctx.plan, ctx.shape, ctx.dtype = lin, pool, plan, x.shape, x.dtype
+        return out.view(*x.shape[:-1], -1)
+
+    @staticmethod
+    def backward(ctx, dout):
+        kept, ids, down = ctx.saved_tensors
+        lin = ctx.lin
+        x = kept if ctx.kept8 is None else ops.Ckpt8.of(kept, ctx.kept8)
+        d2 = dout.reshape(-1, dout.shape[-1])
+        d2 = d2 if d2.dtype == BF else ops.cast(d2.contiguous(), BF)
+        plan = ctx.plan if ctx.plan is not None else ops.lora_pool_plan(ids, lin.n_adapters)
+        want_dx = ctx.needs_input_grad[0]
+        dx, dA, dB = ops.lora_pool_bwd(d2, x, wT_bf16(lin.weight) if want_dx else None, ctx.pool, plan, down, want_dx=want_dx)
+        if want_dx:
+            dx = dx.to(ctx.dtype).view(ctx.shape)
+        return (dx, None, None, None) + deliver((lin.lora_A, lin.lora_B), (dA, dB))
 
 
 class Adapter(nn.Module):

@@ -23,18 +23,17 @@ def test_entry_points_refuse_bad_arguments_before_a_launch():
     assert L.mfnet_layernorm_fwd_ckpt8(16, 0, 48, 16, 16, 16, 16, 16, 16, 16, 4, 48, 1e-6, None) == -1 and b"multiple of 32" in E()
     assert L.mfnet_layernorm_fwd_ckpt8(16, 0, 2080, 16, 16, 16, 16, 16, 16, 16, 4, 2080, 1e-6, None) == -1
     bwd = [16, 1, 64, 16, 16, 16, 16, 16, None, None, 16, None, None, None, None, None, 0, 4, 64, None]
-    for k, v, msg in ((13, 16, b"go together"), (10, None, b"null"), (12, 16, b"beta"), (2, 62, b"lddy")):
+    for k, v, msg in ((13, 16, b"go together"), (10, None, b"null"), (0, None, b"null"), (3, None, b"null"), (12, 16, b"beta"), (2, 62, b"lddy")):
         a = list(bwd)
         a[k] = v
         assert L.mfnet_layernorm_bwd_ckpt8(*a) == -1 and msg in E(), msg
     a = list(bwd)
     a[13] = a[14] = 16
     assert L.mfnet_layernorm_bwd_ckpt8(*a) == -1 and b"workspace" in E()
-    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 64, 64, 20, 16, 16, 16, 16, 16, None) == -1 and b"sizes" in E()          # rank above its padding
-    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 60, 64, 4, 16, 16, 16, 16, 16, None) == -1
-    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 64, 64, 4, 24, 16, 16, 16, 16, None) == -1
-    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 64, 64, 4, 16, 16, 16, None, 16, None) == -1 and b"null" in E()
-    assert L.mfnet_lora_pool_pack(16, 16, 0, 2, 64, 64, 4, 16, 16, 24, 16, 16, None) == -1 and b"misaligned" in E()
+    pack = dict(A=16, B=16, dt=0, scale=None, n=2, K=64, N=64, r=4, RP=16, a_down=16, a_up=16, b_down=16, b_up=16, so=16, s=None)
+    for key, v, msg in (("r", 20, b"sizes"), ("K", 60, b"sizes"), ("N", 4, b"sizes"), ("RP", 24, b"sizes"), ("n", 0, b"sizes"), ("b_down", None, b"null"), ("so", None, b"null"), ("a_up", 24, b"misaligned"),
+                        ("A", 18, b"misaligned"), ("dt", 3, b"dtype")):
+        assert L.mfnet_lora_pool_pack(*dict(pack, **{key: v}).values()) == -1 and msg in E(), key
     assert L.mfnet_lora_pool_plan(16, 1 << 31, 2, 16, 16, 16, 16, None) == -1 and b"sizes" in E()
     assert L.mfnet_lora_pool_plan(None, 8, 2, 16, 16, 16, 16, None) == -1 and b"null" in E()
     fwd = dict(X=16, ldx=64, W=16, ldw=64, bias=None, scale=16, a_down=16, b_up=16, ids=16, n=2, RP=16, down=16, out=16, dt=1, ldo=64, M=8, N=64, K=64, s=None)

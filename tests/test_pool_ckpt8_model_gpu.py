@@ -1,0 +1,240 @@
+"""The pooled adapters and the 8-bit checkpoints inside the framework: lora.PooledLinear, LoraBlock and the train step with
+UNetFormer(checkpoints="int8"), and LayerNorm -> PooledLinear -> GELU -> PooledLinear as a program would chain them."""
+import argparse
+import functools
+import math
+import warnings
+
+import pytest
+import torch
+import torch.nn as nn
+
+from helpers import rel_err, rel_l2
+from ssrs_amd import detfill
+
+pytestmark = pytest.mark.gpu
+# Half a step of a block is at most amax / 127 (amax > 63.5 steps), relative to the block's norm at most sqrt(32) / 127: what one kept
+# activation can change a gradient that is linear in it, plus the bf16 roundings of the chain.
+KEPT = math.sqrt(32) / 127
+
+
+def _rows(g, *shape):
+    return torch.randn(*shape, generator=g)
+
+
+def test_pooled_linear_is_a_linear_with_adapters():
+    """values and gradients against the formula in 64 bits; leaves' gradients by autograd, one index per image"""
+    from ssrs_amd.medsam.models.common import loralib as lora
+    g = torch.Generator().manual_seed(0)
+    for ck in (False, True):
+        lin = lora.PooledLinear(96, 72, 3, 5, lora_alpha=2, checkpoint8=ck).cuda()
+        with torch.no_grad():
+            lin.lora_B.copy_(0.3 * _rows(g, 3, 72, 5))
+            lin.scaling.copy_(torch.tensor([0.5, 1.0, 2.0]))
+        x = _rows(g, 4, 9, 96).cuda().requires_grad_()
+        ids = torch.tensor([2, 0, -1, 2], dtype=torch.int32, device="cuda")
+        dy = _rows(g, 4, 9, 72).cuda()
+        lin(x, ids).backward(dy)
+        r = lambda t: t.detach().bfloat16().double()      # noqa: E731  (the operands of the products)
+        X, W, A, B = r(x).requires_grad_(), r(lin.weight), r(lin.lora_A).requires_grad_(), r(lin.lora_B).requires_grad_()
+        ref = X @ W.t() + lin.bias.detach().double()
+        ref = torch.stack([ref[i] + (lin.scaling[k].double() * (X[i] @ A[k].t()) @ B[k].t() if k >= 0 else 0) for i, k in enumerate(ids.tolist())])
+        ref.backward(r(dy))
+        out = lin(x, ids)
+        assert out.dtype == torch.float32 and rel_err(out.detach(), ref.detach()) < 2e-5          # fp32 sums of 96 bf16 products
+        assert rel_err(x.grad, X.grad) < 2 ** -8 and rel_err(lin.lora_B.grad, B.grad) < 2e-5
+        assert rel_l2(lin.lora_A.grad, A.grad) < (KEPT if ck else 2e-5)
+        assert (lin.lora_A.grad[1] == 0).all() and (lin.lora_B.grad[1] == 0).all()                  # no rows of adapter 1
+        assert lin.weight.grad is None and lin.bias.grad is None
+        per_row = lin(x, ids.view(4, 1).expand(4, 9))
+        assert torch.equal(per_row, out)
+        assert lin(x.detach().bfloat16(), ids).dtype == torch.bfloat16
+        with torch.no_grad():                                                                       # an optimizer step reaches the next call
+            lin.lora_B.mul_(2.0)
+            twice = lin(x, ids)
+            lin.lora_B.mul_(0.5)
+        assert not torch.equal(twice, out) and torch.equal(lin(x, ids), out)
+
+
+def test_pooled_linear_refusals():
+    from ssrs_amd import ops
+    from ssrs_amd.medsam.models.common import loralib as lora
+    for bad in (lambda: lora.PooledLinear(96, 72, 0, 4), lambda: lora.PooledLinear(96, 72, 2, 65), lambda: lora.PooledLinear(90, 72, 2, 4)):
+        with pytest.raises(ValueError):
+            bad()
+    lin = lora.PooledLinear(96, 72, 2, 4).cuda()
+    x = torch.randn(4, 9, 96, device="cuda")
+    with pytest.raises(ValueError):
+        lin(x, torch.zeros(9, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ops.MfnetError):
+        lin(x, torch.zeros(4, dtype=torch.int64, device="cuda"))
+    with ops.precision("fp32"), pytest.raises(NotImplementedError):
+        lin(x, torch.zeros(4, dtype=torch.int32, device="cuda"))
+
+
+def test_pool_of_fine_tuned_layers_serves_each_of_them():
+    """three fine-tuned qkv layers over one frozen weight in one call: every model's rows get what that model's layer gives alone"""
+    from ssrs_amd.medsam.models.common import loralib as lora
+    g = torch.Generator().manual_seed(3)
+    layers = []
+    for i in range(3):
+        m = lora.MergedLinear(128, 384, r=4, enable_lora=[True, False, True])
+        with torch.no_grad():
+            for p in (m.lora_Bx, m.lora_By):
+                p.copy_(0.2 * _rows(g, *p.shape))
+            if layers:
+                m.weight.copy_(layers[0].weight.cpu())
+                m.bias.copy_(layers[0].bias.cpu())
+        layers.append(m.cuda())
+    pool = lora.PooledLinear.from_merged(layers)
+    x, y = _rows(g, 3, 48, 128).cuda(), _rows(g, 3, 48, 128).cuda()
+    ids = torch.arange(6, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        both = pool(torch.stack([x, y], 1).reshape(6, 48, 128), ids).view(3, 2, 48, 384)
+        for i, m in enumerate(layers):
+            ox, oy = m(x[i], y[i])
+            # the layer splits its fp32 factors in two bf16 parts, the pool rounds them once: 2^-8 of the update's terms
+            for got, want, xi, A, B in ((both[i, 0], ox, x[i], m.lora_Ax, m.lora_Bx), (both[i, 1], oy, y[i], m.lora_Ay, m.lora_By)):
+                a = m.scaling * xi.double().abs() @ A.double().abs().t()
+                terms = torch.cat([a[:, :4] @ B[:128].double().abs().t(), torch.zeros(48, 128, device="cuda", dtype=torch.float64), a[:, 4:] @ B[128:].double().abs().t()], 1)
+                assert ((got.double() - want.double()).abs() <= 2.5 * 2 ** -8 * terms + 1e-5).all()
+    with pytest.raises(ValueError):
+        lora.PooledLinear.from_merged([layers[0], lora.MergedLinear(128, 384, r=4, enable_lora=[True, False, True]).cuda()])
+
+
+def test_chain_of_kept_layers():
+    """LayerNorm -> PooledLinear -> GELU -> PooledLinear with everything kept in 8 bits, eager and captured, against 64 bits"""
+    from ssrs_amd import ops
+    g = torch.Generator().manual_seed(5)
+    M, D, H, n, r = 700, 128, 512, 4, 8
+    x = (_rows(g, M, D) * torch.exp(0.5 * _rows(g, D))).cuda()
+    gamma, beta = (1 + 0.2 * _rows(g, D)).cuda(), (0.1 * _rows(g, D)).cuda()
+    W1, W2 = (_rows(g, H, D) / math.sqrt(D)).bfloat16().cuda(), (_rows(g, D, H) / math.sqrt(H)).bfloat16().cuda()
+    A1, B1 = (_rows(g, n, r, D) / math.sqrt(D)).bfloat16().cuda(), (0.3 * _rows(g, n, H, r)).bfloat16().cuda()
+    A2, B2 = (_rows(g, n, r, H) / math.sqrt(H)).bfloat16().cuda(), (0.3 * _rows(g, n, D, r)).bfloat16().cuda()
+    ids = torch.randint(-1, n, (M,), generator=g, dtype=torch.int32).cuda()
+    dy = (0.1 * _rows(g, M, D)).bfloat16().cuda()
+    W1t, W2t = W1.t().contiguous(), W2.t().contiguous()
+
+    def step():
+        plan = ops.lora_pool_plan(ids, n)
+        p1, p2 = ops.lora_pool(A1, B1), ops.lora_pool(A2, B2)
+        y, mean, rstd, ck = ops.layernorm_fwd_ckpt8(x, gamma, beta, 1e-6)
+        pre, d1 = ops.lora_pool_fwd(y, W1, None, p1, ids, want_down=True)
+        act, ca = ops.gelu_fwd_ckpt8(pre)
+        out, d2 = ops.lora_pool_fwd(act, W2, None, p2, ids, out_dtype=torch.float32, want_down=True)
+        # backward: the second layer's input is made again for its dA
+        _, act8 = ops.gelu_bwd_ckpt8(ca, torch.zeros_like(act), want_act=True)
+        dact, dA2, dB2 = ops.lora_pool_bwd(dy, act8, W2t, p2, plan, d2)
+        dpre = ops.gelu_bwd_ckpt8(ca, dact)
+        ln8 = ops.layernorm_y_ckpt8(ck, mean, rstd, gamma, beta)
+        dln, dA1, dB1 = ops.lora_pool_bwd(dpre, ln8, W1t, p1, plan, d1)
+        dx, y8, dgamma, dbeta = ops.layernorm_bwd_ckpt8(dln, ck, mean, rstd, gamma, beta, want_y=True, want_weights=True)
+        assert y8.data_ptr() != ln8.data_ptr()
+        return out, dx, dA1, dB1, dA2, dB2, dgamma, dbeta, y8, ln8
+    got = step()
+    assert torch.equal(got[8], got[9])
+    d = lambda t: t.double().requires_grad_()      # noqa: E731
+    X, G, Bt, a1, b1, a2, b2 = (d(t) for t in (x, gamma, beta, A1, B1, A2, B2))
+
+    def layer(z, W, A, B):
+        o = z @ W.double().t()
+        mask = [(ids == i).double()[:, None] for i in range(n)]
+        return o + sum(m * ((z @ A[i].t()) @ B[i].t()) for i, m in enumerate(mask))
+    h = torch.nn.functional.layer_norm(X, (D,), G, Bt, 1e-6)
+    out = layer(torch.nn.functional.gelu(layer(h, W1, a1, b1)), W2, a2, b2)
+    out.backward(dy.double())
+    assert rel_l2(got[0], out.detach()) < 4 * 2 ** -8                       # three bf16 tensors on the way
+    for t, leaf, name in ((got[1], X, "x"), (got[2], a1, "A1"), (got[3], b1, "B1"), (got[4], a2, "A2"), (got[5], b2, "B2"), (got[6], G, "gamma"), (got[7], Bt, "beta")):
+        # at most the GELU's and the LayerNorm's (or the layer's own) kept input enter a gradient, and six bf16 roundings
+        assert rel_l2(t, leaf.grad) < 2 * KEPT + 6 * 2 ** -8, name
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+        cap = step()
+    for k in range(3):
+        x.copy_(_rows(g, M, D))
+        ids.copy_(torch.randint(-1, n, (M,), generator=g, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(step(), cap)), k
+
+
+def _args(mid_dim=None):
+    return argparse.Namespace(mod="sam_lora", mid_dim=mid_dim, image_size=1024, multimask_output=1)
+
+
+@pytest.mark.parametrize("mid_dim,ws", [(None, 14), (2, 0), (6, 14), (8, 0)])
+def test_block_with_8bit_checkpoints(mid_dim, ws):
+    """the block's outputs agree with bf16 checkpoints' to a bf16 rounding or two; gradients within what the kept activations may change;
+    less than half of the bytes are kept"""
+    from ssrs_amd.vit import LoraBlock
+    blk = LoraBlock(args=_args(mid_dim), dim=128, num_heads=2, mlp_ratio=4.0, norm_layer=functools.partial(nn.LayerNorm, eps=1e-6), use_rel_pos=True,
+                    window_size=ws, input_size=(64, 64))
+    blk.load_state_dict(detfill.fill_state_dict(blk.state_dict(), "k8/"))
+    blk = blk.cuda()
+    for name, p in blk.named_parameters():
+        p.requires_grad = "lora_" in name
+    g = torch.Generator().manual_seed(1)
+    h0 = _rows(g, 2, 2, 16, 16, 128).cuda()
+    dh = _rows(g, 2, 2, 16, 16, 128).cuda()
+    res, kept = {}, {}
+    for mode in (False, True):
+        blk.checkpoint8 = mode
+        blk.zero_grad()
+        h = h0.clone().requires_grad_()
+        seen = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: (seen.append(t), t)[1], lambda t: t):
+            out = blk.forward_stacked(h)
+        kept[mode] = sum({t.data_ptr(): t.numel() * t.element_size() for t in seen if t is not None}.values())
+        out.backward(dh)
+        res[mode] = (out.detach(), {"h": h.grad, **{k: p.grad for k, p in blk.named_parameters() if p.grad is not None}})
+        with torch.no_grad():
+            assert torch.equal(blk.forward_stacked(h0), res[False][0]) or mode       # nothing is kept without a backward: the usual forward
+    assert kept[True] < 0.55 * kept[False], kept
+    assert rel_err(res[True][0], res[False][0]) < 2 ** -7
+    assert set(res[True][1]) == set(res[False][1]) and len(res[True][1]) == 1 + 16
+    for k, want in res[False][1].items():
+        # the attention's gradients pass one kept LayerNorm input, the MLP's that and the GELU's
+        assert rel_l2(res[True][1][k], want) < 2 * KEPT + 4 * 2 ** -8, k
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_train_step_with_8bit_checkpoints(use_graph):
+    """the whole step of the tiny model: loss of the first step as with bf16 checkpoints, gradients within the kept activations' share
+    (two blocks, two branches each), the loss falls over the updates of one batch as it does with bf16 checkpoints"""
+    from ssrs_amd.trainer import TrainEngine
+    from ssrs_amd.unetformer_mmsam import UNetFormer
+    rgb, dsm, tgt = (t.cuda() for t in detfill.tiles("k8t", 2, 256, 6))
+    grads, losses = {}, {}
+    for kind in ("bf16", "int8"):
+        with warnings.catch_warnings():
+            warnings.simplefilter("ignore")
+            m = UNetFormer(num_classes=6, encoder="vit_tiny_test", args=_args(), checkpoints=kind)
+        m.load_state_dict(detfill.fill_state_dict(m.state_dict(), "k8t/"))
+        m = m.cuda().eval()
+        m.decoder.segmentation_head[1].p = 0.0
+        assert m.checkpoints == kind and all(b.checkpoint8 == (kind == "int8") for b in m.image_encoder.blocks)
+        eng = TrainEngine(m, lr=0.01, momentum=0.9, weight_decay=5e-4, class_weight=torch.ones(6, device="cuda"), use_graph=use_graph)
+        ls = []
+        for i in range(4):                   # (graph mode: two eager steps, then capture and replays)
+            ls.append(TrainEngine.read_metrics(eng.step(rgb, dsm, tgt))["loss"])
+            if i == 0:
+                grads[kind] = eng.flat_g.clone()
+        losses[kind] = ls
+    assert abs(losses["int8"][0] - losses["bf16"][0]) < 5e-3 * abs(losses["bf16"][0])
+    assert rel_l2(grads["int8"], grads["bf16"]) < 4 * KEPT
+    assert losses["int8"][3] < losses["int8"][0] and losses["bf16"][3] < losses["bf16"][0]
+
+
+def test_checkpoints_option_refusals():
+    from ssrs_amd.unetformer_mmsam import UNetFormer
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        with pytest.raises(ValueError):
+            UNetFormer(num_classes=6, encoder="vit_tiny_test", args=_args(), checkpoints="int4")
+        with pytest.raises(ValueError):
+            UNetFormer(num_classes=6, encoder="vit_tiny_test", args=_args(), checkpoints="int8", precision="fp32")
+        with pytest.raises(NotImplementedError):
+            a = _args()
+            a.mod = "sam_adpt"
+            UNetFormer(num_classes=6, encoder="vit_tiny_test", args=a, checkpoints="int8")
