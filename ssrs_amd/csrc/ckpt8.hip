@@ -198,6 +198,21 @@ template <> __device__ __forceinline__ float4 load4<bf16_t>(const bf16_t* p) {
   return make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
 }
 
+// four elements as they lie in memory
+template <typename T> struct Raw4;
+template <> struct Raw4<float> {
+  float4 v;
+  __device__ __forceinline__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void zero() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ float4 value() const { return v; }
+};
+template <> struct Raw4<bf16_t> {
+  u32x2_t v;
+  __device__ __forceinline__ void load(const bf16_t* p) { v = *reinterpret_cast<const u32x2_t*>(p); }
+  __device__ __forceinline__ void zero() { v = (u32x2_t){0u, 0u}; }
+  __device__ __forceinline__ float4 value() const { return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y)); }
+};
+
 template <typename T, int NV>
 __global__ __launch_bounds__(256) void ln_fwd_ckpt8_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
                                                            const float* __restrict__ beta, bf16_t* __restrict__ y, float* __restrict__ mean_out,
@@ -271,25 +286,42 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void ln_bwd_ckpt8_kernel(const T* _
     dg[j] = db[j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float invC = 1.0f / (float)C;
-  for (int64_t row = (int64_t)blockIdx.x * LNB_WAVES + wave; row < rows; row += (int64_t)gridDim.x * LNB_WAVES) {
-    float4 d[NV], xh[NV], r[NV];
-    unsigned int w[NV], by[NV];
-    const float mean = mean_in[row], rstd = rstd_in[row];
+  const int64_t stride = (int64_t)gridDim.x * LNB_WAVES;
+  // Operands of a row as they lie in memory. Up to NV = 5 the next row's are requested before this row's arithmetic (registers end it
+  // there): with one row in flight per wave the loop reached 4.1 TB/s.
+  struct Raw { Raw4<T> d[NV]; unsigned int w[NV], by[NV]; float4 r[NV]; float mean, rstd; };
+  auto request = [&](int64_t row, Raw& q) __attribute__((always_inline)) {
+    q.mean = mean_in[row];
+    q.rstd = rstd_in[row];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = 4 * (lane + 64 * j);
       const bool on = c < C;
-      d[j] = on && dy ? load4(dy + row * lddy + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-      w[j] = on ? *reinterpret_cast<const unsigned int*>(codes + row * C + c) : 0u;
-      by[j] = on ? exps[row * (C >> 5) + (c >> 5)] : 0u;
-      if (dres) r[j] = on ? *reinterpret_cast<const float4*>(dres + row * C + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      if (on && dy) q.d[j].load(dy + row * lddy + c); else q.d[j].zero();
+      q.w[j] = on ? *reinterpret_cast<const unsigned int*>(codes + row * C + c) : 0u;
+      q.by[j] = on ? exps[row * (C >> 5) + (c >> 5)] : 0u;
+      q.r[j] = on && dres ? *reinterpret_cast<const float4*>(dres + row * C + c) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
+  };
+  constexpr bool AHEAD = NV <= 5;
+  Raw cur, nxt;
+  int64_t row = (int64_t)blockIdx.x * LNB_WAVES + wave;
+  if (AHEAD && row < rows) request(row, nxt);
+  for (; row < rows; row += stride) {
+    if (AHEAD) {
+      cur = nxt;
+      if (row + stride < rows) request(row + stride, nxt);
+    } else request(row, cur);
+    float4 d[NV], xh[NV];
+    const float mean = cur.mean, rstd = cur.rstd;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) d[j] = cur.d[j].value();
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const float step = ckpt8_step(by[j]);
-      xh[j].x = (ckpt8_value(w[j], 0, step) - mean) * rstd; xh[j].y = (ckpt8_value(w[j], 1, step) - mean) * rstd;
-      xh[j].z = (ckpt8_value(w[j], 2, step) - mean) * rstd; xh[j].w = (ckpt8_value(w[j], 3, step) - mean) * rstd;
+      const float step = ckpt8_step(cur.by[j]);
+      xh[j].x = (ckpt8_value(cur.w[j], 0, step) - mean) * rstd; xh[j].y = (ckpt8_value(cur.w[j], 1, step) - mean) * rstd;
+      xh[j].z = (ckpt8_value(cur.w[j], 2, step) - mean) * rstd; xh[j].w = (ckpt8_value(cur.w[j], 3, step) - mean) * rstd;
       const float tx = d[j].x * ga[j].x, ty = d[j].y * ga[j].y, tz = d[j].z * ga[j].z, tw = d[j].w * ga[j].w;
       s1 += (tx + ty) + (tz + tw);
       if (4 * (lane + 64 * j) < C) s2 += fmaf(tx, xh[j].x, ty * xh[j].y) + fmaf(tz, xh[j].z, tw * xh[j].w);
@@ -307,7 +339,7 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void ln_bwd_ckpt8_kernel(const T* _
       float4 o;
       o.x = rstd * (fmaf(d[j].x, ga[j].x, -m1) - xh[j].x * m2); o.y = rstd * (fmaf(d[j].y, ga[j].y, -m1) - xh[j].y * m2);
       o.z = rstd * (fmaf(d[j].z, ga[j].z, -m1) - xh[j].z * m2); o.w = rstd * (fmaf(d[j].w, ga[j].w, -m1) - xh[j].w * m2);
-      if (dres) { o.x += r[j].x; o.y += r[j].y; o.z += r[j].z; o.w += r[j].w; }
+      if (dres) { o.x += cur.r[j].x; o.y += cur.r[j].y; o.z += cur.r[j].z; o.w += cur.r[j].w; }
       if (dx) *reinterpret_cast<float4*>(dx + row * C + c) = o;
       if (dx_bf) {
         u32x2_t p; p.x = pack_bf16x2(o.x, o.y); p.y = pack_bf16x2(o.z, o.w);

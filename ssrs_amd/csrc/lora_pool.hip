@@ -260,8 +260,9 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
   }
 }
 
-// Few rows, an adapter each as it may be: one row per workgroup, the four waves take every fourth k-step, a lane one rank and 8 columns of
-// it. All requests are independent of each other, where the kernel above takes the adapters of its rows one after the other.
+// Few rows, an adapter each as it may be: one row per workgroup, the four waves take every fourth k-step. The MFMA's 16 columns all hold
+// the one row: a sixteenth of the products, but one instruction where 8 multiply-adds and their conversions would stand. All requests are
+// independent of each other, where the kernel above takes the adapters of its rows one after the other.
 template <int NR>
 __global__ __launch_bounds__(256) void pool_down_row_kernel(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
                                                             const int* __restrict__ ids, int n, float* __restrict__ out, int K) {
@@ -270,36 +271,34 @@ __global__ __launch_bounds__(256) void pool_down_row_kernel(const bf16_t* __rest
   const int fr = lane & 15, fq = lane >> 4;
   const int64_t m = blockIdx.x;
   const int id = ids[m];
-  float s[NR];
+  f32x4_t s[NR];
 #pragma unroll
-  for (int f = 0; f < NR; ++f) s[f] = 0.f;
+  for (int f = 0; f < NR; ++f) s[f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   const bool on = (unsigned)id < (unsigned)n;
   if (on) {
     const bf16_t* fp = F + id * pool_image(K, 16 * NR) + 8 * lane;
     const bf16_t* x = X + m * ldx + 8 * fq;
     for (int k0 = wave; 32 * k0 < K; k0 += 16) {             // four k-steps in flight
-      u32x4_t xv[4], a[4][NR];
+      Frag xv[4], a[4][NR];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int ks = k0 + 4 * j;
         const bool in = 32 * ks + 8 * fq < K;
-        xv[j] = in ? *reinterpret_cast<const u32x4_t*>(x + 32 * ks) : (u32x4_t){0u, 0u, 0u, 0u};
+        xv[j].q = in ? *reinterpret_cast<const u32x4_t*>(x + 32 * ks) : (u32x4_t){0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int f = 0; f < NR; ++f) a[j][f] = in ? *reinterpret_cast<const u32x4_t*>(fp + ((int64_t)ks * NR + f) * 512) : (u32x4_t){0u, 0u, 0u, 0u};
+        for (int f = 0; f < NR; ++f) a[j][f].q = in ? *reinterpret_cast<const u32x4_t*>(fp + ((int64_t)ks * NR + f) * 512) : (u32x4_t){0u, 0u, 0u, 0u};
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int f = 0; f < NR; ++f)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) s[f] = fmaf(bf16_lo(xv[j][q]), bf16_lo(a[j][f][q]), fmaf(bf16_hi(xv[j][q]), bf16_hi(a[j][f][q]), s[f]));
+        for (int f = 0; f < NR; ++f) s[f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][f].v, xv[j].v, s[f], 0, 0, 0);
     }
   }
+  if (fr == 0) {
 #pragma unroll
-  for (int f = 0; f < NR; ++f) {
-    s[f] += __shfl_xor(s[f], 16, 64);
-    s[f] += __shfl_xor(s[f], 32, 64);
-    if (fq == 0) red[wave][16 * f + fr] = s[f];
+    for (int f = 0; f < NR; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) red[wave][16 * f + 4 * fq + r] = s[f][r];
   }
   __syncthreads();
   const int t = threadIdx.x;
@@ -517,6 +516,132 @@ __global__ __launch_bounds__(256) void pool_gemm_rows_kernel(const PoolGemm p) {
     u32x2_t o;
     o.x = pack_bf16x2(t[0] + add[0], t[1] + add[1]);
     o.y = pack_bf16x2(t[2] + add[2], t[3] + add[3]);
+    *reinterpret_cast<u32x2_t*>((bf16_t*)p.out + at) = o;
+  }
+}
+
+// At most 16 rows: both products in one launch. 16 waves per workgroup and 32 columns: wave w computes down of row w (every workgroup
+// again: M 16 NR K products beside the 32 M K of its own, the factors come from L2) while the weight is on its way, then the waves
+// split K for the 32 columns, add up through LDS and add the update. The second launch that this saves costs more than it.
+template <int NR>
+__global__ __launch_bounds__(1024) void pool_rows_fused_kernel(const PoolGemm p, const bf16_t* __restrict__ F, const float* __restrict__ scale, float* __restrict__ down) {
+  constexpr int RP = 16 * NR;
+  __shared__ f32x4_t red[16][2][64];
+  __shared__ float dn[16][RP + 4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int fr = lane & 15, fq = lane >> 4;
+  const int n0 = blockIdx.x * 32, K = p.K, M = (int)p.M;
+  const u32x4_t zero = (u32x4_t){0u, 0u, 0u, 0u};
+  // this wave's 64-wide pieces of K: the first one is requested before the down product
+  const bf16_t* x = p.X + (int64_t)(fr < M ? fr : M - 1) * p.ldx + 8 * fq;
+  const bf16_t* w[2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a) w[a] = p.W + (int64_t)(n0 + 16 * a + fr < p.N ? n0 + 16 * a + fr : p.N - 1) * p.ldw + 8 * fq;
+  const int my = wave < M ? p.ids[wave] : -1;                // the adapter of the row whose down product this wave makes
+  const int cb = n0 + 16 * wave + 4 * fq;                    // waves 0 and 1 finish 16 columns each: row fr, columns cb .. cb + 3
+  const bool fin = wave < 2 && fr < M && cb < p.N;
+  const int fid = fin ? p.ids[fr] : -1;
+  const bool flr = (unsigned)fid < (unsigned)p.n;
+  Frag wf[2][2], xf[2];
+  auto load = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int k = k0 + 32 * j;
+      const bool on = k + 8 * fq < K;                        // chunks behind column K: zeros on both sides
+      xf[j].q = on ? *reinterpret_cast<const u32x4_t*>(x + k) : zero;
+#pragma unroll
+      for (int a = 0; a < 2; ++a) wf[j][a].q = on ? *reinterpret_cast<const u32x4_t*>(w[a] + k) : zero;
+    }
+  };
+  if (64 * wave < K) load(64 * wave);
+  if (wave < M) {
+    const int id = my;
+    const bool on = (unsigned)id < (unsigned)p.n;
+    f32x4_t s[4][NR];                                        // four sums over every fourth k-step: the order of pool_down_row_kernel, the same bits
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int f = 0; f < NR; ++f) s[q][f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    if (on) {
+      const bf16_t* fp = F + id * pool_image(K, RP) + 8 * lane;
+      const bf16_t* xr = p.X + (int64_t)wave * p.ldx + 8 * fq;
+      constexpr int IN = NR == 1 ? 8 : 4;                    // k-steps in flight
+      for (int ks0 = 0; 32 * ks0 < K; ks0 += IN) {
+        Frag xv[IN], a[IN][NR];
+#pragma unroll
+        for (int j = 0; j < IN; ++j) {
+          const int ks = ks0 + j;
+          const bool in = 32 * ks + 8 * fq < K;
+          xv[j].q = in ? *reinterpret_cast<const u32x4_t*>(xr + 32 * ks) : zero;
+#pragma unroll
+          for (int f = 0; f < NR; ++f) a[j][f].q = in ? *reinterpret_cast<const u32x4_t*>(fp + ((int64_t)ks * NR + f) * 512) : zero;
+        }
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+          for (int f = 0; f < NR; ++f) s[j & 3][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][f].v, xv[j].v, s[j & 3][f], 0, 0, 0);
+      }
+    }
+    const float sc = on ? scale[id] : 0.f;
+    if (fr == 0) {
+#pragma unroll
+      for (int f = 0; f < NR; ++f)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = 16 * f + 4 * fq + r;
+          const float v = on ? sc * ((s[0][f][r] + s[1][f][r]) + (s[2][f][r] + s[3][f][r])) : 0.f;
+          dn[wave][j] = v;
+          if (blockIdx.x == 0) down[wave * RP + j] = v;
+        }
+    }
+  }
+  // what the finishing waves need beside the sums (RP = 16: in registers before the barrier)
+  const bf16_t* up = p.Up + ((int64_t)(flr ? fid : 0) * p.N + (fin ? cb : 0)) * RP;
+  u32x4_t uv[NR == 1 ? 8 : 1];
+  if (NR == 1 && flr) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) uv[2 * c + j] = *reinterpret_cast<const u32x4_t*>(up + c * RP + 8 * j);
+  }
+  float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (fin && p.bias) bias = *reinterpret_cast<const float4*>(p.bias + cb);
+  f32x4_t acc[2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a) acc[a] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 64 * wave; k0 < K; k0 += 1024) {
+    if (k0 != 64 * wave) load(k0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int a = 0; a < 2; ++a) acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[j][a].v, xf[j].v, acc[a], 0, 0, 0);
+  }
+#pragma unroll
+  for (int a = 0; a < 2; ++a) red[wave][a][lane] = acc[a];
+  __syncthreads();
+  if (!fin) return;
+  f32x4_t t = red[0][wave][lane];
+#pragma unroll
+  for (int q = 1; q < 16; ++q) t += red[q][wave][lane];
+  t[0] += bias.x; t[1] += bias.y; t[2] += bias.z; t[3] += bias.w;
+  if (flr) {
+    f32x4_t lr = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int j = 0; j < RP; j += 8)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const u32x4_t u = NR == 1 ? uv[(2 * c + j / 8) % (NR == 1 ? 8 : 1)] : *reinterpret_cast<const u32x4_t*>(up + (int64_t)c * RP + j);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) lr[c] = fmaf(dn[fr][j + 2 * q], bf16_lo(u[q]), fmaf(dn[fr][j + 2 * q + 1], bf16_hi(u[q]), lr[c]));
+      }
+    t += lr;
+  }
+  const int64_t at = (int64_t)fr * p.ldo + cb;
+  if (p.out_f32) *reinterpret_cast<float4*>((float*)p.out + at) = make_float4(t[0], t[1], t[2], t[3]);
+  else {
+    u32x2_t o;
+    o.x = pack_bf16x2(t[0], t[1]);
+    o.y = pack_bf16x2(t[2], t[3]);
     *reinterpret_cast<u32x2_t*>((bf16_t*)p.out + at) = o;
   }
 }
@@ -822,6 +947,8 @@ __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_ke
 struct PoolTn {
   const bf16_t* Y; int64_t ldy; const signed char* codes; const unsigned char* exps;
   const float* U; int RP; const int* perm; const int4* table; float* part; int C;
+  float* out; int r;                                       // != NULL (no adapter has more than one chunk): the result itself, without the padded ranks
+  const int* base;
 };
 #define TN_MAX_CH 512
 template <int NR, bool CKPT, bool RANK_MAJOR>
@@ -912,7 +1039,8 @@ __device__ __forceinline__ void pool_tn_body(unsigned char (*lds)[4][32 * 128], 
     }
   }
   // sum of the four waves, one slab of 64 columns after the other (16 KB per wave and fragment column); wave w writes tile t = w
-  float* out = p.part + (int64_t)blockIdx.y * p.RP * C;
+  float* out = p.out ? p.out + (int64_t)blockIdx.y * p.r * C : p.part + (int64_t)blockIdx.y * p.RP * C;
+  const int ld = p.out ? p.r : p.RP, jmax = p.out ? p.r : p.RP;
 #pragma unroll
   for (int f = 0; f < NR; ++f) {
     __syncthreads();
@@ -934,7 +1062,7 @@ __device__ __forceinline__ void pool_tn_body(unsigned char (*lds)[4][32 * 128], 
         for (int w = 0; w < 4; ++w) v += reinterpret_cast<const float*>(lds[w][0])[idx];
         const int a = 4 * fq + r;
         const int c = cw + 64 * wave + 16 * t + (RANK_MAJOR ? fr : a), j = j0 + 16 * f + (RANK_MAJOR ? a : fr);
-        if (c < C) out[RANK_MAJOR ? (int64_t)j * C + c : (int64_t)c * p.RP + j] = v;
+        if (c < C && j < jmax) out[RANK_MAJOR ? (int64_t)j * C + c : (int64_t)c * ld + j] = v;
       }
   }
 }
@@ -944,7 +1072,11 @@ template <int NR, bool CKPT>
 __global__ __launch_bounds__(256, 2) void pool_tn_kernel(const PoolTn a, const PoolTn b, int strips_a) {
   __shared__ __attribute__((aligned(16))) unsigned char lds[4][4][32 * 128];
   __shared__ int rows[TN_MAX_CH];
-  const int4 ck = a.table[blockIdx.y];
+  int4 ck;
+  if (a.out) {                                             // blockIdx.y is an adapter: its only chunk, or no rows (sums of nothing)
+    const int k = a.base[blockIdx.y];
+    ck = k < a.base[blockIdx.y + 1] ? a.table[k] : make_int4((int)blockIdx.y, 0, 0, 0);
+  } else ck = a.table[blockIdx.y];
   if (ck.x < 0) return;
   if ((int)blockIdx.x < strips_a) pool_tn_body<NR, CKPT, true>(lds, rows, a, ck, blockIdx.x);
   else pool_tn_body<NR, false, false>(lds, rows, b, ck, blockIdx.x - strips_a);
@@ -1030,8 +1162,7 @@ static int pool_gemm(PoolGemm& p, hipStream_t stream) {
   const double iters = (p.K + 63) / 64;
   auto tiles = [&](int bm, int bn) { p.tiles_m = (int)ceil_div64(M, bm); p.tiles_n = (int)ceil_div64(N, bn); return (int64_t)p.tiles_m * p.tiles_n; };
 #define PR(XF_) hipLaunchKernelGGL((pool_gemm_rows_kernel<XF_>), dim3((unsigned)ceil_div64(N, 16)), dim3(256), 0, stream, p)
-  if (M <= 16) PR(1);
-  else if (M <= 32) PR(2);
+  if (M <= 32) PR(2);
   else if (M <= 64) PR(4);
 #undef PR
   else {
@@ -1052,6 +1183,20 @@ static int pool_gemm(PoolGemm& p, hipStream_t stream) {
   return MFNET_OK;
 }
 
+// down = scale_i image_i x, out = x W^T (+ bias) + up_i down
+static int pool_products(PoolGemm& p, const void* image, const float* scale, float* down, hipStream_t stream) {
+  if (p.M > 16 || p.RP > 32) {                              // (64 ranks: more registers than 16 waves have)
+    const int rc = pool_down(p.X, p.ldx, image, scale, p.ids, p.n, p.RP, down, p.M, p.K, stream);
+    return rc ? rc : pool_gemm(p, stream);
+  }
+  const dim3 grid((unsigned)ceil_div64(p.N, 32));
+#define PF(NR_) hipLaunchKernelGGL((pool_rows_fused_kernel<NR_>), grid, dim3(1024), 0, stream, p, (const bf16_t*)image, scale, down)
+  if (p.RP == 16) PF(1); else PF(2);
+#undef PF
+  MF_LAUNCH_CHECK("lora_pool (few rows)");
+  return MFNET_OK;
+}
+
 extern "C" int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* scale, const void* a_down,
                                    const void* b_up, const int* ids, int64_t n, int RP, float* down, void* out, int out_dtype, int64_t ldo, int64_t M,
                                    int64_t N, int64_t K, hipStream_t stream) {
@@ -1063,14 +1208,12 @@ extern "C" int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, in
   POOL_CHECK_ROWS("lora_pool_fwd (weight)", W, ldw, K);
   POOL_CHECK_ROWS("lora_pool_fwd (out)", out, ldo, N);
   MF_CHECK_ARG(((uintptr_t)bias | (uintptr_t)down | (uintptr_t)a_down | (uintptr_t)b_up) % 16 == 0, "lora_pool_fwd: misaligned tensor");
-  const int rc = pool_down(X, ldx, a_down, scale, ids, n, RP, down, M, K, stream);
-  if (rc) return rc;
   PoolGemm p;
   p.X = (const bf16_t*)X; p.ldx = ldx; p.W = (const bf16_t*)W; p.ldw = ldw; p.bias = bias;
   p.D = down; p.Up = (const bf16_t*)b_up; p.ids = ids; p.n = (int)n; p.RP = RP;
   p.out = out; p.ldo = ldo; p.out_f32 = out_dtype == MFNET_F32;
   p.M = M; p.N = (int)N; p.K = (int)K;
-  return pool_gemm(p, stream);
+  return pool_products(p, a_down, scale, down, stream);
 }
 
 // floats of workspace of mfnet_lora_pool_bwd: p [M, RP] and the partial sums of dA and dB
@@ -1098,29 +1241,35 @@ extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, 
     MF_CHECK_ARG((uintptr_t)codes % 8 == 0 && ((uintptr_t)table | (uintptr_t)down | (uintptr_t)ws | (uintptr_t)b_down | (uintptr_t)a_up) % 16 == 0, "lora_pool_bwd: misaligned tensor");
     MF_CHECK_ARG(ws_floats >= mfnet_lora_pool_bwd_workspace_floats(M, n, K, N, RP), "lora_pool_bwd: workspace too small");
     MF_CHECK_ARG(chunks <= 65535, "lora_pool_bwd: too many chunks of rows (%lld)", (long long)chunks);
-    int rc = pool_down(dy, lddy, b_down, scale, ids, n, RP, ws, M, N, stream);
-    if (rc) return rc;
-    if (dx) {
+    int rc;
+    if (!dx) rc = pool_down(dy, lddy, b_down, scale, ids, n, RP, ws, M, N, stream);
+    else {
       PoolGemm p;
       p.X = (const bf16_t*)dy; p.ldx = lddy; p.W = (const bf16_t*)Wt; p.ldw = ldwt; p.bias = nullptr;
       p.D = ws; p.Up = (const bf16_t*)a_up; p.ids = ids; p.n = (int)n; p.RP = RP;
       p.out = dx; p.ldo = lddx; p.out_f32 = 0;
       p.M = M; p.N = (int)K; p.K = (int)N;
-      rc = pool_gemm(p, stream);
-      if (rc) return rc;
+      rc = pool_products(p, b_down, scale, ws, stream);
     }
+    if (rc) return rc;
     PoolTn a, b;
     a.Y = (const bf16_t*)X; a.ldy = ldx; a.codes = (const signed char*)codes; a.exps = (const unsigned char*)exps;
     a.U = ws; a.RP = RP; a.perm = perm; a.table = (const int4*)table; a.part = part_a; a.C = (int)K;
     b = a;
     b.Y = (const bf16_t*)dy; b.ldy = lddy; b.U = down; b.part = part_b; b.C = (int)N;
+    const bool one_chunk = M <= pool_chunk_rows(M);
+    a.base = b.base = base;
+    a.r = b.r = r;
+    a.out = one_chunk ? dA : nullptr;
+    b.out = one_chunk ? dB : nullptr;
     const int strips_a = (int)ceil_div64(K, 256), strips_b = (int)ceil_div64(N, 256);
-    const dim3 grid((unsigned)(strips_a + strips_b), (unsigned)chunks, RP == 64 ? 2 : 1);
+    const dim3 grid((unsigned)(strips_a + strips_b), (unsigned)(one_chunk ? n : chunks), RP == 64 ? 2 : 1);
 #define PT(NR_, CK_) hipLaunchKernelGGL((pool_tn_kernel<NR_, CK_>), grid, dim3(256), 0, stream, a, b, strips_a)
     if (RP == 16) { if (codes) PT(1, true); else PT(1, false); }
     else { if (codes) PT(2, true); else PT(2, false); }
 #undef PT
     MF_LAUNCH_CHECK("lora_pool_bwd (sums over rows)");
+    if (one_chunk) return MFNET_OK;
   }
   PoolSum sa, sb;
   sa.part = part_a; sa.out = dA; sa.per = K * RP; sa.ld = (int)K; sa.d0 = r; sa.d1 = (int)K;

@@ -1624,9 +1624,14 @@ def _launch(name, dev, nbytes, flops, *args):
     if torch.cuda.current_device() != dev:
         with torch.cuda.device(dev):
             return tcall(name, nbytes, flops, *args, _raw_stream(dev))
-    if KERNEL_TRACE is None:
-        return call(name, *args, _raw_stream(dev))
-    return tcall(name, nbytes, flops, *args, _raw_stream(dev))
+    return (call(name, *args, _raw_stream(dev)) if KERNEL_TRACE is None else tcall(name, nbytes, flops, *args, _raw_stream(dev)))
+
+
+def _like(t, shape, dtype):
+    """a dense tensor of this shape on t's device"""
+    if t.shape == shape and t.is_contiguous():
+        return torch.empty_like(t, dtype=dtype)
+    return t.new_empty(shape, dtype=dtype)
 
 
 def _rows_any(name, t):
@@ -1649,8 +1654,9 @@ class Ckpt8:
     ckpt8_unpack and the backward kernels."""
     __slots__ = ("buf", "shape", "rows", "C", "at_exps")
 
-    def __init__(self, shape, device):
-        self.buf = torch.empty(self._place(shape), dtype=torch.uint8, device=device)
+    def __init__(self, t):
+        """room for the checkpoint of tensor t"""
+        self.buf = t.new_empty((self._place(t.shape),), dtype=torch.uint8)
 
     def _place(self, shape):
         self.shape = tuple(shape)
@@ -1703,7 +1709,7 @@ def ckpt8_pack(x) -> Ckpt8:
     dev = _device_of("ckpt8_pack", x)
     dt = _ck_dtype("ckpt8_pack", x)
     x2, rows, C, ldx = _rows_any("ckpt8_pack", x)
-    c = Ckpt8(x.shape, x.device)
+    c = Ckpt8(x)
     codes, exps = c._ptrs()
     _launch("mfnet_ckpt8_pack", dev, rows * C * (2 if dt else 4) + c.nbytes, 0, x2.data_ptr(), dt, ldx, codes, exps, rows, C)
     return c
@@ -1714,7 +1720,7 @@ def ckpt8_unpack(c: Ckpt8, dtype=torch.bfloat16):
     dev = _device_of("ckpt8_unpack", c.buf)
     if dtype not in _DT:
         _bad("ckpt8_unpack", f"dtype {dtype}: float32 or bfloat16")
-    x = torch.empty(c.shape, dtype=dtype, device=c.buf.device)
+    x = c.buf.new_empty(c.shape, dtype=dtype)
     codes, exps = c._ptrs()
     _launch("mfnet_ckpt8_unpack", dev, x.numel() * x.element_size() + c.nbytes, 0, codes, exps, x.data_ptr(), _DT[dtype], c.C, c.rows, c.C)
     return x
@@ -1726,8 +1732,8 @@ def gelu_fwd_ckpt8(x):
     dev = _device_of(name, x)
     dt = _ck_dtype(name, x)
     x2, rows, C, ldx = _rows_any(name, x)
-    act = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    c = Ckpt8(x.shape, x.device)
+    act = _like(x, x.shape, x.dtype)
+    c = Ckpt8(x)
     codes, exps = c._ptrs()
     _launch("mfnet_gelu_fwd_ckpt8", dev, rows * C * (4 if dt else 8) + c.nbytes, 0, x2.data_ptr(), dt, ldx, act.data_ptr(), C, codes, exps, rows, C)
     return act, c
@@ -1741,7 +1747,7 @@ def gelu_bwd_ckpt8(c: Ckpt8, dy, want_act=False):
     if dy.shape != c.shape:
         _bad(name, f"dy {tuple(dy.shape)} does not match the checkpoint {c.shape}")
     d2, rows, C, ldd = _rows_any(name, dy)
-    dx = torch.empty(c.shape, dtype=dy.dtype, device=dy.device)
+    dx = _like(dy, c.shape, dy.dtype)
     act = torch.empty_like(dx) if want_act else None
     codes, exps = c._ptrs()
     _launch("mfnet_gelu_bwd_ckpt8", dev, rows * C * (3 if want_act else 2) * (2 if dt else 4) + c.nbytes, 0, codes, exps, d2.data_ptr(), dt, ldd,
@@ -1777,9 +1783,9 @@ def layernorm_fwd_ckpt8(x, gamma, beta, eps):
     _vec_f32(name, "gamma", gamma, C)
     _vec_f32(name, "beta", beta, C)
     gamma, beta = _aligned(gamma), _aligned(beta)
-    y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
-    mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
-    c = Ckpt8(x.shape, x.device)
+    y = _like(x, x.shape, torch.bfloat16)
+    mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind(0)
+    c = Ckpt8(x)
     codes, exps = c._ptrs()
     _launch("mfnet_layernorm_fwd_ckpt8", dev, rows * C * (4 if dt else 6) + c.nbytes + 8 * rows, 0, x2.data_ptr(), dt, ldx, gamma.data_ptr(), beta.data_ptr(),
             y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exps, rows, C, float(eps))
@@ -1809,16 +1815,15 @@ def layernorm_bwd_ckpt8(dy, c: Ckpt8, mean, rstd, gamma, beta=None, dres=None, w
             _bad(name, f"dres must be fp32 {c.shape}")
         dres = _aligned(dres.contiguous())
     gamma, beta = _aligned(gamma), _aligned(beta)
-    device = dy.device
-    dx = torch.empty(c.shape, dtype=torch.float32, device=device) if want_f32 else None
-    dxb = torch.empty(c.shape, dtype=torch.bfloat16, device=device) if want_bf16 else None
-    y = torch.empty(c.shape, dtype=torch.bfloat16, device=device) if want_y else None
+    dx = _like(dy, c.shape, torch.float32) if want_f32 else None
+    dxb = _like(dy, c.shape, torch.bfloat16) if want_bf16 else None
+    y = _like(dy, c.shape, torch.bfloat16) if want_y else None
     dg = db = ws = None
     nws = 0
     if want_weights:
         nws = _lib.lib().mfnet_layernorm_ckpt8_workspace_floats(rows, C)
-        dg, db = torch.empty((2, C), dtype=torch.float32, device=device).unbind(0)
-        ws = torch.empty(nws, dtype=torch.float32, device=device)
+        dg, db = gamma.new_empty((2, C)).unbind(0)
+        ws = gamma.new_empty((nws,))
     per_el = (2 if dt else 4) + (4 if dres is not None else 0) + (4 if want_f32 else 0) + (2 if want_bf16 else 0) + (2 if want_y else 0)
     codes, exps = c._ptrs()
     _launch("mfnet_layernorm_bwd_ckpt8", dev, rows * C * per_el + c.nbytes + 8 * rows, 0, d2.data_ptr(), dt, ldd, codes, exps, mean.data_ptr(),
@@ -1839,7 +1844,7 @@ def layernorm_y_ckpt8(c: Ckpt8, mean, rstd, gamma, beta):
     _vec_f32(name, "gamma", gamma, C)
     _vec_f32(name, "beta", beta, C)
     gamma, beta = _aligned(gamma), _aligned(beta)
-    y = torch.empty(c.shape, dtype=torch.bfloat16, device=c.buf.device)
+    y = c.buf.new_empty(c.shape, dtype=torch.bfloat16)
     codes, exps = c._ptrs()
     _launch("mfnet_layernorm_bwd_ckpt8", dev, 2 * rows * C + c.nbytes + 8 * rows, 0, None, BF16, 0, codes, exps, mean.data_ptr(), rstd.data_ptr(),
             gamma.data_ptr(), beta.data_ptr(), None, None, None, y.data_ptr(), None, None, None, 0, rows, C)
@@ -1944,8 +1949,8 @@ def lora_pool_fwd(x, w, bias, pool: LoraPool, ids, out_dtype=torch.bfloat16, wan
     if bias is not None:
         _vec_f32(name, "bias", bias, N)
         bias = _aligned(bias)
-    down = torch.empty((M, pool.RP), dtype=torch.float32, device=x.device)
-    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    down = x.new_empty((M, pool.RP), dtype=torch.float32)
+    out = x.new_empty((M, N), dtype=out_dtype)
     _launch("mfnet_lora_pool_fwd", dev, 2 * (M * K + N * K + pool.n * pool.r * (K + N)) + M * N * (2 if od else 4), 2.0 * M * (N * K + pool.r * (N + K)),
             x.data_ptr(), ldx, w.data_ptr(), ldw, _p(bias), pool.scale, pool.a_down, pool.b_up, ids.data_ptr(), pool.n, pool.RP, down.data_ptr(),
             out.data_ptr(), od, N, M, N, K)
@@ -1973,16 +1978,15 @@ def lora_pool_bwd(dy, x, w_t, pool: LoraPool, plan: LoraPlan, down, want_dx=True
     if down.shape != (M, RP) or down.dtype != torch.float32 or not down.is_contiguous():
         _bad(name, f"down must be the forward's fp32 [{M}, {RP}]")
     ldw, dx = 0, None
-    device = dy.device
     if want_dx:
         if w_t is None:
             _bad(name, "dx needs w_t")
         w_t, ldw = _bf16_rows(name, "w_t", w_t, K, N)
-        dx = torch.empty((M, K), dtype=torch.bfloat16, device=device)
-    dA = torch.empty((n, pool.r, K), dtype=torch.float32, device=device)
-    dB = torch.empty((n, N, pool.r), dtype=torch.float32, device=device)
+        dx = dy.new_empty((M, K))
+    dA = down.new_empty((n, pool.r, K))
+    dB = down.new_empty((n, N, pool.r))
     nws = _lib.lib().mfnet_lora_pool_bwd_workspace_floats(M, n, K, N, RP)
-    ws = torch.empty(nws, dtype=torch.float32, device=device)
+    ws = down.new_empty((nws,))
     _launch("mfnet_lora_pool_bwd", dev, 2 * M * (N + (2 * K if want_dx else 0)) + 4 * (dA.numel() + dB.numel()) + (2 * N * K if want_dx else 0),
             2.0 * M * ((N * K if want_dx else 0) + pool.r * (2 * N + 2 * K)), dy.data_ptr(), lddy, *src, w_t.data_ptr() if want_dx else None, ldw,
             pool.scale, pool.b_down, pool.a_up, plan.ids.data_ptr(), plan.perm.data_ptr(), plan.base.data_ptr(), plan.table.data_ptr(), n, pool.r, RP,
