@@ -558,8 +558,8 @@ int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, int64_t ldw, 
  * adapter's rows of p x^T, dB [n][N][r] = sum of dy down^T, fp32, overwritten; adapters without rows get zeros. x is the forward's input
  * as bf16 rows (X) or its 8-bit checkpoint (codes, exps; dense), one of the two. */
 int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, int64_t ldx, const void* codes, const void* exps, const void* Wt, int64_t ldwt,
-                        const float* scale, const void* b_down, const void* a_up, const int* ids, const int* perm, const int* base,
-                        const int* table, int64_t n, int r, int RP, const float* down, void* dx, int64_t lddx, float* dA, float* dB, float* ws,
+                        const float* scale, const void* b_down, const void* a_up, const int* ids, const int* offs, const int* perm,
+                        const int* base, const int* table, int64_t n, int r, int RP, const float* down, void* dx, int64_t lddx, float* dA, float* dB, float* ws,
                         int64_t ws_floats, int64_t M, int64_t N, int64_t K, hipStream_t stream);
 int64_t mfnet_lora_pool_bwd_workspace_floats(int64_t M, int64_t n, int64_t K, int64_t N, int RP);
 

@@ -139,7 +139,7 @@ _SIGS = {
     "mfnet_lora_pool_pack": [P, P, I, P, I64, I64, I64, I, I, P, P, P, P, P, P],
     "mfnet_lora_pool_plan": [P, I64, I64, P, P, P, P, P],
     "mfnet_lora_pool_fwd": [P, I64, P, I64, P, P, P, P, P, I64, I, P, P, I, I64, I64, I64, I64, P],
-    "mfnet_lora_pool_bwd": [P, I64, P, I64, P, P, P, I64, P, P, P, P, P, P, P, I64, I, I, P, P, I64, P, P, P, I64, I64, I64, I64, P],
+    "mfnet_lora_pool_bwd": [P, I64, P, I64, P, P, P, I64, P, P, P, P, P, P, P, P, I64, I, I, P, P, I64, P, P, P, I64, I64, I64, I64, P],
 }
 
 # host-side size helpers: name -> (restype, argtypes)

@@ -148,36 +148,107 @@ __global__ __launch_bounds__(256) void pool_chunks_kernel(const int* __restrict_
 }
 
 // ------------------------------------------------------------------------------------------------ down: s_i F_i y_m
+// One row by one wave: the MFMA's 16 columns all hold the row - a sixteenth of the products, but one instruction where 8 multiply-adds
+// and their conversions would stand. Four sums over every fourth k-step, as pool_down_row_kernel's waves have them: the same bits.
+// Lanes with fr = 0 hold the result: ranks 16 f + 4 fq + r.
+template <int NR>
+__device__ __forceinline__ void pool_row_sums(const bf16_t* __restrict__ x, const bf16_t* __restrict__ fp, int K, int lane, f32x4_t (&t)[NR]) {
+  const int fq = lane >> 4;
+  const u32x4_t zero = (u32x4_t){0u, 0u, 0u, 0u};
+  f32x4_t s[4][NR];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int f = 0; f < NR; ++f) s[q][f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  constexpr int IN = NR == 1 ? 8 : 4;                        // k-steps in flight
+  for (int ks0 = 0; 32 * ks0 < K; ks0 += IN) {
+    Frag xv[IN], a[IN][NR];
+#pragma unroll
+    for (int j = 0; j < IN; ++j) {
+      const int ks = ks0 + j;
+      const bool in = 32 * ks + 8 * fq < K;
+      xv[j].q = in ? *reinterpret_cast<const u32x4_t*>(x + 32 * ks + 8 * fq) : zero;
+#pragma unroll
+      for (int f = 0; f < NR; ++f) a[j][f].q = in ? *reinterpret_cast<const u32x4_t*>(fp + ((int64_t)ks * NR + f) * 512 + 8 * lane) : zero;
+    }
+#pragma unroll
+    for (int j = 0; j < IN; ++j)
+#pragma unroll
+      for (int f = 0; f < NR; ++f) s[j & 3][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][f].v, xv[j].v, s[j & 3][f], 0, 0, 0);
+  }
+#pragma unroll
+  for (int f = 0; f < NR; ++f) t[f] = (s[0][f] + s[1][f]) + (s[2][f] + s[3][f]);
+}
+template <int NR>
+__device__ __forceinline__ void pool_down_row(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
+                                              const int* __restrict__ ids, int n, float* __restrict__ out, int64_t m, int K, int lane) {
+  const int id = ids[m];
+  const bool on = (unsigned)id < (unsigned)n;
+  f32x4_t t[NR];
+#pragma unroll
+  for (int f = 0; f < NR; ++f) t[f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  if (on) {
+    pool_row_sums<NR>(X + m * ldx, F + id * pool_image(K, 16 * NR), K, lane, t);
+    const float s = scale[id];
+#pragma unroll
+    for (int f = 0; f < NR; ++f) t[f] *= s;
+  }
+  if ((lane & 15) == 0) {
+#pragma unroll
+    for (int f = 0; f < NR; ++f) *reinterpret_cast<float4*>(out + m * (16 * NR) + 16 * f + 4 * (lane >> 4)) = make_float4(t[f][0], t[f][1], t[f][2], t[f][3]);
+  }
+}
+
 // 16 XR rows per workgroup, the four waves take every fourth piece of 64 columns. The factor is the MFMA's "A" operand, the rows its "B"
 // operand, so a lane ends with four consecutive ranks of row fr. Bound by reading the rows once. Both operands come through a ring of
 // three pieces in LDS of the wave's own (global_load_lds, counted vmcnt, no barrier): rows in whole 128-byte lines, swizzled, the factor
 // as dense KBs of its image. Read straight into registers the rows go 64 bytes at a time and the factor's rows again as often as the
 // rows themselves: 77 us for [32768, 3840] instead of 60.
+// perm: the k-th row of the call is perm[k], and only the *count rows that have an adapter are taken (the backward pass, whose plan has
+// them grouped). A workgroup that meets more adapters than pay takes its rows one by one: each of the rows' own factor once, where the
+// other way reads all its rows again for every adapter (20000 rows in random order over 48 adapters, K = 1280: 147 us to 90).
 template <int NR, int XR>      // NR = RP / 16
 __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
-                                                        const int* __restrict__ ids, int n, float* __restrict__ out, int64_t M, int K) {
+                                                        const int* __restrict__ ids, int n, const int* __restrict__ perm, const int* __restrict__ count,
+                                                        float* __restrict__ out, int64_t M, int K) {
   constexpr int RING = 3, XL = 2 * XR, FL = 2 * NR, PIECE = (XL + FL) * 1024;      // requests of 1 KB per piece: rows, factor
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4][RING][PIECE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4;
   const int64_t mw = (int64_t)blockIdx.x * (16 * XR);
+  if (count) M = *count;
+  if (mw >= M) return;
+  auto row_of = [&](int64_t k) { k = k < M ? k : M - 1; return perm ? (int64_t)perm[k] : k; };
   int id[XR];
+  int64_t mrow[XR];
   f32x4_t sel[XR][NR];
 #pragma unroll
   for (int b = 0; b < XR; ++b) {
-    const int64_t m = mw + 16 * b + fr;
-    id[b] = m < M ? ids[m] : -1;
+    mrow[b] = row_of(mw + 16 * b + fr);
+    id[b] = mw + 16 * b + fr < M ? ids[mrow[b]] : -1;
     if ((unsigned)id[b] >= (unsigned)n) id[b] = -1;
 #pragma unroll
     for (int f = 0; f < NR; ++f) sel[b][f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   }
+  {
+    constexpr int FEW = XR == 1 ? 8 : 10;                    // reads of all rows and a factor against reads of a factor per row
+    int met = 0;
+    for (int last = -1; met <= FEW; ++met) {
+      int cand = NO_ID;
+#pragma unroll
+      for (int b = 0; b < XR; ++b) cand = id[b] > last && id[b] < cand ? id[b] : cand;
+      last = next_id(cand);
+      if (last == NO_ID) break;
+    }
+    if (met > FEW) {
+      for (int j = wave; j < 16 * XR && mw + j < M; j += 4) pool_down_row<NR>(X, ldx, F, scale, ids, n, out, row_of(mw + j), K, lane);
+      return;
+    }
+  }
   const bf16_t* src[XL];                                     // request i: rows 8 i + (lane >> 3), chunk (lane & 7) of its 128 bytes
   const int swz = (lane & 7) ^ (lane >> 3);
 #pragma unroll
-  for (int i = 0; i < XL; ++i) {
-    const int64_t m = mw + 8 * i + (lane >> 3);
-    src[i] = X + (m < M ? m : M - 1) * ldx + 8 * swz;
-  }
+  for (int i = 0; i < XL; ++i) src[i] = X + row_of(mw + 8 * i + (lane >> 3)) * ldx + 8 * swz;
   const int np = ((K + 63) / 64 - wave + 3) / 4;             // pieces of this wave (0 if it has none)
   unsigned char* ring = lds[wave][0];
   for (int last = -1;;) {
@@ -246,8 +317,7 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
   if (wave) return;
 #pragma unroll
   for (int b = 0; b < XR; ++b) {
-    const int64_t m = mw + 16 * b + fr;
-    if (m >= M) continue;
+    if (mw + 16 * b + fr >= M) continue;
     const float s = id[b] >= 0 ? scale[id[b]] : 0.f;
 #pragma unroll
     for (int f = 0; f < NR; ++f) {
@@ -255,14 +325,12 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
       const f32x4_t t = (sel[b][f] + red[0][i][lane]) + (red[1][i][lane] + red[2][i][lane]);
       // (no adapter: zeros, whatever the sums hold)
       const float4 o = id[b] >= 0 ? make_float4(s * t[0], s * t[1], s * t[2], s * t[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<float4*>(out + m * (16 * NR) + 16 * f + 4 * fq) = o;
+      *reinterpret_cast<float4*>(out + mrow[b] * (16 * NR) + 16 * f + 4 * fq) = o;
     }
   }
 }
 
-// Few rows, an adapter each as it may be: one row per workgroup, the four waves take every fourth k-step. The MFMA's 16 columns all hold
-// the one row: a sixteenth of the products, but one instruction where 8 multiply-adds and their conversions would stand. All requests are
-// independent of each other, where the kernel above takes the adapters of its rows one after the other.
+// Few rows: one row per workgroup, the four waves take every fourth k-step.
 template <int NR>
 __global__ __launch_bounds__(256) void pool_down_row_kernel(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
                                                             const int* __restrict__ ids, int n, float* __restrict__ out, int K) {
@@ -331,8 +399,25 @@ template <int G> __device__ __forceinline__ int pool_out_col(int fq, int i) { re
 // Low-rank update, bias and store of a wave's tile: the lane owns rows m0 + r0 + 16 b and four columns per fragment (pool_out_col; rows past
 // the end repeat the last one and are not stored). The update is MFMA k-steps of 32 slots: RP = 16: ranks 0..15 of the factor's part hi,
 // then of its part lo; wider: 32 ranks of one part. A bf16 result needs 16 bits of the fp32 factor (hi + lo), an fp32 one a third part.
-template <int XF, int G>
-__device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[G][XF], int64_t m0, int r0, int ncol, int fr, int fq, unsigned char* bounce) {
+// `pre`: indices and, at RP = 16, the factors, requested before the main loop where registers allow (PRE).
+template <int XF> struct PoolPre { int id[XF]; float4 d[XF][2]; };
+template <int XF>
+__device__ __forceinline__ void pool_prefetch(const PoolGemm& p, PoolPre<XF>& pre, int64_t m0, int r0, int fq) {
+  if (!p.D) return;
+  const int mlim = p.M - m0 - 1 < r0 + 16 * XF ? (int)(p.M - m0) - 1 : r0 + 16 * XF;
+#pragma unroll
+  for (int b = 0; b < XF; ++b) {
+    const int r = r0 + 16 * b < mlim ? r0 + 16 * b : mlim;
+    pre.id[b] = p.ids[m0 + r];
+    if (p.RP == 16) {
+      const float4* d = reinterpret_cast<const float4*>(p.D + (m0 + r) * 16 + 8 * (fq & 1));
+      pre.d[b][0] = d[0];
+      pre.d[b][1] = d[1];
+    }
+  }
+}
+template <int XF, int G, bool PRE>
+__device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[G][XF], int64_t m0, int r0, int ncol, int fr, int fq, unsigned char* bounce, const PoolPre<XF>& pre) {
   const int mlim = p.M - m0 - 1 < r0 + 16 * XF ? (int)(p.M - m0) - 1 : r0 + 16 * XF;       // last row of the matrix, from m0
   if (p.D) {
     const int* ids = p.ids + m0;
@@ -342,7 +427,7 @@ __device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[
 #pragma unroll
     for (int b = 0; b < XF; ++b) {
       const int r = r0 + 16 * b;
-      id[b] = ids[r < mlim ? r : mlim];
+      id[b] = PRE ? pre.id[b] : ids[r < mlim ? r : mlim];
       if ((unsigned)id[b] >= (unsigned)p.n) id[b] = -1;
     }
     const bool wide = RP > 16;
@@ -355,7 +440,8 @@ __device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[
       for (int b = 0; b < XF; ++b) {
         const int r = r0 + 16 * b;
         const float4* d = reinterpret_cast<const float4*>(D + ((r < mlim ? r : mlim) * RP + rk));
-        const float4 d0 = d[0], d1 = d[1];
+        const bool have = PRE && !wide;
+        const float4 d0 = have ? pre.d[b][0] : d[0], d1 = have ? pre.d[b][1] : d[1];
         const float x[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -365,28 +451,40 @@ __device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[
           u[b].w[i] = part == 0 ? hi : (part == 1 ? lo : (part == 2 ? l2 : 0u));
         }
       }
-      for (int last = -1;;) {
+      auto above = [&](int last) __attribute__((always_inline)) {
         int cand = NO_ID;
 #pragma unroll
         for (int b = 0; b < XF; ++b) cand = id[b] > last && id[b] < cand ? id[b] : cand;
-        const int cur = next_id(cand);
-        if (cur == NO_ID) break;
-        last = cur;
-        const bf16_t* up = p.Up + (int64_t)cur * p.N * RP;
-        Frag f[G];
+        return next_id(cand);
+      };
+      auto factors = [&](int i, Frag (&f)[G]) __attribute__((always_inline)) {
+        const bf16_t* up = p.Up + (int64_t)i * p.N * RP;
 #pragma unroll
         for (int a = 0; a < G; ++a) {
           const int c = ncol + pool_col<G>(fr, a);
           f[a].q = *reinterpret_cast<const u32x4_t*>(up + ((int64_t)(c < p.N ? c : p.N - 1) * RP + rk));
         }
+      };
+      Frag f[G];
+      int cur = above(-1);
+      if (cur != NO_ID) factors(cur, f);
+      while (cur != NO_ID) {                                               // the next adapter's factors are on their way meanwhile
+        const int nxt = above(cur);
+        Frag g[G];
+        if (nxt != NO_ID) factors(nxt, g);
 #pragma unroll
-        for (int b = 0; b < XF; ++b)
+        for (int b = 0; b < XF; ++b) {
+          if (!__any(id[b] == cur)) continue;                              // (none of these 16 rows)
 #pragma unroll
           for (int a = 0; a < G; ++a) {
             const f32x4_t t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[a].v, u[b].v, acc[a][b], 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[a][b][r] = id[b] == cur ? t[r] : acc[a][b][r];
           }
+        }
+#pragma unroll
+        for (int a = 0; a < G; ++a) f[a] = g[a];
+        cur = nxt;
       }
     }
   }
@@ -557,39 +655,21 @@ __global__ __launch_bounds__(1024) void pool_rows_fused_kernel(const PoolGemm p,
   if (wave < M) {
     const int id = my;
     const bool on = (unsigned)id < (unsigned)p.n;
-    f32x4_t s[4][NR];                                        // four sums over every fourth k-step: the order of pool_down_row_kernel, the same bits
+    f32x4_t s[NR];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int f = 0; f < NR; ++f) s[q][f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    for (int f = 0; f < NR; ++f) s[f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    float sc = 0.f;
     if (on) {
-      const bf16_t* fp = F + id * pool_image(K, RP) + 8 * lane;
-      const bf16_t* xr = p.X + (int64_t)wave * p.ldx + 8 * fq;
-      constexpr int IN = NR == 1 ? 8 : 4;                    // k-steps in flight
-      for (int ks0 = 0; 32 * ks0 < K; ks0 += IN) {
-        Frag xv[IN], a[IN][NR];
-#pragma unroll
-        for (int j = 0; j < IN; ++j) {
-          const int ks = ks0 + j;
-          const bool in = 32 * ks + 8 * fq < K;
-          xv[j].q = in ? *reinterpret_cast<const u32x4_t*>(xr + 32 * ks) : zero;
-#pragma unroll
-          for (int f = 0; f < NR; ++f) a[j][f].q = in ? *reinterpret_cast<const u32x4_t*>(fp + ((int64_t)ks * NR + f) * 512) : zero;
-        }
-#pragma unroll
-        for (int j = 0; j < IN; ++j)
-#pragma unroll
-          for (int f = 0; f < NR; ++f) s[j & 3][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j][f].v, xv[j].v, s[j & 3][f], 0, 0, 0);
-      }
+      sc = scale[id];
+      pool_row_sums<NR>(p.X + (int64_t)wave * p.ldx, F + id * pool_image(K, RP), K, lane, s);
     }
-    const float sc = on ? scale[id] : 0.f;
     if (fr == 0) {
 #pragma unroll
       for (int f = 0; f < NR; ++f)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = 16 * f + 4 * fq + r;
-          const float v = on ? sc * ((s[0][f][r] + s[1][f][r]) + (s[2][f][r] + s[3][f][r])) : 0.f;
+          const float v = on ? sc * s[f][r] : 0.f;
           dn[wave][j] = v;
           if (blockIdx.x == 0) down[wave * RP + j] = v;
         }
@@ -658,28 +738,33 @@ __device__ __forceinline__ void pool_tile(const PoolGemm& p, int* tm, int* tn) {
   *tn = rem / rows;
 }
 
-// WM x WN waves, each 16 XF rows x 16 G columns; k-tiles of 64 in two LDS buffers filled by global_load_lds. The W rows are the MFMA's
-// "A" operand, read in a permuted order so that a lane ends with 4 G consecutive columns of row fr of each row fragment.
-template <int WM, int WN, int XF, int G>
-__global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void pool_gemm_kernel(const PoolGemm p) {
-  constexpr int NW = WM * WN, BM = 16 * XF * WM, BN = 16 * G * WN, ROWS = BM + BN, STAGE = ROWS * 128, PPW = ROWS / 8 / NW;
-  static_assert(ROWS % (8 * NW) == 0, "whole 1-KB pieces per wave");
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
+// Few tiles: 64 x 64 columns per workgroup, waves of 32 x 32, k-tiles of 64 in a ring of three LDS buffers filled by global_load_lds two
+// tiles ahead; KS groups of four waves take every KS-th k-tile, each with a ring of its own, and add up through LDS at the end (a chip
+// that is not full is bound by the length of this loop: 0.36 us per k-tile). One barrier per k-tile: behind it every wave's requests of
+// tile t have landed and every wave is done with tile t - 1, whose buffer takes tile t + 2. The W rows are the MFMA's "A" operand.
+template <int KS>
+__global__ __launch_bounds__(256 * KS) void pool_gemm_kernel(const PoolGemm p) {
+  constexpr int WN = 2, XF = 2, G = 2, RING = 3, BM = 64, BN = 64, ROWS = BM + BN, STAGE = ROWS * 128, PPW = ROWS / 8 / 4;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds_all[KS * RING * STAGE];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave_all >> 2, wave = wave_all & 3;
+  unsigned char* lds = lds_all + kg * RING * STAGE;
   const int wm = wave / WN, wn = wave % WN;
   const int fr = lane & 15, fq = lane >> 4;
   int tm, tn;
   pool_tile(p, &tm, &tn);
   const int64_t m0 = (int64_t)tm * BM;
   const int n0 = tn * BN;
+  PoolPre<XF> pre;
+  if (kg == 0) pool_prefetch<XF>(p, pre, m0, wm * 16 * XF + fr, fq);
 
   // staging: piece j holds stage rows 8j .. 8j+7; lane -> row 8j + (lane >> 3), destination chunk lane & 7
   const bf16_t* src[PPW];
   int kch[PPW];
 #pragma unroll
   for (int i = 0; i < PPW; ++i) {
-    const int row = 8 * (wave + NW * i) + (lane >> 3);
+    const int row = 8 * (wave + 4 * i) + (lane >> 3);
     if (row < BM) {
       const int64_t m = m0 + row < p.M ? m0 + row : p.M - 1;           // rows and columns past the end repeat the last one: never stored
       kch[i] = ((lane & 7) ^ (row & 7)) << 3;
@@ -690,61 +775,71 @@ __global__ __launch_bounds__(64 * WM * WN, (WM * WN) / 4) void pool_gemm_kernel(
       src[i] = p.W + (int64_t)nn * p.ldw + kch[i];
     }
   }
-  const int nt = (p.K + 63) / 64;
-  auto stage = [&](int kt, int buf) {
-    unsigned char* base = lds + buf * STAGE;
+  const int nt_all = (p.K + 63) / 64, rounds = (nt_all + KS - 1) / KS, nt = (nt_all - kg + KS - 1) / KS;      // k-tiles of this group: kg + KS t
+  auto stage = [&](int t) {
+    unsigned char* base = lds + (t % RING) * STAGE;
+    const int kt = kg + KS * t;
 #pragma unroll
     for (int i = 0; i < PPW; ++i) {
       const bf16_t* s = src[i] + kt * 64;
       if (kt * 64 + 64 > p.K) s = kt * 64 + kch[i] < p.K ? s : reinterpret_cast<const bf16_t*>(g_pool_zero);     // (uniform branch: the last k-tile of a ragged K)
-      __builtin_amdgcn_global_load_lds((gbl_ptr_t)s, (lds_ptr_t)(base + (wave + NW * i) * 1024), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((gbl_ptr_t)s, (lds_ptr_t)(base + (wave + 4 * i) * 1024), 16, 0, 0);
     }
   };
 
-  int x_off[XF], x_sw, w_off[G], w_sw[G];
-#pragma unroll
-  for (int i = 0; i < XF; ++i) x_off[i] = (wm * 16 * XF + i * 16 + fr) * 128;
-  x_sw = fr & 7;
-#pragma unroll
-  for (int i = 0; i < G; ++i) {
-    const int o = pool_col<G>(fr, i);
-    w_off[i] = (BM + wn * 16 * G + o) * 128;
-    w_sw[i] = pool_swz_w<G>(o);
-  }
+  const int x_row = (wm * 16 * XF + fr) * 128, x_sw = fr & 7;
+  const int w_row = (BM + wn * 16 * G + pool_col<G>(fr, 0)) * 128, w_sw = pool_swz_w<G>(pool_col<G>(fr, 0));      // (fragment 1: 4 rows further, the same swizzle)
   f32x4_t acc[G][XF];
 #pragma unroll
   for (int a = 0; a < G; ++a)
 #pragma unroll
     for (int b = 0; b < XF; ++b) acc[a][b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
-  stage(0, 0);
-  for (int t = 0; t < nt; ++t) {
-    if (t + 1 < nt) {
-      stage(t + 1, (t + 1) & 1);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PPW) : "memory");      // tile t landed, tile t + 1 in flight
-    } else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  for (int t = 0; t < RING - 1 && t < nt; ++t) stage(t);
+  for (int t = 0; t < rounds; ++t) {
+    if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PPW) : "memory");      // tile t landed, tile t + 1 may be in flight
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // this wave's reads of tile t - 1
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const unsigned char* base = lds + (t & 1) * STAGE;
+    if (t >= nt) continue;                                            // (the other groups' last round)
+    if (t + RING - 1 < nt) stage(t + RING - 1);
+    const unsigned char* base = lds + (t % RING) * STAGE;
+    bf16x8_t xf[2][XF], wf[2][G];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      bf16x8_t xf[XF], wf[G];
       const int ch = fq + 4 * ks;
 #pragma unroll
-      for (int i = 0; i < XF; ++i) xf[i] = *reinterpret_cast<const bf16x8_t*>(base + x_off[i] + ((ch ^ x_sw) << 4));
+      for (int i = 0; i < XF; ++i) xf[ks][i] = *reinterpret_cast<const bf16x8_t*>(base + x_row + i * 2048 + ((ch ^ x_sw) << 4));
 #pragma unroll
-      for (int i = 0; i < G; ++i) wf[i] = *reinterpret_cast<const bf16x8_t*>(base + w_off[i] + ((ch ^ w_sw[i]) << 4));
+      for (int i = 0; i < G; ++i) wf[ks][i] = *reinterpret_cast<const bf16x8_t*>(base + w_row + i * 512 + ((ch ^ w_sw) << 4));
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int a = 0; a < G; ++a)
 #pragma unroll
-        for (int b = 0; b < XF; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[a], xf[b], acc[a][b], 0, 0, 0);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // this wave's reads of tile t are done: its buffer may be refilled
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+        for (int b = 0; b < XF; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[ks][a], xf[ks][b], acc[a][b], 0, 0, 0);
   }
-
-  pool_epilogue<XF, G>(p, acc, m0, wm * 16 * XF + fr, n0 + wn * 16 * G, fr, fq, nullptr);
+  if (KS > 1) {
+    __syncthreads();
+    f32x4_t* red = reinterpret_cast<f32x4_t*>(lds_all);
+    if (kg) {
+#pragma unroll
+      for (int a = 0; a < G; ++a)
+#pragma unroll
+        for (int b = 0; b < XF; ++b) red[(((kg - 1) * 4 + wave) * (G * XF) + a * XF + b) * 64 + lane] = acc[a][b];
+    }
+    __syncthreads();
+    if (kg) return;
+#pragma unroll
+    for (int g = 0; g < KS - 1; ++g)
+#pragma unroll
+      for (int a = 0; a < G; ++a)
+#pragma unroll
+        for (int b = 0; b < XF; ++b) acc[a][b] += red[((g * 4 + wave) * (G * XF) + a * XF + b) * 64 + lane];
+  }
+  pool_epilogue<XF, G, true>(p, acc, m0, wm * 16 * XF + fr, n0 + wn * 16 * G, fr, fq, nullptr, pre);
 }
 
 // The same product for many rows: 8 waves as 2 (rows) x 4 (columns), wave tile 16 XF x 16 G, two k-tiles of 64 in LDS. A k-tile is
@@ -935,7 +1030,8 @@ __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_ke
     read_x(1);
     mul(1, 0, G);
   }
-  pool_epilogue<XF, G>(p, acc, m0, wm * 16 * XF + fr, n0 + wn * 16 * G, fr, fq, lds + wave * 8192);
+  const PoolPre<XF> none = {};
+  pool_epilogue<XF, G, false>(p, acc, m0, wm * 16 * XF + fr, n0 + wn * 16 * G, fr, fq, lds + wave * 8192, none);
 #endif
 }
 
@@ -1143,10 +1239,12 @@ extern "C" int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* o
   return MFNET_OK;
 }
 
-static int pool_down(const void* X, int64_t ldx, const void* image, const float* scale, const int* ids, int64_t n, int RP, float* out, int64_t M, int64_t K, hipStream_t stream) {
+// perm / count: the rows that have an adapter, grouped by it (NULL: the rows as they come; every row of out is written)
+static int pool_down(const void* X, int64_t ldx, const void* image, const float* scale, const int* ids, int64_t n, int RP, const int* perm, const int* count, float* out, int64_t M,
+                     int64_t K, hipStream_t stream) {
   // Up to 256 rows: a workgroup per row is quicker than 16 rows and their adapters in turn. 32 rows per workgroup halve the factor's
   // traffic where there are enough of them to fill the chip.
-#define PDL(NR_, XR_) hipLaunchKernelGGL((pool_down_kernel<NR_, XR_>), dim3((unsigned)ceil_div64(M, 16 * XR_)), dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)image, scale, ids, (int)n, out, M, (int)K)
+#define PDL(NR_, XR_) hipLaunchKernelGGL((pool_down_kernel<NR_, XR_>), dim3((unsigned)ceil_div64(M, 16 * XR_)), dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)image, scale, ids, (int)n, perm, count, out, M, (int)K)
 #define PD(NR_) do { \
     if (M <= 256) hipLaunchKernelGGL((pool_down_row_kernel<NR_>), dim3((unsigned)M), dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)image, scale, ids, (int)n, out, (int)K); \
     else if (M < 8192) PDL(NR_, 1); else PDL(NR_, 2); } while (0)
@@ -1159,34 +1257,42 @@ static int pool_down(const void* X, int64_t ldx, const void* image, const float*
 
 static int pool_gemm(PoolGemm& p, hipStream_t stream) {
   const int64_t M = p.M, N = p.N;
-  const double iters = (p.K + 63) / 64;
   auto tiles = [&](int bm, int bn) { p.tiles_m = (int)ceil_div64(M, bm); p.tiles_n = (int)ceil_div64(N, bn); return (int64_t)p.tiles_m * p.tiles_n; };
 #define PR(XF_) hipLaunchKernelGGL((pool_gemm_rows_kernel<XF_>), dim3((unsigned)ceil_div64(N, 16)), dim3(256), 0, stream, p)
   if (M <= 32) PR(2);
   else if (M <= 64) PR(4);
 #undef PR
   else {
-    // The tile is the one with the least modelled time: rounds of the 256 CUs x (k-tiles x time of one + what a tile costs beside them),
-    // in us, as measured at K = 768 .. 8192 (256 x 256: 0.72 us and 10; 128 x 192, two workgroups per CU: 0.6 and 7; 64 x 64, up to four:
-    // 0.25 and 3 alone).
-    const bool ld_ok = p.ldx <= (1 << 22) && p.ldw <= (1 << 22);         // the phased kernel's 32-bit offsets
-    const double r84 = ceil(ceil_div64(M, 256) * (double)ceil_div64(N, 256) / 256), c84 = r84 * (iters * 1.45 + 11);
-    const double r43 = ceil(ceil_div64(M, 128) * (double)ceil_div64(N, 192) / 256), c43 = r43 * (iters * 0.63 + 7);
-    const double t64 = ceil_div64(M, 64) * (double)ceil_div64(N, 64), c64 = (t64 <= 512 ? 1.0 : t64 / 512) * iters * 0.5 + 4;
-    const int64_t nwg = !ld_ok || (c64 <= c84 && c64 <= c43) ? tiles(64, 64) : c84 <= c43 ? tiles(256, 256) : tiles(128, 192);
+    // The tile with the least modelled time, in us, as measured at K = 64 .. 8192 on 100 .. 32768 rows: a tile costs a fixed part and a
+    // part per k-tile. 256 x 256: one workgroup per CU, so whole rounds of the 256 CUs count. 128 x 192 and 128 x 128: two per CU, which
+    // hide each other's fixed part; an odd one runs alone. 64 x 64: three or four per CU; with no more tiles than CUs two groups of waves split K.
+    const double it = (p.K + 63) / 64;
+    auto rounds = [&](int bm, int bn) { return ceil((double)ceil_div64(M, bm) * (double)ceil_div64(N, bn) / 256); };
+    auto paired = [&](double r, double fix, double per2, double per1) { return floor(r / 2) * (fix + 2 * per2 * it) + (r - 2 * floor(r / 2)) * (fix + per1 * it); };
+    const double t64 = (double)ceil_div64(M, 64) * (double)ceil_div64(N, 64);
+    const bool split = t64 <= 256 && it >= 4;
+    const double cost[4] = {4.5 + (split ? 0.5 : 1.0) * it * (0.33 + 0.2 * t64 / 256), paired(rounds(128, 128), 5.3, 0.66, 0.72), paired(rounds(128, 192), 6.3, 0.70, 0.74),
+                            rounds(256, 256) * (10 + 1.47 * it)};
+    int best = 0;
+    if (p.ldx <= (1 << 22) && p.ldw <= (1 << 22))                         // (the phased kernel's 32-bit offsets)
+      for (int i = 1; i < 4; ++i) best = cost[i] < cost[best] ? i : best;
+    const int64_t nwg = best == 0 ? tiles(64, 64) : best == 1 ? tiles(128, 128) : best == 2 ? tiles(128, 192) : tiles(256, 256);
     MF_CHECK_ARG(nwg < (1ll << 31), "lora_pool: too many tiles");
-    if (!ld_ok || (c64 <= c84 && c64 <= c43)) hipLaunchKernelGGL((pool_gemm_kernel<2, 2, 2, 2>), dim3((unsigned)nwg), dim3(256), 0, stream, p);
-    else if (c84 <= c43) hipLaunchKernelGGL((pool_gemm_phased_kernel<8, 4>), dim3((unsigned)nwg), dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((pool_gemm_phased_kernel<4, 3>), dim3((unsigned)nwg), dim3(512), 0, stream, p);
+    const dim3 grid((unsigned)nwg);
+    if (best == 0 && split) hipLaunchKernelGGL((pool_gemm_kernel<2>), grid, dim3(512), 0, stream, p);
+    else if (best == 0) hipLaunchKernelGGL((pool_gemm_kernel<1>), grid, dim3(256), 0, stream, p);
+    else if (best == 1) hipLaunchKernelGGL((pool_gemm_phased_kernel<4, 2>), grid, dim3(512), 0, stream, p);
+    else if (best == 2) hipLaunchKernelGGL((pool_gemm_phased_kernel<4, 3>), grid, dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((pool_gemm_phased_kernel<8, 4>), grid, dim3(512), 0, stream, p);
   }
   MF_LAUNCH_CHECK("lora_pool (product)");
   return MFNET_OK;
 }
 
 // down = scale_i image_i x, out = x W^T (+ bias) + up_i down
-static int pool_products(PoolGemm& p, const void* image, const float* scale, float* down, hipStream_t stream) {
+static int pool_products(PoolGemm& p, const void* image, const float* scale, const int* perm, const int* count, float* down, hipStream_t stream) {
   if (p.M > 16 || p.RP > 32) {                              // (64 ranks: more registers than 16 waves have)
-    const int rc = pool_down(p.X, p.ldx, image, scale, p.ids, p.n, p.RP, down, p.M, p.K, stream);
+    const int rc = pool_down(p.X, p.ldx, image, scale, p.ids, p.n, p.RP, perm, count, down, p.M, p.K, stream);
     return rc ? rc : pool_gemm(p, stream);
   }
   const dim3 grid((unsigned)ceil_div64(p.N, 32));
@@ -1213,7 +1319,7 @@ extern "C" int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, in
   p.D = down; p.Up = (const bf16_t*)b_up; p.ids = ids; p.n = (int)n; p.RP = RP;
   p.out = out; p.ldo = ldo; p.out_f32 = out_dtype == MFNET_F32;
   p.M = M; p.N = (int)N; p.K = (int)K;
-  return pool_products(p, a_down, scale, down, stream);
+  return pool_products(p, a_down, scale, nullptr, nullptr, down, stream);
 }
 
 // floats of workspace of mfnet_lora_pool_bwd: p [M, RP] and the partial sums of dA and dB
@@ -1222,8 +1328,8 @@ extern "C" int64_t mfnet_lora_pool_bwd_workspace_floats(int64_t M, int64_t n, in
 }
 
 extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, int64_t ldx, const void* codes, const void* exps, const void* Wt, int64_t ldwt,
-                                   const float* scale, const void* b_down, const void* a_up, const int* ids, const int* perm, const int* base, const int* table,
-                                   int64_t n, int r, int RP, const float* down, void* dx, int64_t lddx, float* dA, float* dB, float* ws, int64_t ws_floats,
+                                   const float* scale, const void* b_down, const void* a_up, const int* ids, const int* offs, const int* perm, const int* base,
+                                   const int* table, int64_t n, int r, int RP, const float* down, void* dx, int64_t lddx, float* dA, float* dB, float* ws, int64_t ws_floats,
                                    int64_t M, int64_t N, int64_t K, hipStream_t stream) {
   MF_CHECK_ARG(pool_counts(M, n) && pool_rp(RP) && r >= 1 && r <= RP, "lora_pool_bwd: bad sizes (M=%lld n=%lld r=%d RP=%d)", (long long)M, (long long)n, r, RP);
   MF_CHECK_ARG(K >= 8 && K % 8 == 0 && K < (1 << 24) && N >= 8 && N % 8 == 0 && N < (1 << 24), "lora_pool_bwd: K=%lld and N=%lld must be multiples of 8", (long long)K, (long long)N);
@@ -1232,7 +1338,7 @@ extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, 
   float* part_a = ws + M * RP;
   float* part_b = part_a + chunks * K * RP;
   if (M > 0) {
-    MF_CHECK_ARG(dy && scale && b_down && ids && perm && table && down && ws && (!dx || (Wt && a_up)), "lora_pool_bwd: null pointer");
+    MF_CHECK_ARG(dy && scale && b_down && ids && offs && perm && table && down && ws && (!dx || (Wt && a_up)), "lora_pool_bwd: null pointer");
     MF_CHECK_ARG((X != nullptr) != (codes != nullptr) && (!codes || exps), "lora_pool_bwd: the input either as bf16 rows or as a checkpoint");
     POOL_CHECK_ROWS("lora_pool_bwd (dy)", dy, lddy, N);
     if (X) POOL_CHECK_ROWS("lora_pool_bwd (x)", X, ldx, K);
@@ -1242,14 +1348,14 @@ extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, 
     MF_CHECK_ARG(ws_floats >= mfnet_lora_pool_bwd_workspace_floats(M, n, K, N, RP), "lora_pool_bwd: workspace too small");
     MF_CHECK_ARG(chunks <= 65535, "lora_pool_bwd: too many chunks of rows (%lld)", (long long)chunks);
     int rc;
-    if (!dx) rc = pool_down(dy, lddy, b_down, scale, ids, n, RP, ws, M, N, stream);
+    if (!dx) rc = pool_down(dy, lddy, b_down, scale, ids, n, RP, perm, offs + n, ws, M, N, stream);
     else {
       PoolGemm p;
       p.X = (const bf16_t*)dy; p.ldx = lddy; p.W = (const bf16_t*)Wt; p.ldw = ldwt; p.bias = nullptr;
       p.D = ws; p.Up = (const bf16_t*)a_up; p.ids = ids; p.n = (int)n; p.RP = RP;
       p.out = dx; p.ldo = lddx; p.out_f32 = 0;
       p.M = M; p.N = (int)K; p.K = (int)N;
-      rc = pool_products(p, b_down, scale, ws, stream);
+      rc = pool_products(p, b_down, scale, perm, offs + n, ws, stream);
     }
     if (rc) return rc;
     PoolTn a, b;

@@ -1989,6 +1989,6 @@ def lora_pool_bwd(dy, x, w_t, pool: LoraPool, plan: LoraPlan, down, want_dx=True
     ws = down.new_empty((nws,))
     _launch("mfnet_lora_pool_bwd", dev, 2 * M * (N + (2 * K if want_dx else 0)) + 4 * (dA.numel() + dB.numel()) + (2 * N * K if want_dx else 0),
             2.0 * M * ((N * K if want_dx else 0) + pool.r * (2 * N + 2 * K)), dy.data_ptr(), lddy, *src, w_t.data_ptr() if want_dx else None, ldw,
-            pool.scale, pool.b_down, pool.a_up, plan.ids.data_ptr(), plan.perm.data_ptr(), plan.base.data_ptr(), plan.table.data_ptr(), n, pool.r, RP,
+            pool.scale, pool.b_down, pool.a_up, plan.ids.data_ptr(), plan.offs.data_ptr(), plan.perm.data_ptr(), plan.base.data_ptr(), plan.table.data_ptr(), n, pool.r, RP,
             down.data_ptr(), _p(dx), K, dA.data_ptr(), dB.data_ptr(), _p(ws), nws, M, N, K)
     return dx, dA, dB

@@ -41,7 +41,7 @@ def test_entry_points_refuse_bad_arguments_before_a_launch():
                         ("RP", 17, b"sizes"), ("n", 0, b"sizes"), ("M", 1 << 31, b"sizes"), ("dt", 2, b"dtype"), ("down", None, b"null"), ("b_up", 24, b"misaligned"), ("ids", None, b"null")):
         assert L.mfnet_lora_pool_fwd(*dict(fwd, **{key: v}).values()) == -1 and msg in E(), key
     assert L.mfnet_lora_pool_fwd(*dict(fwd, M=0).values()) == 0
-    bwd = dict(dy=16, lddy=64, X=16, ldx=64, codes=None, exps=None, Wt=16, ldwt=64, scale=16, b_down=16, a_up=16, ids=16, perm=16, base=16, table=16, n=2, r=4, RP=16, down=16,
+    bwd = dict(dy=16, lddy=64, X=16, ldx=64, codes=None, exps=None, Wt=16, ldwt=64, scale=16, b_down=16, a_up=16, ids=16, offs=16, perm=16, base=16, table=16, n=2, r=4, RP=16, down=16,
                dx=16, lddx=64, dA=16, dB=16, ws=16, nws=1 << 20, M=8, N=64, K=64, s=None)
     for key, v, msg in (("codes", 16, b"either"), ("X", None, b"either"), ("lddy", 60, b"dy"), ("ldx", 60, b"(x)"), ("ldwt", 56, b"weight"), ("lddx", 60, b"dx"), ("r", 17, b"sizes"),
                         ("nws", 100, b"workspace"), ("dA", None, b"null"), ("table", 24, b"misaligned"), ("K", 68, b"multiples of 8"), ("Wt", None, b"null"), ("down", None, b"null")):
