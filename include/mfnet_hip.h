@@ -539,7 +539,7 @@ int64_t mfnet_layernorm_ckpt8_workspace_floats(int64_t rows, int64_t C);
  * Factors are bf16 images padded to RP = 16, 32 or 64 ranks: of each a "down" image of n * mfnet_lora_pool_image_elements(C, RP)
  * elements, in MFMA operand order (the product contracts over C), and an "up" image [n][C][RP] (it contracts over the ranks); pack
  * writes all four from A [n][r][K] and B [n][N][r], fp32 or bf16, and copies scale [n] (NULL: ones). K and N are
- * multiples of 8, rows 16-byte aligned with strides that are multiples of 8; M < 2^31 - 256, n <= 65535. No call synchronises,
+ * multiples of 8, rows 16-byte aligned with strides that are multiples of 8; M < 2^27, n <= 65535. No call synchronises,
  * allocates or uses atomics; the same inputs give the same bits. An adapter's or a row's infinities and NaN reach only the rows of that
  * adapter, or that row, and their gradients. */
 int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, const float* scale, int64_t n, int64_t K, int64_t N, int r, int RP,

@@ -417,7 +417,7 @@ static bool ck_geometry(CkGeom* g, dim3* grid, int64_t rows, int64_t C, int64_t 
   int64_t gy = ceil_div64(rows, 256 >> sh);
   if (gy > 65535) gy = 65535;
   *grid = dim3((unsigned)gx, (unsigned)gy);
-  return gx < (1ll << 31);
+  return gx < (1ll << 24);                                // (a grid dimension holds less than 2^32 threads)
 }
 
 #define CK_CHECK_SHAPE(name)                                                                                                         \
@@ -491,7 +491,7 @@ extern "C" int mfnet_layernorm_fwd_ckpt8(const void* x, int x_dtype, int64_t ldx
   MF_CHECK_ARG(((uintptr_t)gamma | (uintptr_t)beta) % 16 == 0 && (uintptr_t)x % (x_dtype == MFNET_F32 ? 16 : 8) == 0 && (uintptr_t)y % 8 == 0 && (uintptr_t)codes % 4 == 0,
                "layernorm_fwd_ckpt8: misaligned tensor");
   const int64_t gx = ceil_div64(rows, 4);
-  MF_CHECK_ARG(gx < (1ll << 31), "layernorm_fwd_ckpt8: too many rows");
+  MF_CHECK_ARG(gx < (1ll << 24), "layernorm_fwd_ckpt8: too many rows");
 #define LNF(T_, NV_) hipLaunchKernelGGL((ln_fwd_ckpt8_kernel<T_, NV_>), dim3((unsigned)gx), dim3(256), 0, stream, (const T_*)x, ldx, gamma, beta, (bf16_t*)y, mean, rstd, (signed char*)codes, (unsigned char*)exps, rows, (int)C, eps)
 #define LNF_CASE(NV_) case NV_: if (x_dtype == MFNET_F32) LNF(float, NV_); else LNF(bf16_t, NV_); break;
   switch ((int)ceil_div64(C, 256)) { LNF_CASE(1) LNF_CASE(2) LNF_CASE(3) LNF_CASE(4) LNF_CASE(5) LNF_CASE(6) LNF_CASE(7) LNF_CASE(8) }

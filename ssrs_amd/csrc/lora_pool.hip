@@ -92,34 +92,56 @@ __global__ __launch_bounds__(256) void pool_pack_kernel(const PoolPack p) {
 
 // ------------------------------------------------------------------------------------------------ rows grouped by adapter
 // Workgroup i: how many rows belong to adapters below i (their places come first), then the rows of adapter i in ascending order.
-// Deterministic without a sort; the indices are read from L2 twice per adapter.
-__global__ __launch_bounds__(256) void pool_plan_kernel(const int* __restrict__ ids, int M, int n, int* __restrict__ offs, int* __restrict__ perm) {
+// Deterministic without a sort; the indices are read from L2 twice per adapter, four per thread and step (32768 rows, 8 adapters: 17 us;
+// one per thread of 256: 96).
+__global__ __launch_bounds__(1024) void pool_plan_kernel(const int* __restrict__ ids, int M, int n, int* __restrict__ offs, int* __restrict__ perm) {
   const int i = blockIdx.x;                               // 0 .. n; workgroup n only writes offs[n]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  __shared__ int part[4];
+  __shared__ int part[2][16];
   int below = 0;
-  for (int m = threadIdx.x; m < M; m += 256) {
-    const int v = ids[m];
-    below += (v >= 0 && v < i) ? 1 : 0;
-  }
+  for (int m = threadIdx.x; m < M; m += 4096)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = m + 1024 * j, v = k < M ? ids[k] : -1;
+      below += (v >= 0 && v < i) ? 1 : 0;
+    }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) below += __shfl_xor(below, o, 64);
-  if (lane == 0) part[wave] = below;
+  if (lane == 0) part[0][wave] = below;
   __syncthreads();
-  int pos = part[0] + part[1] + part[2] + part[3];
+  int pos = 0;
+  for (int w = 0; w < 16; ++w) pos += part[0][w];
   if (threadIdx.x == 0) offs[i] = pos;
   if (i == n) return;
-  for (int m0 = 0; m0 < M; m0 += 256) {
-    const int m = m0 + threadIdx.x;
-    const bool mine = m < M && ids[m] == i;
-    const unsigned long long b = __ballot(mine);
+  __syncthreads();
+  for (int m0 = 0, step = 0; m0 < M; m0 += 4096, ++step) {
+    int mine[4], cnt = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {                         // four rows in a row: the order inside a thread is the rows' order
+      const int m = m0 + 4 * threadIdx.x + j;
+      mine[j] = m < M && ids[m] == i;
+      cnt += mine[j];
+    }
+    int scan = cnt;                                       // inclusive over the wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int q = __shfl_up(scan, o, 64);
+      if (lane >= o) scan += q;
+    }
+    int* pt = part[step & 1];
+    if (lane == 63) pt[wave] = scan;
     __syncthreads();
-    if (lane == 0) part[wave] = __popcll(b);
-    __syncthreads();
-    int at = pos;
-    for (int w = 0; w < wave; ++w) at += part[w];
-    if (mine) perm[at + __popcll(b & ((1ull << lane) - 1))] = m;
-    pos += part[0] + part[1] + part[2] + part[3];
+    int at = pos + scan - cnt, all = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      const int c = pt[w];
+      at += w < wave ? c : 0;
+      all += c;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (mine[j]) perm[at++] = m0 + 4 * threadIdx.x + j;
+    pos += all;
   }
 }
 // chunks of at most ch rows of one adapter: table[k] = {adapter, first, last + 1 place in perm, 0}, base[i] = first chunk of adapter i.
@@ -1029,6 +1051,7 @@ __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_ke
     mul(0, 0, G);
     read_x(1);
     mul(1, 0, G);
+    __syncthreads();                                         // (the epilogue writes to the same LDS)
   }
   const PoolPre<XF> none = {};
   pool_epilogue<XF, G, false>(p, acc, m0, wm * 16 * XF + fr, n0 + wn * 16 * G, fr, fq, lds + wave * 8192, none);
@@ -1195,7 +1218,8 @@ __global__ __launch_bounds__(256) void pool_sum_kernel(const PoolSum a, const Po
 
 // ------------------------------------------------------------------------------------------------ host
 static bool pool_rp(int RP) { return RP == 16 || RP == 32 || RP == 64; }
-static bool pool_counts(int64_t M, int64_t n) { return M >= 0 && M < (1ll << 31) - 256 && n >= 1 && n <= 65535; }
+// (a launch holds less than 2^32 threads: 2^27 rows keep every grid here below that)
+static bool pool_counts(int64_t M, int64_t n) { return M >= 0 && M < (1ll << 27) && n >= 1 && n <= 65535; }
 // a matrix whose rows are read in 16-byte pieces
 static bool pool_rows(const void* t, int64_t ld, int64_t C) { return C >= 8 && C % 8 == 0 && C < (1 << 24) && ld >= C && ld % 8 == 0 && (uintptr_t)t % 16 == 0; }
 #define POOL_CHECK_ROWS(name, T_, ld_, C_)                                                                                              \
@@ -1232,7 +1256,7 @@ extern "C" int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* o
   MF_CHECK_ARG(pool_counts(M, n), "lora_pool_plan: bad sizes (M=%lld n=%lld)", (long long)M, (long long)n);
   MF_CHECK_ARG(offs && base && (M == 0 || (ids && perm && table)), "lora_pool_plan: null pointer");
   MF_CHECK_ARG((uintptr_t)table % 16 == 0, "lora_pool_plan: table must be 16-byte aligned");
-  hipLaunchKernelGGL(pool_plan_kernel, dim3((unsigned)n + 1), dim3(256), 0, stream, ids, (int)M, (int)n, offs, perm);
+  hipLaunchKernelGGL(pool_plan_kernel, dim3((unsigned)n + 1), dim3(1024), 0, stream, ids, (int)M, (int)n, offs, perm);
   MF_LAUNCH_CHECK("lora_pool_plan");
   hipLaunchKernelGGL(pool_chunks_kernel, dim3((unsigned)n + 1), dim3(256), 0, stream, offs, (int)n, pool_chunk_rows(M), (int)mfnet_lora_pool_chunks(M, n), base, (int4*)table);
   MF_LAUNCH_CHECK("lora_pool_plan (chunks)");
@@ -1277,7 +1301,7 @@ static int pool_gemm(PoolGemm& p, hipStream_t stream) {
     if (p.ldx <= (1 << 22) && p.ldw <= (1 << 22))                         // (the phased kernel's 32-bit offsets)
       for (int i = 1; i < 4; ++i) best = cost[i] < cost[best] ? i : best;
     const int64_t nwg = best == 0 ? tiles(64, 64) : best == 1 ? tiles(128, 128) : best == 2 ? tiles(128, 192) : tiles(256, 256);
-    MF_CHECK_ARG(nwg < (1ll << 31), "lora_pool: too many tiles");
+    MF_CHECK_ARG(nwg < (1ll << 23), "lora_pool: too many tiles (%lld)", (long long)nwg);
     const dim3 grid((unsigned)nwg);
     if (best == 0 && split) hipLaunchKernelGGL((pool_gemm_kernel<2>), grid, dim3(512), 0, stream, p);
     else if (best == 0) hipLaunchKernelGGL((pool_gemm_kernel<1>), grid, dim3(256), 0, stream, p);
