@@ -33,11 +33,11 @@ BF = torch.bfloat16
 # frozen-weight caches (bf16 copies / transposes, resized tables); rebuilt when a parameter is
 # re-loaded (load_state_dict bumps _version) or moved (data_ptr changes)
 # ---------------------------------------------------------------------------------------------
-def _cached(key, params, build):
+def _cached(key, params, build, stamp=None):
     """Derived tensors live in a dict hung on the first source parameter (so they die with it and a
-    recycled id() can never alias another model's entry)."""
+    recycled id() can never alias another model's entry). stamp: one more thing that the entry goes stale with."""
     store = params[0].__dict__.setdefault("_mfnet_derived", {})
-    sig = tuple((p.data_ptr(), p._version, p.device) for p in params)
+    sig = (stamp,) + tuple((p.data_ptr(), p._version, p.device) for p in params)
     hit = store.get(key)
     if hit is not None and hit[0] == sig:
         return hit[1]
@@ -635,28 +635,43 @@ class PooledLinear(nn.Linear):
     def forward(self, x, ids, plan=None):
         if ops.FP32:
             raise NotImplementedError("lora.PooledLinear runs on the bf16 MFMA: it has no fp32 mode")
+        if x.dtype not in (torch.float32, BF):
+            raise ValueError(f"x {x.dtype}: float32 or bfloat16")
         rows = x.shape[:-1]
         if tuple(ids.shape) != tuple(rows):
             if ids.dim() != 1 or not rows or ids.shape[0] != rows[0]:
                 raise ValueError(f"ids {tuple(ids.shape)} for rows {tuple(rows)}: one index per row or per entry of the first dimension")
             ids = ids.view(-1, *[1] * (len(rows) - 1)).expand(rows)
-        return _PooledLinear.apply(x, self, ids.reshape(-1), plan, self.lora_A, self.lora_B)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, self.lora_A, self.lora_B)):
+            return _PooledLinear.apply(x, self, ids.reshape(-1), plan, self.lora_A, self.lora_B)
+        return self._product(x, ids.reshape(-1), False)[0].view(*rows, -1)
+
+    def _factors(self, train):
+        """the factors' images: kept while nothing writes to the factors; made anew (one launch) in a training step, whose optimizer
+        writes to them, and under graph capture, so that a replay reads the factors as they are then"""
+        make = lambda: ops.lora_pool(self.lora_A, self.lora_B, self.scaling)
+        if train or torch.cuda.is_current_stream_capturing():
+            return make()
+        return _cached(("pool",), (self.lora_A, self.lora_B, self.scaling), make, stamp=ops.WEIGHTS_EPOCH[0])
+
+    def _product(self, x, ids, train):
+        """-> (out of x's dtype, the bf16 rows, the factors' images, the down products (train))"""
+        x2 = x.reshape(-1, x.shape[-1])
+        xb = x2 if x2.dtype == BF else ops.cast(x2.contiguous().float(), BF)
+        pool = self._factors(train)
+        out = ops.lora_pool_fwd(xb, w_bf16(self.weight), self.bias, pool, ids, out_dtype=BF if x.dtype == BF else torch.float32, want_down=train)
+        out, down = out if train else (out, None)
+        return out, xb, pool, down
 
 
 @ops.keeps_precision
 class _PooledLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, lin, ids, plan, A, B):
-        x2 = x.reshape(-1, x.shape[-1])
-        xb = x2 if x2.dtype == BF else ops.cast(x2.contiguous().float(), BF)
-        pool = _cached(("pool",), (A, B, lin.scaling), lambda: ops.lora_pool(A, B, lin.scaling))
-        train = any(ctx.needs_input_grad)
-        out = ops.lora_pool_fwd(xb, w_bf16(lin.weight), lin.bias, pool, ids, out_dtype=BF if x.dtype == BF else torch.float32, want_down=train)
-        if train:
-            out, down = out
-            ctx.kept8 = tuple(xb.shape) if lin.checkpoint8 else None
-            ctx.save_for_backward(ops.ckpt8_pack(xb).buf if lin.checkpoint8 else xb, ids, down)
-            ctx.lin, ctx.pool, ctx.plan, ctx.shape, ctx.dtype = lin, pool, plan, x.shape, x.dtype
+        out, xb, pool, down = lin._product(x, ids, True)
+        ctx.kept8 = tuple(xb.shape) if lin.checkpoint8 else None
+        ctx.save_for_backward(ops.ckpt8_pack(xb).buf if lin.checkpoint8 else xb, ids, down)
+        ctx.lin, ctx.pool, ctx.plan, ctx.shape, ctx.dtype = lin, pool, plan, x.shape, x.dtype
         return out.view(*x.shape[:-1], -1)
 
     @staticmethod

@@ -72,6 +72,49 @@ def test_pooled_linear_refusals():
         lin(x, torch.zeros(4, dtype=torch.int32, device="cuda"))
 
 
+def test_pooled_linear_reads_factors_that_a_kernel_wrote():
+    """An update that torch does not see (.data: no version bump, as the engine's SGD kernel) reaches the next training call by itself, the
+    next serving call after bank.weights_changed(), and a captured call at every replay."""
+    from ssrs_amd import bank
+    from ssrs_amd.medsam.models.common import loralib as lora
+    g = torch.Generator().manual_seed(9)
+    lin = lora.PooledLinear(96, 72, 3, 5).cuda()
+    base = 0.3 * _rows(g, 3, 72, 5).cuda()
+    lin.lora_B.data.copy_(base)
+    x, ids = _rows(g, 40, 96).cuda(), torch.randint(0, 3, (40,), generator=g, dtype=torch.int32).cuda()
+
+    def serve():
+        with torch.no_grad():
+            return lin(x, ids)
+
+    def fresh(scale):
+        other = lora.PooledLinear(96, 72, 3, 5).cuda()
+        other.load_state_dict({**lin.state_dict(), "lora_B": scale * base})
+        with torch.no_grad():
+            return other(x, ids)
+
+    assert torch.equal(serve(), fresh(1)) and torch.equal(lin(x, ids), fresh(1))
+    lin.lora_B.data.mul_(2)
+    assert torch.equal(lin(x, ids), fresh(2))
+    bank.weights_changed()
+    assert torch.equal(serve(), fresh(2))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        serve()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = serve()
+    for k in (2, 4, 8):
+        lin.lora_B.data.copy_(k * base)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, fresh(k)), k
+    with pytest.raises(ValueError):
+        lin(x.half(), ids)
+
+
 def test_pool_of_fine_tuned_layers_serves_each_of_them():
     """three fine-tuned qkv layers over one frozen weight in one call: every model's rows get what that model's layer gives alone"""
     from ssrs_amd.medsam.models.common import loralib as lora
