@@ -266,9 +266,7 @@ __global__ __launch_bounds__(256) void ln_fwd_ckpt8_kernel(const T* __restrict__
 // Backward: 8 waves per workgroup, a wave strides over the rows; dgamma / dbeta stay in its registers, the waves' sums are added in
 // order through LDS and leave one slab [2][C] per workgroup, which the second kernel adds in order: no atomics, the same bits each run.
 #define LNB_WAVES 8
-#ifndef LNB_MAX_WG
 #define LNB_MAX_WG 512
-#endif
 template <typename T, int NV, bool WG>
 __global__ __launch_bounds__(64 * LNB_WAVES) void ln_bwd_ckpt8_kernel(const T* __restrict__ dy, int64_t lddy, const signed char* __restrict__ codes,
                                                                       const unsigned char* __restrict__ exps, const float* __restrict__ mean_in,
