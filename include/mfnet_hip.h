@@ -549,11 +549,13 @@ int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, const float* s
 int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* offs, int* perm, int* base, int* table, hipStream_t stream);
 int64_t mfnet_lora_pool_chunks(int64_t M, int64_t n);
 int64_t mfnet_lora_pool_image_elements(int64_t C, int RP);
-/* down [M, RP] fp32 = scale[i] * A_i x_m (zeros for rows without an adapter; the backward pass reads it),
+/* down [M, RP] fp32 = scale[i] * A_i x_m (zeros for rows without an adapter; the backward pass reads it), with workspace behind it:
+ * mfnet_lora_pool_down_floats(M, RP, out_dtype) floats in all;
  * out [M, N] bf16 | fp32 = x W^T (+ bias) + B_i down; X bf16 [M, K], W bf16 [N, K], bias fp32 [N] or NULL. */
 int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* scale, const void* a_down,
-                        const void* b_up, const int* ids, int64_t n, int RP, float* down, void* out, int out_dtype, int64_t ldo, int64_t M,
-                        int64_t N, int64_t K, hipStream_t stream);
+                        const void* b_up, const int* ids, int64_t n, int RP, float* down, int64_t down_floats, void* out, int out_dtype,
+                        int64_t ldo, int64_t M, int64_t N, int64_t K, hipStream_t stream);
+int64_t mfnet_lora_pool_down_floats(int64_t M, int RP, int out_dtype);
 /* With p_m = scale[i] * B_i^T dy_m: dx [M, K] bf16 = dy Wt^T + A_i^T p (Wt bf16 [K, N]; dx = NULL: left out), dA [n][r][K] = sum over the
  * adapter's rows of p x^T, dB [n][N][r] = sum of dy down^T, fp32, overwritten; adapters without rows get zeros. x is the forward's input
  * as bf16 rows (X) or its 8-bit checkpoint (codes, exps; dense), one of the two. */

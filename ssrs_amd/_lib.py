@@ -138,7 +138,7 @@ _SIGS = {
     # ---- pooled low-rank adapters (csrc/lora_pool.hip)
     "mfnet_lora_pool_pack": [P, P, I, P, I64, I64, I64, I, I, P, P, P, P, P, P],
     "mfnet_lora_pool_plan": [P, I64, I64, P, P, P, P, P],
-    "mfnet_lora_pool_fwd": [P, I64, P, I64, P, P, P, P, P, I64, I, P, P, I, I64, I64, I64, I64, P],
+    "mfnet_lora_pool_fwd": [P, I64, P, I64, P, P, P, P, P, I64, I, P, I64, P, I, I64, I64, I64, I64, P],
     "mfnet_lora_pool_bwd": [P, I64, P, I64, P, P, P, I64, P, P, P, P, P, P, P, P, I64, I, I, P, P, I64, P, P, P, I64, I64, I64, I64, P],
 }
 
@@ -147,6 +147,7 @@ _HELPERS = {
     "mfnet_layernorm_ckpt8_workspace_floats": (c_int64, [I64, I64]),
     "mfnet_lora_pool_chunks": (c_int64, [I64, I64]),
     "mfnet_lora_pool_image_elements": (c_int64, [I64, I]),
+    "mfnet_lora_pool_down_floats": (c_int64, [I64, I, I]),
     "mfnet_lora_pool_bwd_workspace_floats": (c_int64, [I64, I64, I64, I64, I]),
 }
 

@@ -202,9 +202,21 @@ __device__ __forceinline__ void pool_row_sums(const bf16_t* __restrict__ x, cons
 #pragma unroll
   for (int f = 0; f < NR; ++f) t[f] = (s[0][f] + s[1][f]) + (s[2][f] + s[3][f]);
 }
+// The result: fp32 [M, RP], and (P > 0) the same in P bf16 parts [M][P][RP], hi + lo (+ lo'), as the up product's MFMA reads them: split
+// once here, not by every wave that meets the row ([32768, 1280] x [1280, 5120]: 422 -> 397 us, [8192, 768] x [768, 2304]: 39 -> 36).
+struct PoolDown { float* out; bf16_t* parts; int P; };
+__device__ __forceinline__ void pool_store_down(const PoolDown& o, int64_t m, int RP, int j, float4 v) {      // ranks j .. j + 3 of row m
+  *reinterpret_cast<float4*>(o.out + m * RP + j) = v;
+  for (int q = 0; q < o.P; ++q) {
+    u32x2_t w;
+    w.x = pack_bf16x2(v.x, v.y); w.y = pack_bf16x2(v.z, v.w);
+    *reinterpret_cast<u32x2_t*>(o.parts + (m * o.P + q) * RP + j) = w;
+    v.x -= bf16_lo(w.x); v.y -= bf16_hi(w.x); v.z -= bf16_lo(w.y); v.w -= bf16_hi(w.y);
+  }
+}
 template <int NR>
 __device__ __forceinline__ void pool_down_row(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
-                                              const int* __restrict__ ids, int n, float* __restrict__ out, int64_t m, int K, int lane) {
+                                              const int* __restrict__ ids, int n, const PoolDown& out, int64_t m, int K, int lane) {
   const int id = ids[m];
   const bool on = (unsigned)id < (unsigned)n;
   f32x4_t t[NR];
@@ -218,7 +230,7 @@ __device__ __forceinline__ void pool_down_row(const bf16_t* __restrict__ X, int6
   }
   if ((lane & 15) == 0) {
 #pragma unroll
-    for (int f = 0; f < NR; ++f) *reinterpret_cast<float4*>(out + m * (16 * NR) + 16 * f + 4 * (lane >> 4)) = make_float4(t[f][0], t[f][1], t[f][2], t[f][3]);
+    for (int f = 0; f < NR; ++f) pool_store_down(out, m, 16 * NR, 16 * f + 4 * (lane >> 4), make_float4(t[f][0], t[f][1], t[f][2], t[f][3]));
   }
 }
 
@@ -233,7 +245,7 @@ __device__ __forceinline__ void pool_down_row(const bf16_t* __restrict__ X, int6
 template <int NR, int XR>      // NR = RP / 16
 __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
                                                         const int* __restrict__ ids, int n, const int* __restrict__ perm, const int* __restrict__ count,
-                                                        float* __restrict__ out, int64_t M, int K) {
+                                                        const PoolDown out, int64_t M, int K) {
   constexpr int RING = 3, XL = 2 * XR, FL = 2 * NR, PIECE = (XL + FL) * 1024;      // requests of 1 KB per piece: rows, factor
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4][RING][PIECE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -348,7 +360,7 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
       const f32x4_t t = (sel[b][f] + red[0][i][lane]) + (red[1][i][lane] + red[2][i][lane]);
       // (no adapter: zeros, whatever the sums hold)
       const float4 o = id[b] >= 0 ? make_float4(s * t[0], s * t[1], s * t[2], s * t[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
-      *reinterpret_cast<float4*>(out + mrow[b] * (16 * NR) + 16 * f + 4 * fq) = o;
+      pool_store_down(out, mrow[b], 16 * NR, 16 * f + 4 * fq, o);
     }
   }
 }
@@ -356,7 +368,7 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
 // Few rows: one row per workgroup, the four waves take every fourth k-step.
 template <int NR>
 __global__ __launch_bounds__(256) void pool_down_row_kernel(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
-                                                            const int* __restrict__ ids, int n, float* __restrict__ out, int K) {
+                                                            const int* __restrict__ ids, int n, const PoolDown out, int K) {
   __shared__ float red[4][16 * NR];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int fr = lane & 15, fq = lane >> 4;
@@ -393,13 +405,18 @@ __global__ __launch_bounds__(256) void pool_down_row_kernel(const bf16_t* __rest
   }
   __syncthreads();
   const int t = threadIdx.x;
-  if (t < 16 * NR) out[m * (16 * NR) + t] = on ? scale[id] * ((red[0][t] + red[1][t]) + (red[2][t] + red[3][t])) : 0.f;
+  if (t >= 4 * NR) return;
+  float v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = on ? scale[id] * ((red[0][4 * t + r] + red[1][4 * t + r]) + (red[2][4 * t + r] + red[3][4 * t + r])) : 0.f;
+  pool_store_down(out, m, 16 * NR, 4 * t, make_float4(v[0], v[1], v[2], v[3]));
 }
 
 // ------------------------------------------------------------------------------------------------ out = X W^T + bias + Up_i down
 struct PoolGemm {
   const bf16_t* X; int64_t ldx; const bf16_t* W; int64_t ldw; const float* bias;
-  const float* D; const bf16_t* Up; const int* ids; int n, RP;
+  const float* D; const bf16_t* U; int P;                   // the down products: fp32 (up to 64 rows), in P parts (more)
+  const bf16_t* Up; const int* ids; int n, RP;
   void* out; int64_t ldo; int out_f32;
   int64_t M; int N, K, tiles_m, tiles_n;
 };
@@ -420,10 +437,16 @@ template <int G> __device__ __forceinline__ int pool_swz_w(int o) {
 template <int G> __device__ __forceinline__ int pool_out_col(int fq, int i) { return pool_single<G>(i) ? 16 * i + 4 * fq : 32 * (i >> 1) + 8 * fq + 4 * (i & 1); }
 
 // Low-rank update, bias and store of a wave's tile: the lane owns rows m0 + r0 + 16 b and four columns per fragment (pool_out_col; rows past
-// the end repeat the last one and are not stored). The update is MFMA k-steps of 32 slots: RP = 16: ranks 0..15 of the factor's part hi,
-// then of its part lo; wider: 32 ranks of one part. A bf16 result needs 16 bits of the fp32 factor (hi + lo), an fp32 one a third part.
-// `pre`: indices and, at RP = 16, the factors, requested before the main loop where registers allow (PRE).
-template <int XF> struct PoolPre { int id[XF]; float4 d[XF][2]; };
+// the end repeat the last one and are not stored). The update is MFMA k-steps of 32 slots: RP = 16: ranks 0..15 of the down product's part
+// hi, then of its part lo; wider: 32 ranks of one part. A bf16 result needs 16 bits of the fp32 factor (hi + lo), an fp32 one a third part.
+// `pre`: indices and the first step's parts, requested before the main loop (PRE).
+template <int XF> struct PoolPre { int id[XF]; Frag u[XF]; };
+__device__ __forceinline__ int pool_part(const PoolGemm& p, int s, int fq) { return p.RP > 16 ? s % p.P : 2 * s + (fq >> 1); }      // of step s; >= P: none
+__device__ __forceinline__ int pool_rank(const PoolGemm& p, int s, int fq) { return p.RP > 16 ? 32 * (s / p.P) + 8 * fq : 8 * (fq & 1); }
+__device__ __forceinline__ u32x4_t pool_parts(const PoolGemm& p, int64_t m, int s, int fq) {
+  const int q = pool_part(p, s, fq);
+  return q < p.P ? *reinterpret_cast<const u32x4_t*>(p.U + (m * p.P + q) * p.RP + pool_rank(p, s, fq)) : (u32x4_t){0u, 0u, 0u, 0u};
+}
 template <int XF>
 __device__ __forceinline__ void pool_prefetch(const PoolGemm& p, PoolPre<XF>& pre, int64_t m0, int r0, int fq) {
   const int mlim = p.M - m0 - 1 < r0 + 16 * XF ? (int)(p.M - m0) - 1 : r0 + 16 * XF;
@@ -431,11 +454,7 @@ __device__ __forceinline__ void pool_prefetch(const PoolGemm& p, PoolPre<XF>& pr
   for (int b = 0; b < XF; ++b) {
     const int r = r0 + 16 * b < mlim ? r0 + 16 * b : mlim;
     pre.id[b] = p.ids[m0 + r];
-    if (p.RP == 16) {
-      const float4* d = reinterpret_cast<const float4*>(p.D + (m0 + r) * 16 + 8 * (fq & 1));
-      pre.d[b][0] = d[0];
-      pre.d[b][1] = d[1];
-    }
+    pre.u[b].q = pool_parts(p, m0 + r, 0, fq);
   }
 }
 template <int XF, int G, bool PRE>
@@ -444,7 +463,6 @@ __device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[
   {
     const int* ids = p.ids + m0;
     const int RP = p.RP;
-    const float* D = p.D + m0 * RP;
     int id[XF];
 #pragma unroll
     for (int b = 0; b < XF; ++b) {
@@ -452,26 +470,15 @@ __device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[
       id[b] = PRE ? pre.id[b] : ids[r < mlim ? r : mlim];
       if ((unsigned)id[b] >= (unsigned)p.n) id[b] = -1;
     }
-    const bool wide = RP > 16;
-    const int parts = p.out_f32 ? 3 : 2, steps = wide ? parts * (RP / 32) : parts - 1;
+    const int steps = RP > 16 ? p.P * (RP / 32) : p.P - 1;
     for (int s = 0; s < steps; ++s) {
-      const int rk = wide ? 32 * (s / parts) + 8 * fq : 8 * (fq & 1);
-      const int part = wide ? s % parts : 2 * s + (fq >> 1);               // 3: none
+      const int rk = pool_rank(p, s, fq);
       Frag u[XF];
 #pragma unroll
       for (int b = 0; b < XF; ++b) {
         const int r = r0 + 16 * b;
-        const float4* d = reinterpret_cast<const float4*>(D + ((r < mlim ? r : mlim) * RP + rk));
-        const bool have = PRE && !wide;
-        const float4 d0 = have ? pre.d[b][0] : d[0], d1 = have ? pre.d[b][1] : d[1];
-        const float x[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned int hi = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-          const float e0 = x[2 * i] - bf16_lo(hi), e1 = x[2 * i + 1] - bf16_hi(hi);
-          const unsigned int lo = pack_bf16x2(e0, e1), l2 = pack_bf16x2(e0 - bf16_lo(lo), e1 - bf16_hi(lo));
-          u[b].w[i] = part == 0 ? hi : (part == 1 ? lo : (part == 2 ? l2 : 0u));
-        }
+        if (PRE && s == 0) u[b] = pre.u[b];
+        else u[b].q = pool_parts(p, m0 + (r < mlim ? r : mlim), s, fq);
       }
       auto above = [&](int last) __attribute__((always_inline)) {
         int cand = NO_ID;
@@ -1264,7 +1271,7 @@ extern "C" int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* o
 }
 
 // perm / count: the rows that have an adapter, grouped by it (NULL: the rows as they come; every row of out is written)
-static int pool_down(const void* X, int64_t ldx, const void* image, const float* scale, const int* ids, int64_t n, int RP, const int* perm, const int* count, float* out, int64_t M,
+static int pool_down(const void* X, int64_t ldx, const void* image, const float* scale, const int* ids, int64_t n, int RP, const int* perm, const int* count, const PoolDown& out, int64_t M,
                      int64_t K, hipStream_t stream) {
   // Up to 256 rows: a workgroup per row is quicker than 16 rows and their adapters in turn. 32 rows per workgroup halve the factor's
   // traffic where there are enough of them to fill the chip.
@@ -1314,9 +1321,14 @@ static int pool_gemm(PoolGemm& p, hipStream_t stream) {
 }
 
 // down = scale_i image_i x, out = x W^T (+ bias) + up_i down
+// (down: M RP fp32 and behind them, above 64 rows, the parts)
 static int pool_products(PoolGemm& p, const void* image, const float* scale, const int* perm, const int* count, float* down, hipStream_t stream) {
+  p.D = down;
   if (p.M > 16 || p.RP > 32) {                              // (64 ranks: more registers than 16 waves have)
-    const int rc = pool_down(p.X, p.ldx, image, scale, p.ids, p.n, p.RP, perm, count, down, p.M, p.K, stream);
+    PoolDown d = {down, reinterpret_cast<bf16_t*>(down + p.M * p.RP), p.M > 64 ? p.out_f32 ? 3 : 2 : 0};
+    p.U = d.parts;
+    p.P = d.P;
+    const int rc = pool_down(p.X, p.ldx, image, scale, p.ids, p.n, p.RP, perm, count, d, p.M, p.K, stream);
     return rc ? rc : pool_gemm(p, stream);
   }
   const dim3 grid((unsigned)ceil_div64(p.N, 32));
@@ -1327,9 +1339,13 @@ static int pool_products(PoolGemm& p, const void* image, const float* scale, con
   return MFNET_OK;
 }
 
+// floats of mfnet_lora_pool_fwd's down: the product [M, RP] and workspace behind it (its parts)
+extern "C" int64_t mfnet_lora_pool_down_floats(int64_t M, int RP, int out_dtype) {
+  return M <= 0 ? 0 : M * RP + (M <= 64 ? 0 : M * RP * (out_dtype == MFNET_F32 ? 3 : 2) / 2);
+}
 extern "C" int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, int64_t ldw, const float* bias, const float* scale, const void* a_down,
-                                   const void* b_up, const int* ids, int64_t n, int RP, float* down, void* out, int out_dtype, int64_t ldo, int64_t M,
-                                   int64_t N, int64_t K, hipStream_t stream) {
+                                   const void* b_up, const int* ids, int64_t n, int RP, float* down, int64_t down_floats, void* out, int out_dtype,
+                                   int64_t ldo, int64_t M, int64_t N, int64_t K, hipStream_t stream) {
   MF_CHECK_ARG(pool_counts(M, n) && pool_rp(RP), "lora_pool_fwd: bad sizes (M=%lld n=%lld RP=%d)", (long long)M, (long long)n, RP);
   MF_CHECK_ARG(out_dtype == MFNET_BF16 || out_dtype == MFNET_F32, "lora_pool_fwd: bad out dtype");
   if (M == 0) return MFNET_OK;
@@ -1338,17 +1354,18 @@ extern "C" int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, in
   POOL_CHECK_ROWS("lora_pool_fwd (weight)", W, ldw, K);
   POOL_CHECK_ROWS("lora_pool_fwd (out)", out, ldo, N);
   MF_CHECK_ARG(((uintptr_t)bias | (uintptr_t)down | (uintptr_t)a_down | (uintptr_t)b_up) % 16 == 0, "lora_pool_fwd: misaligned tensor");
+  MF_CHECK_ARG(down_floats >= mfnet_lora_pool_down_floats(M, RP, out_dtype), "lora_pool_fwd: down holds too few floats (%lld)", (long long)down_floats);
   PoolGemm p;
   p.X = (const bf16_t*)X; p.ldx = ldx; p.W = (const bf16_t*)W; p.ldw = ldw; p.bias = bias;
-  p.D = down; p.Up = (const bf16_t*)b_up; p.ids = ids; p.n = (int)n; p.RP = RP;
+  p.Up = (const bf16_t*)b_up; p.ids = ids; p.n = (int)n; p.RP = RP;
   p.out = out; p.ldo = ldo; p.out_f32 = out_dtype == MFNET_F32;
   p.M = M; p.N = (int)N; p.K = (int)K;
   return pool_products(p, a_down, scale, nullptr, nullptr, down, stream);
 }
 
-// floats of workspace of mfnet_lora_pool_bwd: p [M, RP] and the partial sums of dA and dB
+// floats of workspace of mfnet_lora_pool_bwd: p [M, RP] and its parts, the partial sums of dA and dB
 extern "C" int64_t mfnet_lora_pool_bwd_workspace_floats(int64_t M, int64_t n, int64_t K, int64_t N, int RP) {
-  return M <= 0 ? 0 : M * RP + mfnet_lora_pool_chunks(M, n) * (K + N) * RP;
+  return M <= 0 ? 0 : mfnet_lora_pool_down_floats(M, RP, MFNET_BF16) + mfnet_lora_pool_chunks(M, n) * (K + N) * RP;
 }
 
 extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, int64_t ldx, const void* codes, const void* exps, const void* Wt, int64_t ldwt,
@@ -1359,7 +1376,7 @@ extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, 
   MF_CHECK_ARG(K >= 8 && K % 8 == 0 && K < (1 << 24) && N >= 8 && N % 8 == 0 && N < (1 << 24), "lora_pool_bwd: K=%lld and N=%lld must be multiples of 8", (long long)K, (long long)N);
   MF_CHECK_ARG(dA && dB && base, "lora_pool_bwd: null pointer");
   const int64_t chunks = mfnet_lora_pool_chunks(M, n);
-  float* part_a = ws + M * RP;
+  float* part_a = ws + mfnet_lora_pool_down_floats(M, RP, MFNET_BF16);
   float* part_b = part_a + chunks * K * RP;
   if (M > 0) {
     MF_CHECK_ARG(dy && scale && b_down && ids && offs && perm && table && down && ws && (!dx || (Wt && a_up)), "lora_pool_bwd: null pointer");
@@ -1372,11 +1389,11 @@ extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, 
     MF_CHECK_ARG(ws_floats >= mfnet_lora_pool_bwd_workspace_floats(M, n, K, N, RP), "lora_pool_bwd: workspace too small");
     MF_CHECK_ARG(chunks <= 65535, "lora_pool_bwd: too many chunks of rows (%lld)", (long long)chunks);
     int rc;
-    if (!dx) rc = pool_down(dy, lddy, b_down, scale, ids, n, RP, perm, offs + n, ws, M, N, stream);
+    if (!dx) rc = pool_down(dy, lddy, b_down, scale, ids, n, RP, perm, offs + n, PoolDown{ws, nullptr, 0}, M, N, stream);
     else {
       PoolGemm p;
       p.X = (const bf16_t*)dy; p.ldx = lddy; p.W = (const bf16_t*)Wt; p.ldw = ldwt; p.bias = nullptr;
-      p.D = ws; p.Up = (const bf16_t*)a_up; p.ids = ids; p.n = (int)n; p.RP = RP;
+      p.Up = (const bf16_t*)a_up; p.ids = ids; p.n = (int)n; p.RP = RP;
       p.out = dx; p.ldo = lddx; p.out_f32 = 0;
       p.M = M; p.N = (int)K; p.K = (int)N;
       rc = pool_products(p, b_down, scale, perm, offs + n, ws, stream);

@@ -1949,12 +1949,13 @@ def lora_pool_fwd(x, w, bias, pool: LoraPool, ids, out_dtype=torch.bfloat16, wan
     if bias is not None:
         _vec_f32(name, "bias", bias, N)
         bias = _aligned(bias)
-    down = x.new_empty((M, pool.RP), dtype=torch.float32)
+    nd = _lib.lib().mfnet_lora_pool_down_floats(M, pool.RP, od)
+    down = x.new_empty((nd,), dtype=torch.float32)                 # [M, RP], workspace behind it
     out = x.new_empty((M, N), dtype=out_dtype)
     _launch("mfnet_lora_pool_fwd", dev, 2 * (M * K + N * K + pool.n * pool.r * (K + N)) + M * N * (2 if od else 4), 2.0 * M * (N * K + pool.r * (N + K)),
-            x.data_ptr(), ldx, w.data_ptr(), ldw, _p(bias), pool.scale, pool.a_down, pool.b_up, ids.data_ptr(), pool.n, pool.RP, down.data_ptr(),
+            x.data_ptr(), ldx, w.data_ptr(), ldw, _p(bias), pool.scale, pool.a_down, pool.b_up, ids.data_ptr(), pool.n, pool.RP, down.data_ptr(), nd,
             out.data_ptr(), od, N, M, N, K)
-    return (out, down) if want_down else out
+    return (out, down[:M * pool.RP].view(M, pool.RP)) if want_down else out
 
 
 def lora_pool_bwd(dy, x, w_t, pool: LoraPool, plan: LoraPlan, down, want_dx=True):

@@ -36,9 +36,9 @@ def test_entry_points_refuse_bad_arguments_before_a_launch():
         assert L.mfnet_lora_pool_pack(*dict(pack, **{key: v}).values()) == -1 and msg in E(), key
     assert L.mfnet_lora_pool_plan(16, 1 << 27, 2, 16, 16, 16, 16, None) == -1 and b"sizes" in E()
     assert L.mfnet_lora_pool_plan(None, 8, 2, 16, 16, 16, 16, None) == -1 and b"null" in E()
-    fwd = dict(X=16, ldx=64, W=16, ldw=64, bias=None, scale=16, a_down=16, b_up=16, ids=16, n=2, RP=16, down=16, out=16, dt=1, ldo=64, M=8, N=64, K=64, s=None)
+    fwd = dict(X=16, ldx=64, W=16, ldw=64, bias=None, scale=16, a_down=16, b_up=16, ids=16, n=2, RP=16, down=16, nd=8 * 16, out=16, dt=1, ldo=64, M=8, N=64, K=64, s=None)
     for key, v, msg in (("ldx", 60, b"row stride"), ("K", 60, b"multiple of 8"), ("X", 24, b"16-byte"), ("W", None, b"null"), ("ldw", 56, b"weight"), ("ldo", 62, b"out"),
-                        ("RP", 17, b"sizes"), ("n", 0, b"sizes"), ("M", 1 << 27, b"sizes"), ("dt", 2, b"dtype"), ("down", None, b"null"), ("b_up", 24, b"misaligned"), ("ids", None, b"null")):
+                        ("nd", 8 * 16 - 1, b"too few"), ("RP", 17, b"sizes"), ("n", 0, b"sizes"), ("M", 1 << 27, b"sizes"), ("dt", 2, b"dtype"), ("down", None, b"null"), ("b_up", 24, b"misaligned"), ("ids", None, b"null")):
         assert L.mfnet_lora_pool_fwd(*dict(fwd, **{key: v}).values()) == -1 and msg in E(), key
     assert L.mfnet_lora_pool_fwd(*dict(fwd, M=0).values()) == 0
     bwd = dict(dy=16, lddy=64, X=16, ldx=64, codes=None, exps=None, Wt=16, ldwt=64, scale=16, b_down=16, a_up=16, ids=16, offs=16, perm=16, base=16, table=16, n=2, r=4, RP=16, down=16,
@@ -59,7 +59,15 @@ def test_sizes():
             one_each = min(n, M)
             worst = (one_each - 1) + -(-(M - one_each + 1) // ch)
             assert c >= worst
-            assert L.mfnet_lora_pool_bwd_workspace_floats(M, n, 64, 72, 32) == M * 32 + c * (64 + 72) * 32
+            assert L.mfnet_lora_pool_bwd_workspace_floats(M, n, 64, 72, 32) == L.mfnet_lora_pool_down_floats(M, 32, 1) + c * (64 + 72) * 32
+
+
+def test_room_behind_the_down_products():
+    L = _L()
+    for M in (0, 1, 64, 65, 5000):      # fp32 [M, RP]; above 64 rows two bf16 parts of it for a bf16 result, three for an fp32 one
+        for RP in (16, 64):
+            for dt, parts in ((1, 2), (0, 3)):
+                assert L.mfnet_lora_pool_down_floats(M, RP, dt) == M * RP + (M * RP * parts // 2 if M > 64 else 0)
 
 
 def test_wrappers_refuse_host_tensors():
