@@ -874,17 +874,20 @@ __global__ __launch_bounds__(256 * KS) void pool_gemm_kernel(const PoolGemm p) {
 // The same product for many rows: 8 waves as 2 (rows) x 4 (columns), wave tile 16 XF x 16 G, two k-tiles of 64 in LDS. A k-tile is
 // four phases, one quadrant of the wave's tile each (half the row fragments x half the column fragments x both k-steps):
 //
-//   phase 0  reads x-lo, w-lo     multiplies x-lo w-lo      requests x-hi of tile t + 1
-//   phase 1  reads w-hi           multiplies x-lo w-hi      requests x-lo of tile t + 2
-//   phase 2  reads x-hi           multiplies x-hi w-hi      requests half of W of tile t + 2
-//   phase 3                       multiplies x-hi w-lo      requests the rest of W of tile t + 2
+//   phase 0  reads the rest of x-lo                        multiplies x-lo w-lo      requests x-hi of tile t + 1
+//   phase 1  reads w-hi, a fragment of x-hi                multiplies x-lo w-hi      requests x-lo of tile t + 2
+//   phase 2  reads the rest of x-hi                        multiplies x-hi w-hi      requests half of W of tile t + 2
+//   phase 3  reads w-lo, a fragment of x-lo of tile t + 1  multiplies x-hi w-lo      requests the rest of W of tile t + 2
 //
 // Each phase is a read slot and a multiply slot with a barrier behind each; the waves of the second row half run one slot late, so
-// that on every SIMD one of its two waves multiplies while the other reads. A request overwrites only what both halves have read (waited
-// for by lgkmcnt(0) inside the read slot, published by its barrier) at least one slot earlier. vmcnt counts in order: at the end of
-// phase 3's read slot the requests younger than W of tile t + 1 may be in flight, at the end of phase 1's those younger than x-hi of
-// this tile. Addresses: a fragment's LDS address is one of four lane addresses plus a constant, a request's global one a constant
-// 32-bit offset beside a scalar that advances by 128 bytes a tile, so that the loop has next to no vector instructions beside the MFMAs.
+// that on every SIMD one of its two waves multiplies while the other reads. For that the slots have to be alike: 6 reads in each, where
+// x-lo and w-lo in phase 0 would be 12 of the 24 (with zeros as operands, which leave the clock alone, 3 to 7 % less time; with random
+// ones, where large products are held by the chip's power, 0 to 3 %: [32768, 3840] x [3840, 1280] 270 -> 265 us). The smaller tiles, two
+// workgroups per CU, read everything where it is multiplied first: two workgroups fill each other's gaps, and the early reads cost them
+// up to 6 %. A request overwrites only what both halves have read (waited for by lgkmcnt(0) inside the read slot, published by its
+// barrier) at least one slot earlier. vmcnt counts in order: each wait leaves the requests younger than the wanted ones. Addresses: a fragment's LDS address is one of four lane addresses plus a constant, a
+// request's global one a constant 32-bit offset beside a scalar that advances by 128 bytes a tile, so that the loop has next to no vector
+// instructions beside the MFMAs.
 template <int XF, int G>
 __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_kernel(const PoolGemm p) {
   constexpr int BM = 32 * XF, BN = 64 * G, STAGE = (BM + BN) * 128;
@@ -951,12 +954,15 @@ __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_ke
 #pragma unroll
     for (int b = 0; b < XF; ++b) acc[a][b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   bf16x8_t xf[XH][2], wf[G][2];
+  bf16x8_t xe[2], we[GL][2];                                 // read a phase early: the last fragment of x-lo or x-hi, w-lo
+  constexpr bool EARLY = XF * G >= 32;
   typedef const __attribute__((address_space(3))) bf16x8_t* frag_ptr_t;
-  auto read_x = [&](int h) __attribute__((always_inline)) {
+  auto read_x = [&](int h, int i1) __attribute__((always_inline)) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-      for (int i = 0; i < XH; ++i) xf[i][ks] = *(frag_ptr_t)(uintptr_t)(xa[ks] + (h * XH + i) * 2048);
+      for (int i = 0; i < XH; ++i)
+        if (i < i1) xf[i][ks] = *(frag_ptr_t)(uintptr_t)(xa[ks] + (h * XH + i) * 2048);
   };
   auto read_w = [&](int i0, int i1) __attribute__((always_inline)) {
 #pragma unroll
@@ -964,6 +970,21 @@ __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_ke
 #pragma unroll
       for (int i = 0; i < G; ++i)
         if (i >= i0 && i < i1) wf[i][ks] = *(frag_ptr_t)(uintptr_t)(pool_single<G>(i) ? wa1[ks] : wa[ks] + (i >> 1) * 4096 + (i & 1) * 512);
+  };
+  auto early_x = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) xe[ks] = *(frag_ptr_t)(uintptr_t)(xa[ks] + (h * XH + XH - 1) * 2048);
+  };
+  auto early_w = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < GL; ++i) we[i][ks] = *(frag_ptr_t)(uintptr_t)(wa[ks] + (i >> 1) * 4096 + (i & 1) * 512);
+  };
+  auto rest_x = [&](int h) __attribute__((always_inline)) {
+    read_x(h, XH - 1);
+    xf[XH - 1][0] = xe[0];
+    xf[XH - 1][1] = xe[1];
   };
   auto mul = [&](int h, int i0, int i1) __attribute__((always_inline)) {
     __builtin_amdgcn_s_setprio(1);
@@ -1001,45 +1022,56 @@ __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_ke
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   if (wm) __builtin_amdgcn_s_barrier();                      // the second row half runs one slot late
-  // MORE: two further tiles exist
+  auto flip = [&](unsigned int (&at)[2], int t) __attribute__((always_inline)) {      // to the other buffer
+    const unsigned int d = t & 1 ? (unsigned int)-STAGE : (unsigned int)STAGE;
+    at[0] += d;
+    at[1] += d;
+  };
+  // MORE: two further tiles exist. What the next phase reads has to have landed at a read slot's end: x-hi of this tile (before phase 1,
+  // or 2), x-lo and W of the next one (before phase 3, or 0).
   auto tile = [&](auto more, int t) __attribute__((always_inline)) {
     constexpr bool MORE = decltype(more)::value;
-    read_x(0);
-    read_w(0, GL);
-    if (MORE || t + 1 < nt) req_x(1, t + 1);
+    const bool next = MORE || t + 1 < nt;
+    if (!EARLY) { early_w(); early_x(0); }
+    rest_x(0);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int i = 0; i < GL; ++i) wf[i][ks] = we[i][ks];
+    if (next) req_x(1, t + 1);
+    if (EARLY && next) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * XP + WP) : "memory");
+    else if (EARLY) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     end_read();
     mul(0, 0, GL);
     end_mul();
     read_w(GL, G);
-    if (MORE) {
-      req_x(0, t + 2);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * XP + WP) : "memory");
-    } else if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (EARLY) early_x(1);
+    if (MORE) req_x(0, t + 2);
+    if (!EARLY && MORE) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * XP + WP) : "memory");
+    else if (!EARLY && next) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP) : "memory");
+    else if (!EARLY) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     end_read();
     mul(0, GL, G);
     end_mul();
-    read_x(1);
+    if (!EARLY) early_x(1);
+    rest_x(1);
     if (MORE) req_w(0, W0, t + 2);
+    if (EARLY) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MORE ? 2 * XP + W0 : XP) : "memory");
     end_read();
     mul(1, GL, G);
     end_mul();
-    if (MORE) {
-      req_w(W0, WP, t + 2);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * XP + WP) : "memory");
-    } else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XP) : "memory");
+    flip(xa, t); flip(wa, t); flip(wa1, t);
+    if (EARLY && next) { early_w(); early_x(0); }
+    if (MORE) req_w(W0, WP, t + 2);
+    if (!EARLY) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(MORE ? 2 * XP + WP : XP) : "memory");
     end_read();
     mul(1, 0, GL);
     end_mul();
   };
-  auto flip = [&](int t) __attribute__((always_inline)) {      // to the other buffer
-    const unsigned int d = t & 1 ? (unsigned int)-STAGE : (unsigned int)STAGE;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) { xa[ks] += d; wa[ks] += d; wa1[ks] += d; }
-  };
+  if (EARLY && nt > 0) { early_w(); early_x(0); }
   int t = 0;
-  for (; t + 2 < nt; ++t) { tile(std::true_type{}, t); flip(t); }
-  for (; t < nt; ++t) { tile(std::false_type{}, t); flip(t); }
+  for (; t + 2 < nt; ++t) tile(std::true_type{}, t);
+  for (; t < nt; ++t) tile(std::false_type{}, t);
   if (!wm) __builtin_amdgcn_s_barrier();
   if (ragged) {                                              // the columns behind the last whole k-tile; zeros behind column K on both sides
     __syncthreads();
@@ -1052,11 +1084,11 @@ __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_ke
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (nt & 1) flip(1);                                     // the chunks went to buffer 0
+    if (nt & 1) { flip(xa, 1); flip(wa, 1); flip(wa1, 1); }  // the chunks went to buffer 0
     read_w(0, G);
-    read_x(0);
+    read_x(0, XH);
     mul(0, 0, G);
-    read_x(1);
+    read_x(1, XH);
     mul(1, 0, G);
     __syncthreads();                                         // (the epilogue writes to the same LDS)
   }
