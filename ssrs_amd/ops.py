@@ -1854,9 +1854,25 @@ def layernorm_y_ckpt8(c: Ckpt8, mean, rstd, gamma, beta):
 # ------------------------------------------------------------------------------------------ pooled low-rank adapters
 class LoraPool:
     """n low-rank adapters of one layer, laid out for the kernels (lora_pool): bf16 images of A [n, r, K] and B [n, N, r] padded to
-    RP = 16, 32 or 64 ranks, one per direction of use, and
-    the scales. A copy: later changes of A, B and scale do not reach it."""
+    RP = 16, 32 or 64 ranks, one per direction of use, and the scales. A copy: later changes of A, B and scale do not reach it."""
     __slots__ = ("n", "r", "K", "N", "RP", "scale", "buf", "a_down", "a_up", "b_down", "b_up")
+
+    def _place(self):
+        """device addresses of the four images, every one a multiple of 16 bytes, and of the fp32 scales [n]"""
+        n, RP, K, N = self.n, self.RP, self.K, self.N
+        K64, N64 = (K + 63) // 64 * 64, (N + 63) // 64 * 64    # the down images end in zeros up to a multiple of 64 columns
+        self.a_down = self.buf.data_ptr()
+        self.a_up = self.a_down + 2 * n * RP * K64
+        self.b_down = self.a_up + 2 * n * RP * K
+        self.b_up = self.b_down + 2 * n * RP * N64
+        self.scale = self.b_up + 2 * n * RP * N
+
+    def __getstate__(self):                                    # (copied or stored: the addresses are the new buffer's)
+        return self.n, self.r, self.K, self.N, self.RP, self.buf
+
+    def __setstate__(self, state):
+        self.n, self.r, self.K, self.N, self.RP, self.buf = state
+        self._place()
 
 
 def lora_pool(A, B, scale=None) -> LoraPool:
@@ -1881,13 +1897,8 @@ def lora_pool(A, B, scale=None) -> LoraPool:
     A, B = A.detach().contiguous(), B.detach().contiguous()
     if scale is not None:
         _vec_f32(name, "scale", scale, n)
-    K64, N64 = (K + 63) // 64 * 64, (N + 63) // 64 * 64    # the down images end in zeros up to a multiple of 64 columns
-    p.buf = torch.empty(n * RP * (K64 + K + N64 + N) + 2 * n, dtype=torch.bfloat16, device=A.device)
-    p.a_down = p.buf.data_ptr()                           # device addresses of the four images: every one a multiple of 16 bytes
-    p.a_up = p.a_down + 2 * n * RP * K64
-    p.b_down = p.a_up + 2 * n * RP * K
-    p.b_up = p.b_down + 2 * n * RP * N64
-    p.scale = p.b_up + 2 * n * RP * N                     # fp32 [n]
+    p.buf = torch.empty(n * RP * ((K + 63) // 64 * 64 + K + (N + 63) // 64 * 64 + N) + 2 * n, dtype=torch.bfloat16, device=A.device)
+    p._place()
     _launch("mfnet_lora_pool_pack", dev, A.element_size() * n * r * (K + N) + 2 * p.buf.numel(), 0, A.data_ptr(), B.data_ptr(), dt, _p(scale), n, K, N, r, RP,
             p.a_down, p.a_up, p.b_down, p.b_up, p.scale)
     return p

@@ -245,3 +245,26 @@ def test_refusals():
                 lambda: b(t["dy"], o.ckpt8_pack(t["x"][:39]), t["w_t"], pool, plan, down), lambda: b(t["dy"].float(), t["x"], t["w_t"], pool, plan, down)):
         with pytest.raises(MfnetError):
             bad()
+
+
+def test_copied_and_stored_pools():
+    """a copy and a stored pool hold addresses of their own buffer, not of the one they were made from"""
+    import copy
+    import io
+    import pickle
+    from ssrs_amd import ops
+    g = torch.Generator().manual_seed(0)
+    A, B = torch.randn(3, 5, 72, generator=g).cuda(), torch.randn(3, 40, 5, generator=g).cuda()
+    x, w = torch.randn(33, 72, generator=g).bfloat16().cuda(), torch.randn(40, 72, generator=g).bfloat16().cuda()
+    ids = torch.randint(-1, 3, (33,), generator=g, dtype=torch.int32).cuda()
+    pool = ops.lora_pool(A, B, torch.tensor([0.5, 1.0, 2.0], device="cuda"))
+    want = ops.lora_pool_fwd(x, w, None, pool, ids)
+    stored = io.BytesIO()
+    torch.save(pool, stored)
+    stored.seek(0)
+    others = [copy.deepcopy(pool), pickle.loads(pickle.dumps(pool)), torch.load(stored, weights_only=False)]
+    for other in others:
+        assert other.a_down == other.buf.data_ptr() != pool.a_down and other.scale - other.a_down == pool.scale - pool.a_down
+    pool.buf.fill_(float("nan"))                                 # (nothing may read it any more)
+    for other in others:
+        assert torch.equal(ops.lora_pool_fwd(x, w, None, other, ids), want)
