@@ -170,11 +170,12 @@ def _attention_bwd(qkv, attn_mod, tb, o, dO, lse, G, Sh, Sw, heads, ws):
     return ops.attn_bwd(qkv, attn_mod.qkv.bias, tbl, tblT, o, dO, lse, G, Sh, Sw, heads, ws, Lh, Lw, hd ** -0.5)
 
 
-def _keeps8(blk, ctx):
+def _keeps8(blk, h, params):
     """activations of this branch kept in 8 bits until the backward pass: asked for (UNetFormer(checkpoints="int8")), a backward pass may
-    come, bf16 mode, and a row length the kernels take"""
-    C = blk.norm1.weight.shape[0]
-    return getattr(blk, "checkpoint8", False) and not ops.FP32 and any(ctx.needs_input_grad) and C % 32 == 0 and C <= 2048
+    come, bf16 mode, and a row length the kernels take (asked outside the Function: inside, gradients are always off)"""
+    C = h.shape[-1]
+    return (getattr(blk, "checkpoint8", False) and not ops.FP32 and torch.is_grad_enabled() and any(t.requires_grad for t in (h, *params)) and
+            C % 32 == 0 and C <= 2048)
 
 
 def _down8(ln, A_x, A_y, half, wx=None, wy=None):
@@ -191,7 +192,7 @@ class _LoraAttnBranch(torch.autograd.Function):
     """h -> h + proj(attn(qkv_lora(LN1(h))))  for the stacked token matrix (lora_block.py:64-82)."""
 
     @staticmethod
-    def forward(ctx, h, blk, geom, Ax, Ay, Bx, By):
+    def forward(ctx, h, blk, keep8, geom, Ax, Ay, Bx, By):
         B, Sh, Sw, heads, ws = geom
         attn = blk.attn
         D = h.shape[-1]
@@ -200,7 +201,7 @@ class _LoraAttnBranch(torch.autograd.Function):
         r = Ax.shape[0] // 2
         h2 = h.reshape(M, D)
         ck = None
-        if _keeps8(blk, ctx):                    # h in 8 bits beside its statistics instead of h and LN(h)
+        if keep8:                                # h in 8 bits beside its statistics instead of h and LN(h)
             ln, mean, rstd, ck = ops.layernorm_fwd_ckpt8(h2, blk.norm1.weight, blk.norm1.bias, blk.norm1.eps)
             a = _down8(ln, Ax, Ay, half)[0]
         elif 2 * r in (4, 8) and half % 2 == 0 and _ln_lora_fits(2 * r, D):      # LayerNorm and the down-projection a = LN(h) @ A_g^T in one launch
@@ -258,14 +259,14 @@ class _LoraAttnBranch(torch.autograd.Function):
             del ln
             ops.tn_flush()                       # a collected dA product would keep LN(h) in bf16 until the step's end
         if not ctx.needs_input_grad[0]:          # first block over a frozen patch embedding: nothing upstream wants dh
-            return (None, None, None) + grads
+            return (None, None, None, None) + grads
         dln = ops.gemm(dqkv, wT_bf16(attn.qkv.weight), U=da, V=_stack2("A", Ax, Ay, transpose=True), rows_per_group=half, n_groups=2)
         if ck is not None:
             dh, dh_bf = ops.layernorm_bwd_ckpt8(dln, ck, mean, rstd, blk.norm1.weight, dres=d2, want_bf16=True)
         else:
             dh, dh_bf = ops.layernorm_bwd(dln, h2, mean, rstd, blk.norm1.weight, dres=d2, want_bf16=True)
         ops.remember_bf16_twin(dh, dh_bf)
-        return (dh.view(dout.shape), None, None) + grads
+        return (dh.view(dout.shape), None, None, None) + grads
 
 
 def _mix_linear_fwd(x_bf, lin, half, act, residual, aU=None):
@@ -339,13 +340,13 @@ class _LoraMlpBranch(torch.autograd.Function):
     """h -> h + lin2(gelu(lin1(LN2(h))))  with the cross-modal LoRA mix (lora_block.py:83-85,104-108)."""
 
     @staticmethod
-    def forward(ctx, h, blk, *params):
+    def forward(ctx, h, blk, keep8, *params):
         D = h.shape[-1]
         M = h.numel() // D
         half = M // 2
         h2 = h.reshape(M, D)
         l1 = blk.mlp.lin1
-        if _keeps8(blk, ctx):                    # kept in 8 bits: h (with its statistics) and lin1's output; not LN(h), not GELU(lin1)
+        if keep8:                                # kept in 8 bits: h (with its statistics) and lin1's output; not LN(h), not GELU(lin1)
             l2 = blk.mlp.lin2
             ln, mean, rstd, ck = ops.layernorm_fwd_ckpt8(h2, blk.norm2.weight, blk.norm2.bias, blk.norm2.eps)
             s1 = _down8(ln, l1.lora_Ax, l1.lora_Ay, half, l1.lora_wx.detach(), l1.lora_wy.detach())
@@ -383,7 +384,7 @@ class _LoraMlpBranch(torch.autograd.Function):
         dln, g1 = _mix_linear_bwd(dpre, ln, blk.mlp.lin1, (a1, U1), half)
         dh, dh_bf = ops.layernorm_bwd(dln, h2, mean, rstd, blk.norm2.weight, dres=d2, want_bf16=True)
         ops.remember_bf16_twin(dh, dh_bf)
-        return (dh.view(dout.shape), None) + deliver(blk._mlp_params(), g1 + g2)     # order of LoraBlock._mlp_params()
+        return (dh.view(dout.shape), None, None) + deliver(blk._mlp_params(), g1 + g2)     # order of LoraBlock._mlp_params()
 
     @staticmethod
     def backward8(blk, ck, mean, rstd, ckp, s1, s2, dout):
@@ -402,7 +403,7 @@ class _LoraMlpBranch(torch.autograd.Function):
         dh = kept["dh"]
         ops.remember_bf16_twin(dh, dh_bf)
         ops.tn_flush()                           # the collected dA products would keep GELU(lin1) and LN(h) in bf16 until the step's end
-        return (dh.view(dout.shape), None) + deliver(blk._mlp_params(), g1 + g2)
+        return (dh.view(dout.shape), None, None) + deliver(blk._mlp_params(), g1 + g2)
 
 
 @ops.keeps_precision
@@ -642,6 +643,8 @@ class PooledLinear(nn.Linear):
             if ids.dim() != 1 or not rows or ids.shape[0] != rows[0]:
                 raise ValueError(f"ids {tuple(ids.shape)} for rows {tuple(rows)}: one index per row or per entry of the first dimension")
             ids = ids.view(-1, *[1] * (len(rows) - 1)).expand(rows)
+        if plan is not None and (plan.M != ids.numel() or plan.n != self.n_adapters):
+            raise ValueError(f"the plan is of {plan.M} rows and {plan.n} adapters, not of {ids.numel()} and {self.n_adapters}")
         if torch.is_grad_enabled() and any(t.requires_grad for t in (x, self.lora_A, self.lora_B)):
             return _PooledLinear.apply(x, self, ids.reshape(-1), plan, self.lora_A, self.lora_B)
         return self._product(x, ids.reshape(-1), False)[0].view(*rows, -1)
@@ -810,9 +813,10 @@ class LoraBlock(nn.Module):
 
     def forward_stacked(self, h: torch.Tensor) -> torch.Tensor:
         q = self.attn.qkv
-        h = _LoraAttnBranch.apply(h, self, _geom(h, self.num_heads, self.window_size),
-                                  q.lora_Ax, q.lora_Ay, q.lora_Bx, q.lora_By)
-        return _LoraMlpBranch.apply(h, self, *self._mlp_params())
+        factors = (q.lora_Ax, q.lora_Ay, q.lora_Bx, q.lora_By)
+        h = _LoraAttnBranch.apply(h, self, _keeps8(self, h, factors), _geom(h, self.num_heads, self.window_size), *factors)
+        factors = self._mlp_params()
+        return _LoraMlpBranch.apply(h, self, _keeps8(self, h, factors), *factors)
 
     def forward(self, x: torch.Tensor, y: torch.Tensor):
         h = self.forward_stacked(torch.stack([x, y]).float().contiguous())

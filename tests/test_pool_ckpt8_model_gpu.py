@@ -64,6 +64,9 @@ def test_pooled_linear_refusals():
             bad()
     lin = lora.PooledLinear(96, 72, 2, 4).cuda()
     x = torch.randn(4, 9, 96, device="cuda")
+    for rows, n in ((35, 2), (36, 3)):
+        with pytest.raises(ValueError, match="plan"):
+            lin(x, torch.zeros(4, dtype=torch.int32, device="cuda"), plan=ops.lora_pool_plan(torch.zeros(rows, dtype=torch.int32, device="cuda"), n))
     with pytest.raises(ValueError):
         lin(x, torch.zeros(9, dtype=torch.int32, device="cuda"))
     with pytest.raises(ops.MfnetError):
@@ -241,10 +244,35 @@ def test_block_with_8bit_checkpoints(mid_dim, ws):
         assert rel_l2(res[True][1][k], want) < 2 * KEPT + 4 * 2 ** -8, k
 
 
+def test_block_without_a_backward_pass_keeps_nothing(monkeypatch):
+    """under no_grad (whatever the parameters ask for), and with nothing to train: the usual forward, no checkpoint is made"""
+    from ssrs_amd import ops
+    from ssrs_amd.vit import LoraBlock
+    blk = LoraBlock(args=_args(None), dim=128, num_heads=2, mlp_ratio=4.0, norm_layer=functools.partial(nn.LayerNorm, eps=1e-6), use_rel_pos=True,
+                    window_size=0, input_size=(16, 16))
+    blk.load_state_dict(detfill.fill_state_dict(blk.state_dict(), "k8n/"))
+    blk = blk.cuda()
+    h = _rows(torch.Generator().manual_seed(1), 2, 2, 16, 16, 128).cuda()
+    with torch.no_grad():
+        want = blk.forward_stacked(h)
+    blk.checkpoint8 = True
+    made = []
+    for name in ("layernorm_fwd_ckpt8", "gelu_fwd_ckpt8", "ckpt8_pack"):
+        monkeypatch.setattr(ops, name, lambda *a, _f=getattr(ops, name), **k: (made.append(1), _f(*a, **k))[1])
+    with torch.no_grad():
+        assert torch.equal(blk.forward_stacked(h), want)
+    for p in blk.parameters():
+        p.requires_grad = False
+    assert torch.equal(blk.forward_stacked(h), want) and not made
+    blk.forward_stacked(h.requires_grad_())
+    assert len(made) == 3
+
+
 @pytest.mark.parametrize("use_graph", [False, True])
 def test_train_step_with_8bit_checkpoints(use_graph):
     """the whole step of the tiny model: loss of the first step as with bf16 checkpoints, gradients within the kept activations' share
-    (two blocks, two branches each), the loss falls over the updates of one batch as it does with bf16 checkpoints"""
+    (two blocks, two branches each), and the same gradients in every step, eager or replayed, while the learning rate is zero (up to
+    sums by float atomics, which may turn single bf16 roundings)"""
     from ssrs_amd.trainer import TrainEngine
     from ssrs_amd.unetformer_mmsam import UNetFormer
     rgb, dsm, tgt = (t.cuda() for t in detfill.tiles("k8t", 2, 256, 6))
@@ -257,16 +285,16 @@ def test_train_step_with_8bit_checkpoints(use_graph):
         m = m.cuda().eval()
         m.decoder.segmentation_head[1].p = 0.0
         assert m.checkpoints == kind and all(b.checkpoint8 == (kind == "int8") for b in m.image_encoder.blocks)
-        eng = TrainEngine(m, lr=0.01, momentum=0.9, weight_decay=5e-4, class_weight=torch.ones(6, device="cuda"), use_graph=use_graph)
+        eng = TrainEngine(m, lr=0.0, momentum=0.9, weight_decay=5e-4, class_weight=torch.ones(6, device="cuda"), use_graph=use_graph)
         ls = []
         for i in range(4):                   # (graph mode: two eager steps, then capture and replays)
             ls.append(TrainEngine.read_metrics(eng.step(rgb, dsm, tgt))["loss"])
             if i == 0:
                 grads[kind] = eng.flat_g.clone()
+            assert rel_l2(eng.flat_g, grads[kind]) < 2 ** -8, (kind, i)
         losses[kind] = ls
     assert abs(losses["int8"][0] - losses["bf16"][0]) < 5e-3 * abs(losses["bf16"][0])
     assert rel_l2(grads["int8"], grads["bf16"]) < 4 * KEPT
-    assert losses["int8"][3] < losses["int8"][0] and losses["bf16"][3] < losses["bf16"][0]
 
 
 def test_checkpoints_option_refusals():
