@@ -269,3 +269,35 @@ def test_refusals():
                 lambda: o.layernorm_bwd_ckpt8(x, c, m, m, v, want_f32=False), lambda: o.layernorm_bwd_ckpt8(x, c, m, m, v, dres=x.double())):
         with pytest.raises(MfnetError):
             bad()
+
+
+def test_offsets_past_32_bits():
+    """more elements than 2^31, as one dense tensor and as far-apart rows: the same as the rows by themselves"""
+    from ssrs_amd import ops
+    rows, C = 1100000, 2048
+    x = torch.empty(rows, C, device="cuda", dtype=torch.bfloat16)
+    x.view(-1)[:1 << 22].normal_()
+    x[2048:] = x[:2048].repeat(rows // 2048 + 1, 1)[:rows - 2048]
+    x[-70:] = torch.randn(70, C, device="cuda", dtype=torch.bfloat16)
+    g, b = torch.rand(C, device="cuda") + 0.5, torch.randn(C, device="cuda")
+    tail = x[-100:].contiguous()
+    c, ct = ops.ckpt8_pack(x), ops.ckpt8_pack(tail)
+    assert torch.equal(c.codes[-100:], ct.codes) and torch.equal(c.exps[-100:], ct.exps)
+    assert torch.equal(ops.ckpt8_unpack(c)[-100:], ops.ckpt8_unpack(ct))
+    act, cg = ops.gelu_fwd_ckpt8(x)
+    act_t, cgt = ops.gelu_fwd_ckpt8(tail)
+    assert torch.equal(act[-100:], act_t) and torch.equal(cg.codes[-100:], ct.codes)
+    assert torch.equal(ops.gelu_bwd_ckpt8(cg, x)[-100:], ops.gelu_bwd_ckpt8(cgt, tail))
+    del act, cg
+    y, mean, rstd, cl = ops.layernorm_fwd_ckpt8(x, g, b, 1e-6)
+    yt, mt, rt, clt = ops.layernorm_fwd_ckpt8(tail, g, b, 1e-6)
+    assert torch.equal(y[-100:], yt) and torch.equal(mean[-100:], mt) and torch.equal(cl.codes[-100:], clt.codes)
+    dx = ops.layernorm_bwd_ckpt8(y, cl, mean, rstd, g, want_f32=False, want_bf16=True)
+    assert torch.equal(dx[-100:], ops.layernorm_bwd_ckpt8(yt, clt, mt, rt, g, want_f32=False, want_bf16=True))
+    del x, y, dx, cl, c
+    far = torch.empty(40000, 65541, device="cuda", dtype=torch.bfloat16)      # (rows at odd addresses: an element per lane)
+    for width in (96, 77):
+        v = far[:, 5:5 + width]
+        v.copy_(torch.randn(40000, width, device="cuda"))
+        a, b = ops.ckpt8_pack(v), ops.ckpt8_pack(v.contiguous())
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.exps, b.exps)

@@ -268,3 +268,39 @@ def test_copied_and_stored_pools():
     pool.buf.fill_(float("nan"))                                 # (nothing may read it any more)
     for other in others:
         assert torch.equal(ops.lora_pool_fwd(x, w, None, other, ids), want)
+
+
+def test_offsets_past_32_bits():
+    """rows whose byte or element offsets pass 32 bits: far-apart rows of x, dy and w, and more output elements than 2^31"""
+    o = ops()
+    t = make(40000, 64, 72, 3, 8, "mixed", seed=2)
+    far = torch.empty(40000, 65544, device="cuda", dtype=torch.bfloat16)
+    x, dy = far[:, 8:72], far[:, 128:200]
+    x.copy_(t["x"])
+    dy.copy_(t["dy"])
+    w = torch.empty(72, (1 << 22) + 8, device="cuda", dtype=torch.bfloat16)[:, :64]
+    w.copy_(t["w"])
+    pool, plan = o.lora_pool(t["A"], t["B"], t["scale"]), o.lora_pool_plan(t["ids"], 3)
+
+    def run(x, w, dy):
+        out, down = o.lora_pool_fwd(x, w, t["bias"], pool, t["ids"], want_down=True)
+        return (out, down) + o.lora_pool_bwd(dy, x, t["w_t"], pool, plan, down)
+    ref, tol = formulas(t)
+    for got in (run(x, t["w"], dy), run(x, w, dy)):
+        assert close(got[0], ref[0], tol[0], HALF_BF16) and close(got[2], ref[1], tol[1], HALF_BF16) and close(got[3], ref[2], tol[2]) and close(got[4], ref[3], tol[3])
+    del far, x, dy, w
+    t = make(3000, 1280, 5120, 3, 8, "mixed", seed=4)            # the largest tile, rows as far apart as it takes and a little further
+    pool = o.lora_pool(t["A"], t["B"], t["scale"])
+    ref, tol = formulas(t)
+    for ld in (1 << 22, (1 << 22) + 8):
+        x = torch.empty(3000, ld, device="cuda", dtype=torch.bfloat16)[:, -1280:]
+        x.copy_(t["x"])
+        assert close(o.lora_pool_fwd(x, t["w"], t["bias"], pool, t["ids"]), ref[0], tol[0], HALF_BF16), ld
+        del x
+    M, N = 300000, 8192
+    t = make(M, 64, N, 2, 4, "mixed", seed=3)
+    out = o.lora_pool_fwd(t["x"], t["w"], t["bias"], o.lora_pool(t["A"], t["B"], t["scale"]), t["ids"])
+    for rows in (slice(0, 64), slice(M - 100, M)):
+        part = {k: (v[rows] if k in ("x", "dy", "ids") else v) for k, v in t.items()}
+        ref, tol = formulas(part)
+        assert close(out[rows], ref[0], tol[0], HALF_BF16), rows
