@@ -513,7 +513,8 @@ int mfnet_adapter_mix_bwd_f32(const float* dh, const float* ada, const float* wx
  * [rows, ceil(C / 32)]. With amax the block's largest magnitude, e is the smallest integer in [-126, 121] with amax <= 127 * 2^e (121 if
  * none), code = rint(x * 2^-e) clamped to +-127, the byte is e + 127; byte 255 marks a block that holds an infinity or NaN, all of whose
  * elements stand for NaN. code * 2^e is exact in bf16. Any C >= 1 and any row stride >= C; rows whose C, strides and addresses allow
- * 16-byte accesses (C % 8 == 0) take the fast kernels. codes / exps are dense. rows = 0 is allowed everywhere (nothing is launched). */
+ * 16-byte accesses (C % 8 == 0) take the fast kernels. codes / exps are dense. rows = 0 is allowed everywhere (nothing is launched). No output may
+ * overlap an input. */
 int mfnet_ckpt8_pack(const void* x, int x_dtype, int64_t ldx, void* codes, void* exps, int64_t rows, int64_t C, hipStream_t stream);
 int mfnet_ckpt8_unpack(const void* codes, const void* exps, void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t C, hipStream_t stream);
 /* act = GELU(x) (erf form, nn.GELU) and the checkpoint of x; x and act of one dtype. */
@@ -541,7 +542,7 @@ int64_t mfnet_layernorm_ckpt8_workspace_floats(int64_t rows, int64_t C);
  * writes all four from A [n][r][K] and B [n][N][r], fp32 or bf16, and copies scale [n] (NULL: ones). K and N are
  * multiples of 8, rows 16-byte aligned with strides that are multiples of 8; M < 2^27, n <= 65535. No call synchronises,
  * allocates or uses atomics; the same inputs give the same bits. An adapter's or a row's infinities and NaN reach only the rows of that
- * adapter, or that row, and their gradients. */
+ * adapter, or that row, and their gradients. No output or workspace may overlap an input. */
 int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, const float* scale, int64_t n, int64_t K, int64_t N, int r, int RP,
                          void* a_down, void* a_up, void* b_down, void* b_up, float* scale_out, hipStream_t stream);
 /* Rows grouped by adapter, ascending inside each: offs [n + 1], perm [M], and chunks of rows for the backward sums: base [n + 1], table
@@ -558,7 +559,7 @@ int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, int64_t ldw, 
 int64_t mfnet_lora_pool_down_floats(int64_t M, int RP, int out_dtype);
 /* With p_m = scale[i] * B_i^T dy_m: dx [M, K] bf16 = dy Wt^T + A_i^T p (Wt bf16 [K, N]; dx = NULL: left out), dA [n][r][K] = sum over the
  * adapter's rows of p x^T, dB [n][N][r] = sum of dy down^T, fp32, overwritten; adapters without rows get zeros. x is the forward's input
- * as bf16 rows (X) or its 8-bit checkpoint (codes, exps; dense), one of the two. */
+ * as bf16 rows (X) or its 8-bit checkpoint (codes, exps; dense), one of the two. mfnet_lora_pool_chunks(M, n) <= 65535. */
 int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, int64_t ldx, const void* codes, const void* exps, const void* Wt, int64_t ldwt,
                         const float* scale, const void* b_down, const void* a_up, const int* ids, const int* offs, const int* perm,
                         const int* base, const int* table, int64_t n, int r, int RP, const float* down, void* dx, int64_t lddx, float* dA, float* dB, float* ws,

@@ -645,6 +645,8 @@ class PooledLinear(nn.Linear):
             ids = ids.view(-1, *[1] * (len(rows) - 1)).expand(rows)
         if plan is not None and (plan.M != ids.numel() or plan.n != self.n_adapters):
             raise ValueError(f"the plan is of {plan.M} rows and {plan.n} adapters, not of {ids.numel()} and {self.n_adapters}")
+        if torch.is_grad_enabled() and (self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad)):
+            raise NotImplementedError("the shared projection of a lora.PooledLinear is frozen: its weight and bias get no gradients")
         if torch.is_grad_enabled() and any(t.requires_grad for t in (x, self.lora_A, self.lora_B)):
             return _PooledLinear.apply(x, self, ids.reshape(-1), plan, self.lora_A, self.lora_B)
         return self._product(x, ids.reshape(-1), False)[0].view(*rows, -1)

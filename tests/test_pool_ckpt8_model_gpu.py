@@ -73,6 +73,11 @@ def test_pooled_linear_refusals():
         lin(x, torch.zeros(4, dtype=torch.int64, device="cuda"))
     with ops.precision("fp32"), pytest.raises(NotImplementedError):
         lin(x, torch.zeros(4, dtype=torch.int32, device="cuda"))
+    for p in (lin.weight, lin.bias):
+        p.requires_grad = True
+        with pytest.raises(NotImplementedError, match="frozen"):
+            lin(x, torch.zeros(4, dtype=torch.int32, device="cuda"))
+        p.requires_grad = False
 
 
 def test_pooled_linear_reads_factors_that_a_kernel_wrote():
@@ -116,6 +121,44 @@ def test_pooled_linear_reads_factors_that_a_kernel_wrote():
         assert torch.equal(out, fresh(k)), k
     with pytest.raises(ValueError):
         lin(x.half(), ids)
+
+
+@pytest.mark.parametrize("ck", [False, True])
+def test_pooled_linear_step_in_a_graph(ck):
+    """forward and backward captured, replayed on new rows, indices and factors between eager steps of another module"""
+    from ssrs_amd.medsam.models.common import loralib as lora
+    g = torch.Generator().manual_seed(11)
+    lin, ref = (lora.PooledLinear(96, 72, 3, 5, checkpoint8=ck).cuda() for _ in range(2))
+    ref.load_state_dict(lin.state_dict())
+    x, dy = torch.zeros(130, 96, device="cuda", requires_grad=True), torch.zeros(130, 72, device="cuda")
+    ids = torch.zeros(130, dtype=torch.int32, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):                                   # (warm-up; nothing of it may live while the leaves are captured)
+        lin(x, ids).backward(dy)
+    torch.cuda.current_stream().wait_stream(s)
+    x.grad = None
+    lin.zero_grad(set_to_none=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lin(x, ids)
+        out.backward(dy)
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(_rows(g, 130, 96))
+            dy.copy_(_rows(g, 130, 72))
+            ids.copy_(torch.randint(-1, 3, (130,), generator=g, dtype=torch.int32))
+            for p, q in ((lin.lora_A, ref.lora_A), (lin.lora_B, ref.lora_B)):
+                p.copy_(0.2 * _rows(g, *p.shape))
+                q.copy_(p)
+        graph.replay()
+        torch.cuda.synchronize()
+        xr = x.detach().clone().requires_grad_()
+        ref.zero_grad(set_to_none=True)
+        want = ref(xr, ids)
+        want.backward(dy)
+        assert torch.equal(out, want) and torch.equal(x.grad, xr.grad), k
+        assert torch.equal(lin.lora_A.grad, ref.lora_A.grad) and torch.equal(lin.lora_B.grad, ref.lora_B.grad), k
 
 
 def test_pool_of_fine_tuned_layers_serves_each_of_them():
