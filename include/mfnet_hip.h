@@ -528,7 +528,7 @@ int mfnet_layernorm_fwd_ckpt8(const void* x, int x_dtype, int64_t ldx, const flo
                               float* rstd, void* codes, void* exps, int64_t rows, int64_t C, float eps, hipStream_t stream);
 /* With xh = (x8 - mean) rstd and t = dy gamma: dx = rstd (t - mean(t) - xh mean(t xh)) (+ dres), written as fp32 (dx) and / or bf16
  * (dx_bf16), all dense [rows, C]; y (optional, needs beta) = bf16(xh gamma + beta), the LayerNorm output again; dgamma = sum dy xh and
- * dbeta = sum dy (both or neither; overwritten; ws of mfnet_layernorm_ckpt8_workspace_floats). Deterministic: no atomics. dy = NULL with
+ * dbeta = sum dy (both or neither; overwritten; ws of mfnet_layernorm_ckpt8_workspace_floats, none up to 2048 rows). Deterministic: no atomics. dy = NULL with
  * neither dx: y alone. */
 int mfnet_layernorm_bwd_ckpt8(const void* dy, int dy_dtype, int64_t lddy, const void* codes, const void* exps, const float* mean,
                               const float* rstd, const float* gamma, const float* beta, const float* dres, float* dx, void* dx_bf16, void* y,

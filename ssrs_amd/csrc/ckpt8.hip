@@ -267,14 +267,54 @@ __global__ __launch_bounds__(256) void ln_fwd_ckpt8_kernel(const T* __restrict__
 // order through LDS and leave one slab [2][C] per workgroup, which the second kernel adds in order: no atomics, the same bits each run.
 #define LNB_WAVES 8
 #define LNB_MAX_WG 512
+#define LNB_FEW 2048
+// Few rows: dgamma and dbeta of 32 columns (a block of the checkpoint) by one workgroup more per block in the same launch, which reads
+// dy and the codes of all rows again: 64 groups of rows, added in order. [512, 768]: 8.9 us with slabs and a second launch, 4.4 so (18.3
+// and 13.7 issued one by one); [2048, 1280] 14.0 and 12.3; [4096, 768] 17.4 and 20.4, where re-reading costs more than the launch.
+template <typename T>
+__device__ __forceinline__ void ln_bwd_ckpt8_columns(const T* __restrict__ dy, int64_t lddy, const signed char* __restrict__ codes, const unsigned char* __restrict__ exps,
+                                                     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, float* __restrict__ dgamma,
+                                                     float* __restrict__ dbeta, int rows, int C, int block) {
+  __shared__ float part[2][64][33];
+  const int l = threadIdx.x & 7, k = threadIdx.x >> 3, c = 32 * block + 4 * l;
+  float dg[4] = {0.f, 0.f, 0.f, 0.f}, db[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int row = k; row < rows; row += 64) {
+    Raw4<T> q;
+    q.load(dy + (int64_t)row * lddy + c);
+    const float4 d = q.value();
+    const unsigned int w = *reinterpret_cast<const unsigned int*>(codes + (int64_t)row * C + c);
+    const float step = ckpt8_step(exps[(int64_t)row * (C >> 5) + block]), mean = mean_in[row], rstd = rstd_in[row];
+    const float dv[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      dg[i] = fmaf(dv[i], (ckpt8_value(w, i, step) - mean) * rstd, dg[i]);
+      db[i] += dv[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { part[0][k][4 * l + i] = dg[i]; part[1][k][4 * l + i] = db[i]; }
+  __syncthreads();
+  const int j = threadIdx.x & 31, z = (threadIdx.x >> 5) & 1;
+  if (threadIdx.x >= 64) return;
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) t += part[z][i][j];
+  (z ? dbeta : dgamma)[32 * block + j] = t;
+}
 template <typename T, int NV, bool WG>
 __global__ __launch_bounds__(64 * LNB_WAVES) void ln_bwd_ckpt8_kernel(const T* __restrict__ dy, int64_t lddy, const signed char* __restrict__ codes,
                                                                       const unsigned char* __restrict__ exps, const float* __restrict__ mean_in,
                                                                       const float* __restrict__ rstd_in, const float* __restrict__ gamma,
                                                                       const float* __restrict__ beta, const float* __restrict__ dres,
                                                                       float* __restrict__ dx, bf16_t* __restrict__ dx_bf, bf16_t* __restrict__ y,
-                                                                      float* __restrict__ slabs, int64_t rows, int C) {
+                                                                      float* __restrict__ slabs, int64_t rows, int C, int col_wgs, float* __restrict__ dgamma,
+                                                                      float* __restrict__ dbeta) {
   extern __shared__ float lds_w[];      // WG: [2][C]
+  if (!WG && (int)blockIdx.x < col_wgs) {
+    ln_bwd_ckpt8_columns<T>(dy, lddy, codes, exps, mean_in, rstd_in, dgamma, dbeta, (int)rows, C, blockIdx.x);
+    return;
+  }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float4 ga[NV], dg[NV], db[NV];
 #pragma unroll
@@ -284,7 +324,7 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void ln_bwd_ckpt8_kernel(const T* _
     dg[j] = db[j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   const float invC = 1.0f / (float)C;
-  const int64_t stride = (int64_t)gridDim.x * LNB_WAVES;
+  const int64_t stride = (int64_t)(gridDim.x - col_wgs) * LNB_WAVES;
   // Operands of a row as they lie in memory. Up to NV = 5 the next row's are requested before this row's arithmetic (registers end it
   // there): with one row in flight per wave the loop reached 4.1 TB/s.
   struct Raw { Raw4<T> d[NV]; unsigned int w[NV], by[NV]; float4 r[NV]; float mean, rstd; };
@@ -303,7 +343,7 @@ __global__ __launch_bounds__(64 * LNB_WAVES) void ln_bwd_ckpt8_kernel(const T* _
   };
   constexpr bool AHEAD = NV <= 5;
   Raw cur, nxt;
-  int64_t row = (int64_t)blockIdx.x * LNB_WAVES + wave;
+  int64_t row = (int64_t)(blockIdx.x - col_wgs) * LNB_WAVES + wave;
   if (AHEAD && row < rows) request(row, nxt);
   for (; row < rows; row += stride) {
     if (AHEAD) {
@@ -499,13 +539,15 @@ extern "C" int mfnet_layernorm_fwd_ckpt8(const void* x, int x_dtype, int64_t ldx
   return MFNET_OK;
 }
 
+// few rows (see ln_bwd_ckpt8_columns)
+static bool ln_ck_few(int64_t rows) { return rows <= LNB_FEW; }
 static int64_t ln_ck_wgs(int64_t rows) {
   const int64_t n = ceil_div64(rows, LNB_WAVES);
   return n < LNB_MAX_WG ? n : LNB_MAX_WG;
 }
 // floats of workspace of mfnet_layernorm_bwd_ckpt8 with weight gradients
 extern "C" int64_t mfnet_layernorm_ckpt8_workspace_floats(int64_t rows, int64_t C) {
-  return rows <= 0 || C <= 0 ? 0 : ln_ck_wgs(rows) * 2 * C;
+  return rows <= 0 || C <= 0 || ln_ck_few(rows) ? 0 : ln_ck_wgs(rows) * 2 * C;
 }
 
 extern "C" int mfnet_layernorm_bwd_ckpt8(const void* dy, int dy_dtype, int64_t lddy, const void* codes, const void* exps, const float* mean,
@@ -519,20 +561,22 @@ extern "C" int mfnet_layernorm_bwd_ckpt8(const void* dy, int dy_dtype, int64_t l
                "layernorm_bwd_ckpt8: null pointer (dy with dx, or y alone)");
   MF_CHECK_ARG(!y || beta, "layernorm_bwd_ckpt8: y needs beta");
   const int64_t n = rows ? ln_ck_wgs(rows) : 0;
-  MF_CHECK_ARG(!wg || n == 0 || (ws && ws_floats >= n * 2 * C), "layernorm_bwd_ckpt8: workspace too small");
+  const bool few = rows && ln_ck_few(rows), slabs = wg && !few;
+  const int col_wgs = wg && few ? (int)(C / 32) : 0;
+  MF_CHECK_ARG(!slabs || n == 0 || (ws && ws_floats >= n * 2 * C), "layernorm_bwd_ckpt8: workspace too small");
   if (rows) {
     MF_CHECK_ARG(!dy || (lddy >= C && lddy % 4 == 0), "layernorm_bwd_ckpt8: lddy must be >= C and a multiple of 4");
     MF_CHECK_ARG(((uintptr_t)gamma | (uintptr_t)beta | (uintptr_t)dres | (uintptr_t)dx) % 16 == 0 && (uintptr_t)dy % (dy_dtype == MFNET_F32 ? 16 : 8) == 0 &&
                  ((uintptr_t)dx_bf16 | (uintptr_t)y) % 8 == 0 && (uintptr_t)codes % 4 == 0, "layernorm_bwd_ckpt8: misaligned tensor");
-#define LNB(T_, NV_, W_) hipLaunchKernelGGL((ln_bwd_ckpt8_kernel<T_, NV_, W_>), dim3((unsigned)n), dim3(64 * LNB_WAVES), W_ ? 2 * (size_t)C * 4 : 0, stream, (const T_*)dy, lddy, \
-    (const signed char*)codes, (const unsigned char*)exps, mean, rstd, gamma, beta, dres, dx, (bf16_t*)dx_bf16, (bf16_t*)y, ws, rows, (int)C)
-#define LNB_CASE(NV_) case NV_: if (dy_dtype == MFNET_F32) { if (wg) LNB(float, NV_, true); else LNB(float, NV_, false); } else { if (wg) LNB(bf16_t, NV_, true); else LNB(bf16_t, NV_, false); } break;
+#define LNB(T_, NV_, W_) hipLaunchKernelGGL((ln_bwd_ckpt8_kernel<T_, NV_, W_>), dim3((unsigned)(n + col_wgs)), dim3(64 * LNB_WAVES), W_ ? 2 * (size_t)C * 4 : 0, stream, (const T_*)dy, lddy, \
+    (const signed char*)codes, (const unsigned char*)exps, mean, rstd, gamma, beta, dres, dx, (bf16_t*)dx_bf16, (bf16_t*)y, ws, rows, (int)C, col_wgs, dgamma, dbeta)
+#define LNB_CASE(NV_) case NV_: if (dy_dtype == MFNET_F32) { if (slabs) LNB(float, NV_, true); else LNB(float, NV_, false); } else { if (slabs) LNB(bf16_t, NV_, true); else LNB(bf16_t, NV_, false); } break;
     switch ((int)ceil_div64(C, 256)) { LNB_CASE(1) LNB_CASE(2) LNB_CASE(3) LNB_CASE(4) LNB_CASE(5) LNB_CASE(6) LNB_CASE(7) LNB_CASE(8) }
 #undef LNB_CASE
 #undef LNB
     MF_LAUNCH_CHECK("layernorm_bwd_ckpt8");
   }
-  if (wg) {      // (no rows: the sums of nothing, zeros)
+  if (slabs) {      // (no rows: the sums of nothing, zeros)
     hipLaunchKernelGGL(ln_bwd_ckpt8_sum_kernel, dim3((unsigned)(C / 16)), dim3(1024), 0, stream, ws, (int)n, (int)C, dgamma, dbeta);
     MF_LAUNCH_CHECK("layernorm_bwd_ckpt8 (sums)");
   }

@@ -1823,7 +1823,7 @@ def layernorm_bwd_ckpt8(dy, c: Ckpt8, mean, rstd, gamma, beta=None, dres=None, w
     if want_weights:
         nws = _lib.lib().mfnet_layernorm_ckpt8_workspace_floats(rows, C)
         dg, db = gamma.new_empty((2, C)).unbind(0)
-        ws = gamma.new_empty((nws,))
+        ws = gamma.new_empty((nws,)) if nws else None
     per_el = (2 if dt else 4) + (4 if dres is not None else 0) + (4 if want_f32 else 0) + (2 if want_bf16 else 0) + (2 if want_y else 0)
     codes, exps = c._ptrs()
     _launch("mfnet_layernorm_bwd_ckpt8", dev, rows * C * per_el + c.nbytes + 8 * rows, 0, d2.data_ptr(), dt, ldd, codes, exps, mean.data_ptr(),

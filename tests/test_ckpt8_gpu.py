@@ -147,7 +147,8 @@ def ln64(x, gamma, beta, eps):
 LN_CASES = [(1, 32, torch.float32, torch.bfloat16), (5, 64, torch.bfloat16, torch.float32), (33, 128, torch.float32, torch.float32),
             (512, 768, torch.float32, torch.bfloat16), (70, 1024, torch.bfloat16, torch.bfloat16), (4200, 1280, torch.float32, torch.bfloat16),
             (9, 2048, torch.float32, torch.bfloat16), (0, 96, torch.float32, torch.bfloat16), (6, 1760, torch.bfloat16, torch.bfloat16),
-            (10, 1376, torch.float32, torch.float32)]
+            (10, 1376, torch.float32, torch.float32), (2048, 96, torch.bfloat16, torch.float32), (2049, 96, torch.float32, torch.float32),
+            (2100, 1760, torch.float32, torch.bfloat16), (65, 32, torch.float32, torch.float32)]
 
 
 @pytest.mark.parametrize("rows,C,xdt,ddt", LN_CASES)

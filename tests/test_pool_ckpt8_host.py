@@ -29,6 +29,7 @@ def test_entry_points_refuse_bad_arguments_before_a_launch():
         assert L.mfnet_layernorm_bwd_ckpt8(*a) == -1 and msg in E(), msg
     a = list(bwd)
     a[13] = a[14] = 16
+    a[17] = 2049                               # (up to 2048 rows need none)
     assert L.mfnet_layernorm_bwd_ckpt8(*a) == -1 and b"workspace" in E()
     pack = dict(A=16, B=16, dt=0, scale=None, n=2, K=64, N=64, r=4, RP=16, a_down=16, a_up=16, b_down=16, b_up=16, so=16, s=None)
     for key, v, msg in (("r", 20, b"sizes"), ("K", 60, b"sizes"), ("N", 4, b"sizes"), ("RP", 24, b"sizes"), ("n", 0, b"sizes"), ("b_down", None, b"null"), ("so", None, b"null"), ("a_up", 24, b"misaligned"),
@@ -50,7 +51,7 @@ def test_entry_points_refuse_bad_arguments_before_a_launch():
 
 def test_sizes():
     L = _L()
-    assert L.mfnet_layernorm_ckpt8_workspace_floats(1, 64) == 128 and L.mfnet_layernorm_ckpt8_workspace_floats(1 << 20, 64) == 512 * 128
+    assert [L.mfnet_layernorm_ckpt8_workspace_floats(r, 64) for r in (0, 1, 2048, 2049, 1 << 20)] == [0, 0, 0, 257 * 128, 512 * 128]
     assert L.mfnet_lora_pool_chunks(0, 5) == 0 and L.mfnet_lora_pool_chunks(3, 100) == 3
     for M in (1, 127, 128, 129, 5000, 16384, 16385, 100000):      # every split of M rows over n adapters fits
         for n in (1, 3, 50):
