@@ -1098,7 +1098,7 @@ __global__ __launch_bounds__(512, XF * G <= 12 ? 4 : 2) void pool_gemm_phased_ke
 }
 
 // ------------------------------------------------------------------------------------------------ dA / dB: sums over an adapter's rows
-// part[chunk] = sum over the chunk's rows of y_m u_m^T. 256 columns of y per workgroup, the four waves take every fourth step of 32 rows:
+// part[chunk] = sum over the chunk's rows of y_m u_m^T. 256 columns of y per workgroup, its W waves take every W-th step of 32 rows:
 // a step is copied into wave-private [32][64] LDS slabs (row-major, swizzled) and read transposed (ds_read_b64_tr_b16) as one MFMA
 // operand; the other is u (fp32), split into three bf16 parts. Rows behind the chunk are zeros on BOTH sides, rows of other adapters are
 // never read. y is bf16 or an 8-bit checkpoint, whose values are exact in bf16. RANK_MAJOR: part [RP][C] (dA), else [C][RP] (dB).
@@ -1109,13 +1109,13 @@ struct PoolTn {
   const int* base;
 };
 #define TN_MAX_CH 512
-template <int NR, bool CKPT, bool RANK_MAJOR>
+template <int NR, bool CKPT, bool RANK_MAJOR, int W>
 __device__ __forceinline__ void pool_tn_body(unsigned char (*lds)[4][32 * 128], int* rows, const PoolTn& p, const int4 ck, int strip) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int fr = lane & 15, fq = lane >> 4;
   const int cw = strip * 256, C = p.C, len = ck.z - ck.y;
   const int j0 = 16 * NR * blockIdx.z;                               // first rank of this workgroup
-  for (int i = threadIdx.x; i < len; i += 256) rows[i] = p.perm[ck.y + i];
+  for (int i = threadIdx.x; i < len; i += 64 * W) rows[i] = p.perm[ck.y + i];
   __syncthreads();
   f32x4_t acc[4][4][NR];
 #pragma unroll
@@ -1155,7 +1155,7 @@ __device__ __forceinline__ void pool_tn_body(unsigned char (*lds)[4][32 * 128], 
   };
   int i0 = 32 * wave;
   if (i0 < len) issue(i0);
-  for (; i0 < len; i0 += 128) {
+  for (; i0 < len; i0 += 32 * W) {
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
@@ -1176,7 +1176,7 @@ __device__ __forceinline__ void pool_tn_body(unsigned char (*lds)[4][32 * 128], 
     for (int f = 0; f < NR; ++f)
 #pragma unroll
       for (int q = 0; q < 3; ++q) up[f][q] = split_part(uv[f], q);
-    if (i0 + 128 < len) issue(i0 + 128);
+    if (i0 + 32 * W < len) issue(i0 + 32 * W);
     const int trow = 4 * fq + (fr >> 2);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -1196,7 +1196,7 @@ __device__ __forceinline__ void pool_tn_body(unsigned char (*lds)[4][32 * 128], 
       }
     }
   }
-  // sum of the four waves, one slab of 64 columns after the other (16 KB per wave and fragment column); wave w writes tile t = w
+  // sum of the waves, in order (16 KB per wave and fragment column); wave w writes slab w % 4, of eight waves each half of its tiles
   float* out = p.out ? p.out + (int64_t)blockIdx.y * p.r * C : p.part + (int64_t)blockIdx.y * p.RP * C;
   const int ld = p.out ? p.r : p.RP, jmax = p.out ? p.r : p.RP;
 #pragma unroll
@@ -1211,24 +1211,24 @@ __device__ __forceinline__ void pool_tn_body(unsigned char (*lds)[4][32 * 128], 
         for (int r = 0; r < 4; ++r) mine[((s * 4 + t) * 4 + r) * 64 + lane] = acc[s][t][f][r];
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int ti = 0; ti < 16 / W; ++ti)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int idx = ((wave * 4 + t) * 4 + r) * 64 + lane;
+        const int t = ti + 16 / W * (wave >> 2), idx = (((wave & 3) * 4 + t) * 4 + r) * 64 + lane;
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) v += reinterpret_cast<const float*>(lds[w][0])[idx];
+        for (int w = 0; w < W; ++w) v += reinterpret_cast<const float*>(lds[w][0])[idx];
         const int a = 4 * fq + r;
-        const int c = cw + 64 * wave + 16 * t + (RANK_MAJOR ? fr : a), j = j0 + 16 * f + (RANK_MAJOR ? a : fr);
+        const int c = cw + 64 * (wave & 3) + 16 * t + (RANK_MAJOR ? fr : a), j = j0 + 16 * f + (RANK_MAJOR ? a : fr);
         if (c < C && j < jmax) out[RANK_MAJOR ? (int64_t)j * C + c : (int64_t)c * ld + j] = v;
       }
   }
 }
 
 // both sums of a layer in one launch: the first strips_a workgroups of a chunk row take dA, the others dB
-template <int NR, bool CKPT>
-__global__ __launch_bounds__(256, 2) void pool_tn_kernel(const PoolTn a, const PoolTn b, int strips_a) {
-  __shared__ __attribute__((aligned(16))) unsigned char lds[4][4][32 * 128];
+template <int NR, bool CKPT, int W>
+__global__ __launch_bounds__(64 * W, 2) void pool_tn_kernel(const PoolTn a, const PoolTn b, int strips_a) {
+  __shared__ __attribute__((aligned(16))) unsigned char lds[W][4][32 * 128];
   __shared__ int rows[TN_MAX_CH];
   int4 ck;
   if (a.out) {                                             // blockIdx.y is an adapter: its only chunk, or no rows (sums of nothing)
@@ -1236,8 +1236,8 @@ __global__ __launch_bounds__(256, 2) void pool_tn_kernel(const PoolTn a, const P
     ck = k < a.base[blockIdx.y + 1] ? a.table[k] : make_int4((int)blockIdx.y, 0, 0, 0);
   } else ck = a.table[blockIdx.y];
   if (ck.x < 0) return;
-  if ((int)blockIdx.x < strips_a) pool_tn_body<NR, CKPT, true>(lds, rows, a, ck, blockIdx.x);
-  else pool_tn_body<NR, false, false>(lds, rows, b, ck, blockIdx.x - strips_a);
+  if ((int)blockIdx.x < strips_a) pool_tn_body<NR, CKPT, true, W>(lds, rows, a, ck, blockIdx.x);
+  else pool_tn_body<NR, false, false, W>(lds, rows, b, ck, blockIdx.x - strips_a);
 }
 
 // out[i] = sum over the chunks of adapter i, in order; part entries [d0][ld] -> out [d0][d1] (the padded ranks are dropped). No rows: zeros.
@@ -1285,8 +1285,11 @@ extern "C" int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, con
   return MFNET_OK;
 }
 
-// rows of a chunk of the backward sums
-static int pool_chunk_rows(int64_t M) { return M <= 16384 ? 128 : TN_MAX_CH; }
+// Rows of a chunk of the backward sums. Up to 512 rows: every adapter's rows are one chunk, whose sums are the result (no second launch);
+// above 128 rows eight waves share it. Against chunks of 128 rows and their sum: 509 rows of 2 adapters, 768 -> 768: 25.2 to 22.0 us a
+// backward call; 512 of 8, 1280 -> 3840: 35.2 to 32.1, of 1: 34.7 to 35.6.
+static bool pool_one_chunk(int64_t M) { return M <= TN_MAX_CH; }
+static int pool_chunk_rows(int64_t M) { return !pool_one_chunk(M) && M <= 16384 ? 128 : TN_MAX_CH; }
 extern "C" int64_t mfnet_lora_pool_chunks(int64_t M, int64_t n) {
   return M <= 0 || n <= 0 ? 0 : M / pool_chunk_rows(M) + (n < M ? n : M);
 }
@@ -1395,9 +1398,9 @@ extern "C" int mfnet_lora_pool_fwd(const void* X, int64_t ldx, const void* W, in
   return pool_products(p, a_down, scale, nullptr, nullptr, down, stream);
 }
 
-// floats of workspace of mfnet_lora_pool_bwd: p [M, RP] and its parts, the partial sums of dA and dB
+// floats of workspace of mfnet_lora_pool_bwd: p [M, RP] and its parts, the partial sums of dA and dB (more than one chunk per adapter)
 extern "C" int64_t mfnet_lora_pool_bwd_workspace_floats(int64_t M, int64_t n, int64_t K, int64_t N, int RP) {
-  return M <= 0 ? 0 : mfnet_lora_pool_down_floats(M, RP, MFNET_BF16) + mfnet_lora_pool_chunks(M, n) * (K + N) * RP;
+  return M <= 0 ? 0 : mfnet_lora_pool_down_floats(M, RP, MFNET_BF16) + (pool_one_chunk(M) ? 0 : mfnet_lora_pool_chunks(M, n) * (K + N) * RP);
 }
 
 extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, int64_t ldx, const void* codes, const void* exps, const void* Wt, int64_t ldwt,
@@ -1436,16 +1439,18 @@ extern "C" int mfnet_lora_pool_bwd(const void* dy, int64_t lddy, const void* X, 
     a.U = ws; a.RP = RP; a.perm = perm; a.table = (const int4*)table; a.part = part_a; a.C = (int)K;
     b = a;
     b.Y = (const bf16_t*)dy; b.ldy = lddy; b.U = down; b.part = part_b; b.C = (int)N;
-    const bool one_chunk = M <= pool_chunk_rows(M);
+    const bool one_chunk = pool_one_chunk(M);
     a.base = b.base = base;
     a.r = b.r = r;
     a.out = one_chunk ? dA : nullptr;
     b.out = one_chunk ? dB : nullptr;
     const int strips_a = (int)ceil_div64(K, 256), strips_b = (int)ceil_div64(N, 256);
     const dim3 grid((unsigned)(strips_a + strips_b), (unsigned)(one_chunk ? n : chunks), RP == 64 ? 2 : 1);
-#define PT(NR_, CK_) hipLaunchKernelGGL((pool_tn_kernel<NR_, CK_>), grid, dim3(256), 0, stream, a, b, strips_a)
-    if (RP == 16) { if (codes) PT(1, true); else PT(1, false); }
-    else { if (codes) PT(2, true); else PT(2, false); }
+#define PT(NR_, CK_, W_) hipLaunchKernelGGL((pool_tn_kernel<NR_, CK_, W_>), grid, dim3(64 * W_), 0, stream, a, b, strips_a)
+#define PTW(W_) do { if (RP == 16) { if (codes) PT(1, true, W_); else PT(1, false, W_); } \
+    else { if (codes) PT(2, true, W_); else PT(2, false, W_); } } while (0)
+    if (one_chunk && M > 128) PTW(8); else PTW(4);
+#undef PTW
 #undef PT
     MF_LAUNCH_CHECK("lora_pool_bwd (sums over rows)");
     if (one_chunk) return MFNET_OK;
