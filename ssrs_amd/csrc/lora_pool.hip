@@ -647,9 +647,9 @@ __global__ __launch_bounds__(256) void pool_gemm_rows_kernel(const PoolGemm p) {
   }
 }
 
-// At most 16 rows: both products in one launch. 16 waves per workgroup and 32 columns: wave w computes down of row w (every workgroup
+// At most 16 rows, short ones: both products in one launch. 16 waves per workgroup and 32 columns: wave w computes down of row w (every workgroup
 // again: M 16 NR K products beside the 32 M K of its own, the factors come from L2) while the weight is on its way, then the waves
-// split K for the 32 columns, add up through LDS and add the update. The second launch that this saves costs more than it.
+// split K for the 32 columns, add up through LDS and add the update.
 template <int NR>
 __global__ __launch_bounds__(1024) void pool_rows_fused_kernel(const PoolGemm p, const bf16_t* __restrict__ F, const float* __restrict__ scale, float* __restrict__ down) {
   constexpr int RP = 16 * NR;
@@ -1359,7 +1359,12 @@ static int pool_gemm(PoolGemm& p, hipStream_t stream) {
 // (down: M RP fp32 and behind them, above 64 rows, the parts)
 static int pool_products(PoolGemm& p, const void* image, const float* scale, const int* perm, const int* count, float* down, hipStream_t stream) {
   p.D = down;
-  if (p.M > 16 || p.RP > 32) {                              // (64 ranks: more registers than 16 waves have)
+  // One launch for both products saves the host 3 us, but every workgroup makes all down products again: it pays while they are few. us a
+  // call, issued one by one (on the GPU alone): 16 rows, 768 -> 2304, rank 16: 11.4 (10.8) in one launch, 14.7 (7.1) in two; 8 rows,
+  // 1280 -> 3840: 11.3 (10.8), 14.3 (8.1); 16 rows: 15.8 (16.1), 14.7 (8.6); 1 row, 1280 -> 5120, rank 32: 11.3 (10.6), 14.9 (10.0); 1 row,
+  // 5120 -> 1280, rank 16: 21.0 (21.5), 15.8 (15.5). (64 ranks: more registers than 16 waves have.)
+  const int64_t one_row = (int64_t)p.K * p.RP;
+  if (p.M > 16 || p.RP > 32 || one_row > 40960 || p.M * one_row > (1 << 18)) {
     PoolDown d = {down, reinterpret_cast<bf16_t*>(down + p.M * p.RP), p.M > 64 ? p.out_f32 ? 3 : 2 : 0};
     p.U = d.parts;
     p.P = d.P;
