@@ -365,7 +365,7 @@ __global__ __launch_bounds__(256) void pool_down_kernel(const bf16_t* __restrict
   }
 }
 
-// Few rows: one row per workgroup, the four waves take every fourth k-step.
+// One row per workgroup, the four waves take every fourth k-step.
 template <int NR>
 __global__ __launch_bounds__(256) void pool_down_row_kernel(const bf16_t* __restrict__ X, int64_t ldx, const bf16_t* __restrict__ F, const float* __restrict__ scale,
                                                             const int* __restrict__ ids, int n, const PoolDown out, int K) {
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256) void pool_down_row_kernel(const bf16_t* __rest
 // ------------------------------------------------------------------------------------------------ out = X W^T + bias + Up_i down
 struct PoolGemm {
   const bf16_t* X; int64_t ldx; const bf16_t* W; int64_t ldw; const float* bias;
-  const float* D; const bf16_t* U; int P;                   // the down products: fp32 (up to 64 rows), in P parts (more)
+  const float* D; const bf16_t* U; int P;                   // the down products: fp32 (few rows), in P parts
   const bf16_t* Up; const int* ids; int n, RP;
   void* out; int64_t ldo; int out_f32;
   int64_t M; int N, K, tiles_m, tiles_n;
@@ -572,7 +572,7 @@ __device__ __forceinline__ void pool_epilogue(const PoolGemm& p, f32x4_t (&acc)[
   }
 }
 
-// Few rows (M <= 16 XF): 16 columns per workgroup, the four waves take every fourth 64-wide piece of K and add up through LDS: the
+// Few rows: 16 XF of them and 16 columns per workgroup, the four waves take every fourth 64-wide piece of K and add up through LDS: the
 // weight is streamed once and every request of a wave is independent. Bound by latency. The low-rank update needs no matrix
 // instruction here: a lane owns one row and four columns, whose RP factors lie in one piece; they are requested before the products.
 template <int XF>
@@ -580,8 +580,8 @@ __global__ __launch_bounds__(256) void pool_gemm_rows_kernel(const PoolGemm p) {
   __shared__ f32x4_t red[4][XF][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fr = lane & 15, fq = lane >> 4;
-  const int n0 = blockIdx.x * 16, K = p.K, M = (int)p.M;
-  const int mf = 16 * wave + fr, cb = n0 + 4 * fq;           // the row and columns this lane finishes (waves below XF)
+  const int m0 = blockIdx.y * 16 * XF, n0 = blockIdx.x * 16, K = p.K, M = (int)p.M;
+  const int mf = m0 + 16 * wave + fr, cb = n0 + 4 * fq;           // the row and columns this lane finishes (waves below XF)
   const bool fin = wave < XF && mf < M && cb < p.N;
   float add[4] = {0.f, 0.f, 0.f, 0.f};
   if (fin && p.bias) {
@@ -612,7 +612,7 @@ __global__ __launch_bounds__(256) void pool_gemm_rows_kernel(const PoolGemm p) {
   const bf16_t* w = p.W + (int64_t)(n0 + fr < p.N ? n0 + fr : p.N - 1) * p.ldw + 8 * fq;
   const bf16_t* x[XF];
 #pragma unroll
-  for (int b = 0; b < XF; ++b) x[b] = p.X + (int64_t)(16 * b + fr < M ? 16 * b + fr : M - 1) * p.ldx + 8 * fq;
+  for (int b = 0; b < XF; ++b) x[b] = p.X + (int64_t)(m0 + 16 * b + fr < M ? m0 + 16 * b + fr : M - 1) * p.ldx + 8 * fq;
   f32x4_t acc[XF];
 #pragma unroll
   for (int b = 0; b < XF; ++b) acc[b] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
@@ -1305,14 +1305,21 @@ extern "C" int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* o
   return MFNET_OK;
 }
 
+// Few rows, which the product takes 64 at a time with 16 columns per workgroup: up to 64, and more while the workgroups fill the chip once
+// (long rows) or twice. us a call, 16 adapters in random order, 64 x 64 tiles and so: [256, 768] -> 768 15.2, 10.0; [192, 768] -> 2304,
+// rank 32 21.9, 17.4; [100, 256] -> 4096 12.7, 8.8; [192, 1280] -> 1280 17.2, 12.6; but [256, 1280] -> 1280 17.6, 18.9 and
+// [256, 768] -> 2304 21.8, 23.2.
+static bool pool_few(int64_t M, int64_t N, int64_t K) { return M <= 64 || ceil_div64(M, 64) * ceil_div64(N, 16) <= (K <= 1024 ? 512 : 256); }
+
 // perm / count: the rows that have an adapter, grouped by it (NULL: the rows as they come; every row of out is written)
 static int pool_down(const void* X, int64_t ldx, const void* image, const float* scale, const int* ids, int64_t n, int RP, const int* perm, const int* count, const PoolDown& out, int64_t M,
                      int64_t K, hipStream_t stream) {
-  // Up to 256 rows: a workgroup per row is quicker than 16 rows and their adapters in turn. 32 rows per workgroup halve the factor's
-  // traffic where there are enough of them to fill the chip.
+  // Up to 1024 rows: a workgroup per row, whatever the adapters' order; above, 16 rows that share their factor (a call on 16 adapters,
+  // K = 1280, rank 16: 1024 rows in runs 13.7 us with a workgroup per row, 13.0 with 16 rows, in random order 14.1 and 25.0; 4096 rows
+  // 22.7 and 15.4, 22.9 and 29.5). 32 rows per workgroup halve the factor's traffic where there are enough of them to fill the chip.
 #define PDL(NR_, XR_) hipLaunchKernelGGL((pool_down_kernel<NR_, XR_>), dim3((unsigned)ceil_div64(M, 16 * XR_)), dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)image, scale, ids, (int)n, perm, count, out, M, (int)K)
 #define PD(NR_) do { \
-    if (M <= 256) hipLaunchKernelGGL((pool_down_row_kernel<NR_>), dim3((unsigned)M), dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)image, scale, ids, (int)n, out, (int)K); \
+    if (M <= 1024) hipLaunchKernelGGL((pool_down_row_kernel<NR_>), dim3((unsigned)M), dim3(256), 0, stream, (const bf16_t*)X, ldx, (const bf16_t*)image, scale, ids, (int)n, out, (int)K); \
     else if (M < 8192) PDL(NR_, 1); else PDL(NR_, 2); } while (0)
   if (RP == 16) PD(1); else if (RP == 32) PD(2); else PD(4);
 #undef PD
@@ -1324,9 +1331,9 @@ static int pool_down(const void* X, int64_t ldx, const void* image, const float*
 static int pool_gemm(PoolGemm& p, hipStream_t stream) {
   const int64_t M = p.M, N = p.N;
   auto tiles = [&](int bm, int bn) { p.tiles_m = (int)ceil_div64(M, bm); p.tiles_n = (int)ceil_div64(N, bn); return (int64_t)p.tiles_m * p.tiles_n; };
-#define PR(XF_) hipLaunchKernelGGL((pool_gemm_rows_kernel<XF_>), dim3((unsigned)ceil_div64(N, 16)), dim3(256), 0, stream, p)
+#define PR(XF_) hipLaunchKernelGGL((pool_gemm_rows_kernel<XF_>), dim3((unsigned)ceil_div64(N, 16), (unsigned)ceil_div64(M, 16 * XF_)), dim3(256), 0, stream, p)
   if (M <= 32) PR(2);
-  else if (M <= 64) PR(4);
+  else if (pool_few(M, N, p.K)) PR(4);
 #undef PR
   else {
     // The tile with the least modelled time, in us, as measured at K = 64 .. 8192 on 100 .. 32768 rows: a tile costs a fixed part and a
@@ -1356,7 +1363,7 @@ static int pool_gemm(PoolGemm& p, hipStream_t stream) {
 }
 
 // down = scale_i image_i x, out = x W^T (+ bias) + up_i down
-// (down: M RP fp32 and behind them, above 64 rows, the parts)
+// (down: M RP fp32 and behind them, unless there are few rows, the parts)
 static int pool_products(PoolGemm& p, const void* image, const float* scale, const int* perm, const int* count, float* down, hipStream_t stream) {
   p.D = down;
   // One launch for both products saves the host 3 us, but every workgroup makes all down products again: it pays while they are few. us a
@@ -1365,7 +1372,7 @@ static int pool_products(PoolGemm& p, const void* image, const float* scale, con
   // 5120 -> 1280, rank 16: 21.0 (21.5), 15.8 (15.5). (64 ranks: more registers than 16 waves have.)
   const int64_t one_row = (int64_t)p.K * p.RP;
   if (p.M > 16 || p.RP > 32 || one_row > 40960 || p.M * one_row > (1 << 18)) {
-    PoolDown d = {down, reinterpret_cast<bf16_t*>(down + p.M * p.RP), p.M > 64 ? p.out_f32 ? 3 : 2 : 0};
+    PoolDown d = {down, reinterpret_cast<bf16_t*>(down + p.M * p.RP), pool_few(p.M, p.N, p.K) ? 0 : p.out_f32 ? 3 : 2};
     p.U = d.parts;
     p.P = d.P;
     const int rc = pool_down(p.X, p.ldx, image, scale, p.ids, p.n, p.RP, perm, count, d, p.M, p.K, stream);

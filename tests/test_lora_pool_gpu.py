@@ -74,7 +74,7 @@ CASES = [(1, 64, 64, 1, 1, "one"), (1, 8, 8, 3, 5, "mixed"), (2, 72, 24, 2, 4, "
          (16, 1096, 200, 5, 32, "mixed"), (9, 3840, 72, 2, 20, "mixed"), (12, 264, 136, 3, 64, "mixed"), (17, 768, 2304, 70, 16, "mixed"), (128, 136, 264, 40, 16, "mixed"), (100, 72, 520, 3, 48, "runs"), (63, 128, 40, 3, 17, "runs"), (65, 1280, 128, 5, 64, "mixed"), (130, 200, 392, 24, 33, "mixed"),
          (257, 264, 520, 7, 16, "runs"), (509, 768, 768, 2, 5, "runs"), (700, 1024, 1032, 300, 8, "mixed"), (1200, 64, 1000, 3, 16, "none"),
          (3907, 520, 1160, 24, 16, "runs"), (6000, 328, 2312, 5, 16, "mixed"), (8192, 768, 2304, 8, 8, "runs"), (4000, 1096, 4104, 6, 16, "mixed"), (33000, 24, 520, 3, 16, "mixed"), (4100, 64, 4096, 3, 40, "runs"), (3800, 136, 4000, 4, 20, "mixed"), (16900, 72, 776, 3, 12, "runs"),
-         (16, 1288, 72, 3, 16, "mixed"), (3, 2568, 72, 2, 9, "mixed"), (1, 5120, 136, 2, 32, "one"), (512, 264, 776, 3, 40, "one"), (512, 72, 136, 2, 5, "one"), (513, 72, 136, 2, 5, "one"), (400, 520, 72, 20, 20, "mixed")]
+         (100, 264, 4104, 3, 16, "mixed"), (192, 776, 2312, 3, 32, "runs"), (1024, 264, 136, 9, 20, "mixed"), (1025, 264, 136, 9, 20, "mixed"), (1030, 1288, 264, 20, 64, "mixed"), (16, 1288, 72, 3, 16, "mixed"), (3, 2568, 72, 2, 9, "mixed"), (1, 5120, 136, 2, 32, "one"), (512, 264, 776, 3, 40, "one"), (512, 72, 136, 2, 5, "one"), (513, 72, 136, 2, 5, "one"), (400, 520, 72, 20, 20, "mixed")]
 
 
 @pytest.mark.parametrize("M,K,N,n,r,ids", CASES)
