@@ -8,6 +8,7 @@ from __future__ import annotations
 
 from typing import Optional
 
+import math
 import os
 
 import torch
@@ -1597,6 +1598,7 @@ def gather(pairs, accumulate=False):
 # The wrappers below are called with tensors of a few microseconds' work: their checks are written to cost about one (device indices
 # instead of device objects, messages formatted only when raised, one allocation for what belongs together).
 _raw_stream = torch._C._cuda_getCurrentRawStream        # torch.cuda.current_stream(device).cuda_stream without the Stream object
+_current_device = torch._C._cuda_getDevice              # torch.cuda.current_device() of a process that holds device tensors
 
 
 def _bad(name, what):
@@ -1621,10 +1623,12 @@ def _device_of(name, *ts):
 
 def _launch(name, dev, nbytes, flops, *args):
     """the entry point on the current stream of device dev, whichever device is current"""
-    if torch.cuda.current_device() != dev:
+    if _current_device() != dev:
         with torch.cuda.device(dev):
             return tcall(name, nbytes, flops, *args, _raw_stream(dev))
-    return (call(name, *args, _raw_stream(dev)) if KERNEL_TRACE is None else tcall(name, nbytes, flops, *args, _raw_stream(dev)))
+    if KERNEL_TRACE is not None:
+        return tcall(name, nbytes, flops, *args, _raw_stream(dev))
+    return call(name, *args, _raw_stream(dev))
 
 
 def _like(t, shape, dtype):
@@ -1656,16 +1660,13 @@ class Ckpt8:
 
     def __init__(self, t):
         """room for the checkpoint of tensor t"""
-        self.buf = t.new_empty((self._place(t.shape),), dtype=torch.uint8)
+        self.buf = t.new_empty(self._place(t.shape, t.numel()), dtype=torch.uint8)
 
-    def _place(self, shape):
-        self.shape = tuple(shape)
-        self.C = C = self.shape[-1]
-        rows = 1
-        for d in self.shape[:-1]:
-            rows *= d
-        self.rows = rows
-        self.at_exps = (rows * C + 15) // 16 * 16
+    def _place(self, shape, numel):
+        self.shape = shape
+        self.C = C = shape[-1]
+        self.rows = rows = numel // C
+        self.at_exps = (numel + 15) // 16 * 16
         return self.at_exps + rows * ((C + 31) // 32)
 
     @property
@@ -1692,7 +1693,7 @@ class Ckpt8:
     def of(cls, buf, shape):
         """the checkpoint whose buffer was kept by itself (autograd keeps tensors)"""
         c = cls.__new__(cls)
-        c._place(shape)
+        c._place(torch.Size(shape), math.prod(shape))
         c.buf = buf
         return c
 
