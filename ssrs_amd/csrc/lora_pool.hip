@@ -1305,11 +1305,11 @@ extern "C" int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* o
   return MFNET_OK;
 }
 
-// Few rows, which the product takes 64 at a time with 16 columns per workgroup: up to 64, and more while the workgroups fill the chip once
-// (long rows) or twice. us a call, 16 adapters in random order, 64 x 64 tiles and so: [256, 768] -> 768 15.2, 10.0; [192, 768] -> 2304,
-// rank 32 21.9, 17.4; [100, 256] -> 4096 12.7, 8.8; [192, 1280] -> 1280 17.2, 12.6; but [256, 1280] -> 1280 17.6, 18.9 and
-// [256, 768] -> 2304 21.8, 23.2.
-static bool pool_few(int64_t M, int64_t N, int64_t K) { return M <= 64 || ceil_div64(M, 64) * ceil_div64(N, 16) <= (K <= 1024 ? 512 : 256); }
+// Few rows, which the product takes 64 at a time with 16 columns per workgroup: up to 64, and more while the workgroups fill the chip at
+// most once. us a call with the 64 x 64 tiles and so, 2 adapters in runs: [256, 768] -> 768 9.8, 9.6; [192, 1280] -> 1280 11.9, 12.2;
+// [192, 3840] -> 1280 23.0, 24.9; 16 in random order (a tile multiplies with each in turn): 15.3, 10.0; 17.2, 12.5; 31.9, 27.5. Beyond:
+// [384, 768] -> 768 10.0, 13.3 in runs, 15.0, 14.2 in random order.
+static bool pool_few(int64_t M, int64_t N) { return M <= 64 || ceil_div64(M, 64) * ceil_div64(N, 16) <= 256; }
 
 // perm / count: the rows that have an adapter, grouped by it (NULL: the rows as they come; every row of out is written)
 static int pool_down(const void* X, int64_t ldx, const void* image, const float* scale, const int* ids, int64_t n, int RP, const int* perm, const int* count, const PoolDown& out, int64_t M,
@@ -1333,7 +1333,7 @@ static int pool_gemm(PoolGemm& p, hipStream_t stream) {
   auto tiles = [&](int bm, int bn) { p.tiles_m = (int)ceil_div64(M, bm); p.tiles_n = (int)ceil_div64(N, bn); return (int64_t)p.tiles_m * p.tiles_n; };
 #define PR(XF_) hipLaunchKernelGGL((pool_gemm_rows_kernel<XF_>), dim3((unsigned)ceil_div64(N, 16), (unsigned)ceil_div64(M, 16 * XF_)), dim3(256), 0, stream, p)
   if (M <= 32) PR(2);
-  else if (pool_few(M, N, p.K)) PR(4);
+  else if (pool_few(M, N)) PR(4);
 #undef PR
   else {
     // The tile with the least modelled time, in us, as measured at K = 64 .. 8192 on 100 .. 32768 rows: a tile costs a fixed part and a
@@ -1372,7 +1372,7 @@ static int pool_products(PoolGemm& p, const void* image, const float* scale, con
   // 5120 -> 1280, rank 16: 21.0 (21.5), 15.8 (15.5). (64 ranks: more registers than 16 waves have.)
   const int64_t one_row = (int64_t)p.K * p.RP;
   if (p.M > 16 || p.RP > 32 || one_row > 40960 || p.M * one_row > (1 << 18)) {
-    PoolDown d = {down, reinterpret_cast<bf16_t*>(down + p.M * p.RP), pool_few(p.M, p.N, p.K) ? 0 : p.out_f32 ? 3 : 2};
+    PoolDown d = {down, reinterpret_cast<bf16_t*>(down + p.M * p.RP), pool_few(p.M, p.N) ? 0 : p.out_f32 ? 3 : 2};
     p.U = d.parts;
     p.P = d.P;
     const int rc = pool_down(p.X, p.ldx, image, scale, p.ids, p.n, p.RP, perm, count, d, p.M, p.K, stream);
