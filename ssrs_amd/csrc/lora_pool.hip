@@ -1289,7 +1289,10 @@ extern "C" int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, con
 // above 128 rows eight waves share it. Against chunks of 128 rows and their sum: 509 rows of 2 adapters, 768 -> 768: 25.2 to 22.0 us a
 // backward call; 512 of 8, 1280 -> 3840: 35.2 to 32.1, of 1: 34.7 to 35.6.
 static bool pool_one_chunk(int64_t M) { return M <= TN_MAX_CH; }
-static int pool_chunk_rows(int64_t M) { return !pool_one_chunk(M) && M <= 16384 ? 128 : TN_MAX_CH; }
+// More rows: short chunks while they are few (they fill the chip), long ones where their partial sums would be bytes (both sums of K = 768,
+// N = 2304, rank 8, us with chunks of 128, 256 and 512: 4000 rows 23.2, 22.8, 28.3, 8192 rows 31.8, 28.4, 30.2, 24000 rows 69.1, 64.7,
+// 64.8; of K = N = 768: 15.1, 17.1, 23.1; 20.9, 20.1, 25.4; 43.7, 41.6, 37.6).
+static int pool_chunk_rows(int64_t M) { return pool_one_chunk(M) || M > 12288 ? TN_MAX_CH : M > 5000 ? 256 : 128; }
 extern "C" int64_t mfnet_lora_pool_chunks(int64_t M, int64_t n) {
   return M <= 0 || n <= 0 ? 0 : M / pool_chunk_rows(M) + (n < M ? n : M);
 }

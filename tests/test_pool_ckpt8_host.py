@@ -53,10 +53,10 @@ def test_sizes():
     L = _L()
     assert [L.mfnet_layernorm_ckpt8_workspace_floats(r, 64) for r in (0, 1, 2048, 2049, 1 << 20)] == [0, 0, 0, 257 * 128, 512 * 128]
     assert L.mfnet_lora_pool_chunks(0, 5) == 0 and L.mfnet_lora_pool_chunks(3, 100) == 3
-    for M in (1, 127, 128, 129, 512, 513, 5000, 16384, 16385, 100000):      # every split of M rows over n adapters fits
+    for M in (1, 127, 128, 129, 512, 513, 5000, 5001, 12288, 12289, 100000):      # every split of M rows over n adapters fits
         for n in (1, 3, 50):
             c = L.mfnet_lora_pool_chunks(M, n)
-            ch = 128 if 512 < M <= 16384 else 512
+            ch = 512 if M <= 512 or M > 12288 else 128 if M <= 5000 else 256
             one_each = min(n, M)
             worst = (one_each - 1) + -(-(M - one_each + 1) // ch)
             assert c >= worst
