@@ -613,7 +613,7 @@ class PooledLinear(nn.Linear):
     @classmethod
     def from_merged(cls, layers, checkpoint8=False):
         """the pool of several fine-tuned lora.MergedLinear layers over the same frozen weight: adapters 2 i and 2 i + 1 are the x and y
-        modality of layers[i] (rank 2 r: r columns feed the q third of the output, r the v third)"""
+        modality of layers[i] (rank 2 r: r columns feed the q third of the output, r the v third), with that layer's scaling"""
         first = layers[0]
         r, D = first.r, first.out_features // 3
         if any(m.r != r or m.weight.shape != first.weight.shape for m in layers):
@@ -625,8 +625,8 @@ class PooledLinear(nn.Linear):
             pool.weight.copy_(first.weight)
             pool.bias.copy_(first.bias)
             pool.lora_B.zero_()
-            pool.scaling.fill_(first.scaling)
             for i, m in enumerate(layers):
+                pool.scaling[2 * i:2 * i + 2] = m.scaling            # (lora_alpha / r: a fine-tune's own)
                 for j, (A, B) in enumerate(((m.lora_Ax, m.lora_Bx), (m.lora_Ay, m.lora_By))):
                     pool.lora_A[2 * i + j] = A
                     pool.lora_B[2 * i + j, :D, :r] = B[:D]

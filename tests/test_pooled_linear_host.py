@@ -1,0 +1,39 @@
+"""lora.PooledLinear before any launch (no GPU): the pool made of fine-tuned layers."""
+import pytest
+import torch
+
+
+def _merged(g, alpha, first=None, bias=True, r=4):
+    from ssrs_amd.medsam.models.common import loralib as lora
+    m = lora.MergedLinear(64, 192, r=r, lora_alpha=alpha, enable_lora=[True, False, True], bias=bias)
+    with torch.no_grad():
+        for p in (m.lora_Ax, m.lora_Ay, m.lora_Bx, m.lora_By):
+            p.copy_(torch.randn(p.shape, generator=g))
+        if first is not None:
+            m.weight.copy_(first.weight)
+            if bias:
+                m.bias.copy_(first.bias)
+    return m
+
+
+def _update(m, A, B):
+    """a layer's low-rank update of its [3 D, in] weight (q and v thirds), from its definition in 64 bits"""
+    r, D = m.r, m.out_features // 3
+    dw = torch.zeros(3 * D, m.in_features, dtype=torch.float64)
+    dw[:D] = m.scaling * B[:D].double() @ A[:r].double()
+    dw[2 * D:] = m.scaling * B[D:].double() @ A[r:].double()
+    return dw.detach()
+
+
+def test_pool_of_layers_keeps_each_layers_scaling():
+    from ssrs_amd.medsam.models.common import loralib as lora
+    g = torch.Generator().manual_seed(0)
+    layers = [_merged(g, 1)]
+    layers += [_merged(g, alpha, layers[0]) for alpha in (16, 3)]
+    pool = lora.PooledLinear.from_merged(layers)
+    assert pool.scaling.tolist() == [0.25, 0.25, 4.0, 4.0, 0.75, 0.75]
+    for i, m in enumerate(layers):
+        for j, (A, B) in enumerate(((m.lora_Ax, m.lora_Bx), (m.lora_Ay, m.lora_By))):
+            k = 2 * i + j
+            got = pool.scaling[k].double() * pool.lora_B[k].double() @ pool.lora_A[k].double()
+            assert torch.allclose(got.detach(), _update(m, A, B), rtol=1e-12, atol=1e-12), k
