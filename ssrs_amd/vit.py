@@ -618,12 +618,14 @@ class PooledLinear(nn.Linear):
         r, D = first.r, first.out_features // 3
         if any(m.r != r or m.weight.shape != first.weight.shape for m in layers):
             raise ValueError("the layers of a pool share rank and shape")
-        if any(not torch.equal(m.weight, first.weight) or not torch.equal(m.bias, first.bias) for m in layers[1:]):
+        has_bias = first.bias is not None
+        if any((m.bias is not None) != has_bias or not torch.equal(m.weight, first.weight) or (has_bias and not torch.equal(m.bias, first.bias)) for m in layers[1:]):
             raise ValueError("the layers of a pool share their frozen weight and bias")
-        pool = cls(first.in_features, first.out_features, 2 * len(layers), 2 * r, bias=True, checkpoint8=checkpoint8).to(first.weight.device)
+        pool = cls(first.in_features, first.out_features, 2 * len(layers), 2 * r, bias=has_bias, checkpoint8=checkpoint8).to(first.weight.device)
         with torch.no_grad():
             pool.weight.copy_(first.weight)
-            pool.bias.copy_(first.bias)
+            if has_bias:
+                pool.bias.copy_(first.bias)
             pool.lora_B.zero_()
             for i, m in enumerate(layers):
                 pool.scaling[2 * i:2 * i + 2] = m.scaling            # (lora_alpha / r: a fine-tune's own)

@@ -37,3 +37,19 @@ def test_pool_of_layers_keeps_each_layers_scaling():
             k = 2 * i + j
             got = pool.scaling[k].double() * pool.lora_B[k].double() @ pool.lora_A[k].double()
             assert torch.allclose(got.detach(), _update(m, A, B), rtol=1e-12, atol=1e-12), k
+
+
+def test_pool_of_layers_without_a_bias():
+    """no layer has a bias: the pool has none; some have one: refused like any other difference of the shared projection"""
+    from ssrs_amd.medsam.models.common import loralib as lora
+    g = torch.Generator().manual_seed(1)
+    layers = [_merged(g, 1, bias=False)]
+    layers.append(_merged(g, 1, layers[0], bias=False))
+    pool = lora.PooledLinear.from_merged(layers)
+    assert pool.bias is None and torch.equal(pool.weight, layers[0].weight) and torch.equal(pool.lora_A[3], layers[1].lora_Ay)
+    with_bias = _merged(g, 1)
+    with torch.no_grad():
+        with_bias.weight.copy_(layers[0].weight)
+    for mixed in ([layers[0], with_bias], [with_bias, layers[0]]):
+        with pytest.raises(ValueError, match="bias"):
+            lora.PooledLinear.from_merged(mixed)
