@@ -35,7 +35,8 @@ BF = torch.bfloat16
 # ---------------------------------------------------------------------------------------------
 def _cached(key, params, build, stamp=None):
     """Derived tensors live in a dict hung on the first source parameter (so they die with it and a
-    recycled id() can never alias another model's entry). stamp: one more thing that the entry goes stale with."""
+    recycled id() can never alias another model's entry). stamp: one more thing that the entry goes stale with. What is built while a
+    graph is captured belongs to that graph - only its replays fill it, in memory that goes with it - and is not kept."""
     store = params[0].__dict__.setdefault("_mfnet_derived", {})
     sig = (stamp,) + tuple((p.data_ptr(), p._version, p.device) for p in params)
     hit = store.get(key)
@@ -43,7 +44,8 @@ def _cached(key, params, build, stamp=None):
         return hit[1]
     with torch.no_grad():
         val = build()
-    store[key] = (sig, val)
+    if not (params[0].is_cuda and torch.cuda.is_current_stream_capturing()):
+        store[key] = (sig, val)
     return val
 
 

@@ -34,3 +34,55 @@ def test_pool_serves_layers_of_different_scaling():
                 a = m.scaling * xi.double().abs() @ A.double().abs().t()
                 terms = torch.cat([a[:, :4] @ B[:128].double().abs().t(), torch.zeros(48, 128, device="cuda", dtype=torch.float64), a[:, 4:] @ B[128:].double().abs().t()], 1)
                 assert ((got.double() - want.double()).abs() <= 2.5 * 2 ** -8 * terms + 1e-5).all()
+
+
+def _twins(seed, n=3, r=5, K=96, N=72, **kw):
+    """two modules of the same weights: one to look at, one to compare with"""
+    from ssrs_amd.medsam.models.common import loralib as lora
+    g = torch.Generator().manual_seed(seed)
+    a, b = (lora.PooledLinear(K, N, n, r, **kw).cuda() for _ in range(2))
+    with torch.no_grad():
+        a.lora_B.copy_(0.3 * _rows(g, n, N, r))
+    b.load_state_dict(a.state_dict())
+    return g, a, b
+
+
+def _dx(lin, x, ids, dy):
+    """the gradient of x alone (needs the transposed weight)"""
+    x = x.detach().clone().requires_grad_()
+    return torch.autograd.grad(lin(x, ids), x, dy)[0]
+
+
+def test_first_call_under_capture():
+    """A module whose first call is a captured one: what the capture makes of the frozen weight is the graph's own. Eager calls before the
+    first replay, between replays and after the graph is gone give what a module that was never captured gives."""
+    g, lin, ref = _twins(21)
+    x, dy = _rows(g, 130, 96).cuda(), _rows(g, 130, 72).cuda()
+    ids = torch.randint(-1, 3, (130,), generator=g, dtype=torch.int32).cuda()
+    with torch.no_grad():
+        want = ref(x, ids)
+    wdx = _dx(ref, x, ids, dy)                                # (the kernels are loaded; lin has not been called)
+    xs = x.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lin(xs, ids)
+        dx = torch.autograd.grad(out, xs, dy)[0]
+    del xs
+
+    def eager():
+        with torch.no_grad():
+            assert torch.equal(lin(x, ids), want)
+        assert torch.equal(_dx(lin, x, ids, dy), wdx)
+    eager()
+    for _ in range(3):
+        out.detach().zero_()
+        dx.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.detach(), want) and torch.equal(dx, wdx)
+        eager()
+    del out, dx
+    graph.reset()
+    junk = [torch.full((1 << 16,), float("nan"), device="cuda") for _ in range(64)]
+    eager()
+    del junk
