@@ -1597,7 +1597,7 @@ def gather(pairs, accumulate=False):
 # ------------------------------------------------------------------------------------------ 8-bit activation checkpoints
 # The wrappers below are called with tensors of a few microseconds' work: their checks are written to cost about one (device indices
 # instead of device objects, messages formatted only when raised, one allocation for what belongs together).
-_raw_stream = torch._C._cuda_getCurrentRawStream        # torch.cuda.current_stream(device).cuda_stream without the Stream object
+raw_stream = torch._C._cuda_getCurrentRawStream        # torch.cuda.current_stream(device).cuda_stream without the Stream object
 _current_device = torch._C._cuda_getDevice              # torch.cuda.current_device() of a process that holds device tensors
 
 
@@ -1625,10 +1625,10 @@ def _launch(name, dev, nbytes, flops, *args):
     """the entry point on the current stream of device dev, whichever device is current"""
     if _current_device() != dev:
         with torch.cuda.device(dev):
-            return tcall(name, nbytes, flops, *args, _raw_stream(dev))
+            return tcall(name, nbytes, flops, *args, raw_stream(dev))
     if KERNEL_TRACE is not None:
-        return tcall(name, nbytes, flops, *args, _raw_stream(dev))
-    return call(name, *args, _raw_stream(dev))
+        return tcall(name, nbytes, flops, *args, raw_stream(dev))
+    return call(name, *args, raw_stream(dev))
 
 
 def _like(t, shape, dtype):

@@ -33,19 +33,54 @@ BF = torch.bfloat16
 # frozen-weight caches (bf16 copies / transposes, resized tables); rebuilt when a parameter is
 # re-loaded (load_state_dict bumps _version) or moved (data_ptr changes)
 # ---------------------------------------------------------------------------------------------
+class _Derived:
+    """One entry of _cached: the value, the signature of what it was made from, and the streams that are ordered behind its making."""
+    __slots__ = ("sig", "val", "made", "streams")
+
+    def __init__(self, sig, val, dev):
+        self.sig, self.val, self.made, self.streams = sig, val, None, None
+        if dev >= 0:
+            self.made = torch.cuda.Event()
+            self.made.record(torch.cuda.current_stream(dev))
+            self.streams = {ops.raw_stream(dev)}
+
+    def join(self, dev):
+        """a stream that meets the entry for the first time waits for its making, and the memory is not given away before that stream
+        has read it. (Under capture nothing outside it can be waited for: torch.cuda.graph() waits for the device beforehand.)"""
+        raw = ops.raw_stream(dev)
+        if raw in self.streams or torch.cuda.is_current_stream_capturing():
+            return
+        stream = torch.cuda.current_stream(dev)
+        stream.wait_event(self.made)
+        for t in (self.val.buf,) if isinstance(self.val, ops.LoraPool) else (self.val,) if torch.is_tensor(self.val) else self.val:
+            if torch.is_tensor(t):
+                t.record_stream(stream)
+        self.streams.add(raw)
+
+    def __getstate__(self):                # (a stored module makes its entries anew: addresses, events and streams are this process's)
+        return None, None
+
+    def __setstate__(self, _):
+        self.sig = self.val = self.made = self.streams = None
+
+
 def _cached(key, params, build, stamp=None):
     """Derived tensors live in a dict hung on the first source parameter (so they die with it and a
     recycled id() can never alias another model's entry). stamp: one more thing that the entry goes stale with. What is built while a
-    graph is captured belongs to that graph - only its replays fill it, in memory that goes with it - and is not kept."""
+    graph is captured belongs to that graph - only its replays fill it, in memory that goes with it - and is not kept. An entry may be
+    used on any stream: see _Derived.join."""
     store = params[0].__dict__.setdefault("_mfnet_derived", {})
     sig = (stamp,) + tuple((p.data_ptr(), p._version, p.device) for p in params)
+    dev = params[0].get_device()
     hit = store.get(key)
-    if hit is not None and hit[0] == sig:
-        return hit[1]
+    if hit is not None and hit.sig == sig:
+        if dev >= 0:
+            hit.join(dev)
+        return hit.val
     with torch.no_grad():
         val = build()
-    if not (params[0].is_cuda and torch.cuda.is_current_stream_capturing()):
-        store[key] = (sig, val)
+    if dev < 0 or not torch.cuda.is_current_stream_capturing():
+        store[key] = _Derived(sig, val, dev)
     return val
 
 

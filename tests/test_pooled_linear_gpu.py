@@ -86,3 +86,53 @@ def test_first_call_under_capture():
     junk = [torch.full((1 << 16,), float("nan"), device="cuda") for _ in range(64)]
     eager()
     del junk
+
+
+def _occupy():
+    """some 20 ms of products on the current stream: what is queued behind them has not run when the host gets there"""
+    a = torch.ones(8192, 8192, device="cuda", dtype=torch.bfloat16)
+    for _ in range(30):
+        a = a @ a
+
+
+def test_streams_without_an_order_share_a_module():
+    """Two streams serve one module and nothing orders them: the second meets the images (and the weight's copies) that the first one has
+    queued behind other work. Then the factors and the weight change: the first stream makes new copies, and what the second stream has
+    queued before still reads the old ones."""
+    g, lin, ref = _twins(22, n=7, r=30, K=768, N=520)
+    x, dy = _rows(g, 300, 768).cuda(), _rows(g, 300, 520).cuda()
+    ids = torch.randint(-1, 7, (300,), generator=g, dtype=torch.int32).cuda()
+
+    def calls(m):
+        with torch.no_grad():
+            y = m(x, ids)
+        return y, _dx(m, x, ids, dy)
+    want = calls(ref)
+    new_B, new_w = 0.2 * _rows(g, 7, 520, 30).cuda(), _rows(g, 520, 768).cuda()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(a):                                  # (the library's own set-up for the products)
+        _occupy()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        _occupy()
+        got_a = calls(lin)
+    with torch.cuda.stream(b):
+        got_b = calls(lin)
+    torch.cuda.synchronize()
+    for got in (got_a, got_b):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    with torch.cuda.stream(b), torch.no_grad():                 # queued, not run yet, when the copies go stale (it reads nothing else of them)
+        _occupy()
+        late = lin(x, ids)
+    with torch.no_grad():
+        for m in (lin, ref):
+            m.lora_B.copy_(new_B)
+            m.weight.copy_(new_w)
+    a.wait_stream(torch.cuda.current_stream())                  # (the program orders its own writes to the factors)
+    with torch.cuda.stream(a):
+        got_a = calls(lin)
+        junk = [torch.full((n,), float("nan"), device="cuda", dtype=torch.bfloat16) for n in (768 * 520, lin.lora_A.numel(), lin.lora_B.numel()) * 8]
+    torch.cuda.synchronize()
+    assert torch.equal(late, want[0])
+    assert all(torch.equal(p, q) for p, q in zip(got_a, calls(ref)))
+    del junk
