@@ -34,11 +34,13 @@ BF = torch.bfloat16
 # re-loaded (load_state_dict bumps _version) or moved (data_ptr changes)
 # ---------------------------------------------------------------------------------------------
 class _Derived:
-    """One entry of _cached: the value, the signature of what it was made from, and the streams that are ordered behind its making."""
-    __slots__ = ("sig", "val", "made", "streams")
+    """One entry of _cached: the value, the signature of what it was made from, the streams that are ordered behind its making,
+    whether a captured graph reads it, and the values before it that captured graphs still read."""
+    __slots__ = ("sig", "val", "made", "streams", "captured", "older")
 
-    def __init__(self, sig, val, dev):
-        self.sig, self.val, self.made, self.streams = sig, val, None, None
+    def __init__(self, sig, val, dev, older=None):
+        self.sig, self.val, self.made, self.streams, self.captured = sig, val, None, None, False
+        self.older = () if older is None else older.older + ((older.val,) if older.captured else ())
         if dev >= 0:
             self.made = torch.cuda.Event()
             self.made.record(torch.cuda.current_stream(dev))
@@ -47,8 +49,11 @@ class _Derived:
     def join(self, dev):
         """a stream that meets the entry for the first time waits for its making, and the memory is not given away before that stream
         has read it. (Under capture nothing outside it can be waited for: torch.cuda.graph() waits for the device beforehand.)"""
+        if torch.cuda.is_current_stream_capturing():
+            self.captured = True
+            return
         raw = ops.raw_stream(dev)
-        if raw in self.streams or torch.cuda.is_current_stream_capturing():
+        if raw in self.streams:
             return
         stream = torch.cuda.current_stream(dev)
         stream.wait_event(self.made)
@@ -62,13 +67,15 @@ class _Derived:
 
     def __setstate__(self, _):
         self.sig = self.val = self.made = self.streams = None
+        self.captured, self.older = False, ()
 
 
 def _cached(key, params, build, stamp=None):
     """Derived tensors live in a dict hung on the first source parameter (so they die with it and a
     recycled id() can never alias another model's entry). stamp: one more thing that the entry goes stale with. What is built while a
     graph is captured belongs to that graph - only its replays fill it, in memory that goes with it - and is not kept. An entry may be
-    used on any stream: see _Derived.join."""
+    used on any stream: see _Derived.join. A captured graph goes on reading the entry it met: its memory is kept, as it was then, after
+    a new one has taken its place."""
     store = params[0].__dict__.setdefault("_mfnet_derived", {})
     sig = (stamp,) + tuple((p.data_ptr(), p._version, p.device) for p in params)
     dev = params[0].get_device()
@@ -80,7 +87,7 @@ def _cached(key, params, build, stamp=None):
     with torch.no_grad():
         val = build()
     if dev < 0 or not torch.cuda.is_current_stream_capturing():
-        store[key] = _Derived(sig, val, dev)
+        store[key] = _Derived(sig, val, dev, hit)
     return val
 
 
@@ -628,7 +635,8 @@ class PooledLinear(nn.Linear):
     forward(x, ids): x [..., in] fp32 or bf16, ids int32 - one per row (x.shape[:-1]) or one per entry of x's first dimension; an index
     outside [0, n) takes the projection alone. -> [..., out] of x's dtype. lora_A [n, r, in] and lora_B [n, out, r] are trainable,
     `scaling` [n] is a buffer; the factors are rounded to bf16 for the products, their gradients are fp32.
-    checkpoint8: keep the input in 8 bits until the backward pass (ops.Ckpt8; in multiples of 8). plan: ops.lora_pool_plan of the same
+    checkpoint8: keep the input in 8 bits until the backward pass (ops.Ckpt8; in multiples of 8). A captured call reads the factors as
+    they are at each replay, and the frozen weight as it was at capture. plan: ops.lora_pool_plan of the same
     rows, to share one among the layers of a batch (None: the backward pass makes its own)."""
 
     def __init__(self, in_features, out_features, n_adapters, r, lora_alpha=1, bias=True, checkpoint8=False):

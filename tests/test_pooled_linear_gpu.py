@@ -136,3 +136,53 @@ def test_streams_without_an_order_share_a_module():
     assert torch.equal(late, want[0])
     assert all(torch.equal(p, q) for p, q in zip(got_a, calls(ref)))
     del junk
+
+
+def test_captured_call_keeps_the_weight_it_met():
+    """The frozen weight is re-loaded and an eager call makes a new copy of it: a graph captured before goes on with the weight as it was at
+    its capture (and the factors as they are), not with memory that was given away; the eager calls have the new weight."""
+    g, lin, ref = _twins(23, K=256, N=264)
+    x, dy = _rows(g, 130, 256).cuda(), _rows(g, 130, 264).cuda()
+    ids = torch.randint(-1, 3, (130,), generator=g, dtype=torch.int32).cuda()
+    _dx(lin, x, ids, dy)
+    xs = x.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lin(xs, ids)
+        dx = torch.autograd.grad(out, xs, dy)[0]
+    old_w = lin.weight.detach().clone()
+    for k in range(3):
+        with torch.no_grad():
+            lin.weight.copy_(_rows(g, 264, 256))
+            lin.lora_B.copy_(0.2 * _rows(g, 3, 264, 5))
+            ref.load_state_dict(lin.state_dict())
+        assert torch.equal(_dx(lin, x, ids, dy), _dx(ref, x, ids, dy))
+        junk = [torch.full((264 * 256,), float("nan"), device="cuda", dtype=torch.bfloat16) for _ in range(16)]
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            ref.weight.copy_(old_w)
+            assert torch.equal(out.detach(), ref(x, ids)), k
+        assert torch.equal(dx, _dx(ref, x, ids, dy)), k
+        del junk
+
+
+def test_stored_module_makes_its_copies_anew():
+    """torch.save of a whole module that has been called, and a deep copy: the copies it holds are not stored, the other module's are its own"""
+    import copy
+    import io
+    g, lin, ref = _twins(24)
+    x, dy = _rows(g, 40, 96).cuda(), _rows(g, 40, 72).cuda()
+    ids = torch.randint(-1, 3, (40,), generator=g, dtype=torch.int32).cuda()
+    want, wdx = lin(x, ids).detach(), _dx(lin, x, ids, dy)
+    with torch.no_grad():
+        assert torch.equal(lin(x, ids), want)
+    f = io.BytesIO()
+    torch.save(lin, f)
+    f.seek(0)
+    for other in (torch.load(f, weights_only=False), copy.deepcopy(lin)):
+        with torch.no_grad():
+            assert torch.equal(other(x, ids), want)
+            other.lora_B.mul_(2)
+            assert not torch.equal(other(x, ids), want) and torch.equal(lin(x, ids), want)
+        assert torch.equal(_dx(lin, x, ids, dy), wdx)
