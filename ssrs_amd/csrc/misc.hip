@@ -29,9 +29,9 @@ static inline unsigned grid_for(int64_t work_items) {
   return (unsigned)g;
 }
 extern "C" int mfnet_cast(const void* x, int x_dtype, void* y, int y_dtype, int64_t n, hipStream_t stream) {
-  MF_CHECK_ARG(x && y, "cast: null pointer");
   MF_CHECK_ARG(n >= 0 && n % 8 == 0, "cast: n=%lld must be a multiple of 8", (long long)n);
   if (n == 0) return MFNET_OK;
+  MF_CHECK_ARG(x && y, "cast: null pointer");
   if (x_dtype == MFNET_F32 && y_dtype == MFNET_BF16)
     hipLaunchKernelGGL(cast_f32_bf16_kernel, dim3(grid_for(n / 8)), dim3(256), 0, stream, (const float*)x, (bf16_t*)y, n / 8);
   else if (x_dtype == MFNET_BF16 && y_dtype == MFNET_F32)

@@ -696,7 +696,7 @@ class PooledLinear(nn.Linear):
             raise NotImplementedError("the shared projection of a lora.PooledLinear is frozen: its weight and bias get no gradients")
         if torch.is_grad_enabled() and any(t.requires_grad for t in (x, self.lora_A, self.lora_B)):
             return _PooledLinear.apply(x, self, ids.reshape(-1), plan, self.lora_A, self.lora_B)
-        return self._product(x, ids.reshape(-1), False)[0].view(*rows, -1)
+        return self._product(x, ids.reshape(-1), False)[0].view(*rows, self.out_features)
 
     def _factors(self, train):
         """the factors' images: kept while nothing writes to the factors; made anew (one launch) in a training step, whose optimizer
@@ -724,7 +724,7 @@ class _PooledLinear(torch.autograd.Function):
         ctx.kept8 = tuple(xb.shape) if lin.checkpoint8 else None
         ctx.save_for_backward(ops.ckpt8_pack(xb).buf if lin.checkpoint8 else xb, ids, down)
         ctx.lin, ctx.pool, ctx.plan, ctx.shape, ctx.dtype = lin, pool, plan, x.shape, x.dtype
-        return out.view(*x.shape[:-1], -1)
+        return out.view(*x.shape[:-1], lin.out_features)
 
     @staticmethod
     def backward(ctx, dout):

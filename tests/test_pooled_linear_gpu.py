@@ -186,3 +186,26 @@ def test_stored_module_makes_its_copies_anew():
             other.lora_B.mul_(2)
             assert not torch.equal(other(x, ids), want) and torch.equal(lin(x, ids), want)
         assert torch.equal(_dx(lin, x, ids, dy), wdx)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(0, 96), (0, 9, 96), (4, 0, 96)])
+@pytest.mark.parametrize("checkpoint8", [False, True])
+def test_batch_without_rows(shape, dtype, checkpoint8):
+    """[..., out] without rows, a gradient of x's shape, zero gradients of the factors; with a plan and without"""
+    from ssrs_amd import ops
+    g, lin, _ = _twins(25, checkpoint8=checkpoint8)
+    x = torch.zeros(shape, device="cuda", dtype=dtype)
+    ids = torch.zeros(shape[0], device="cuda", dtype=torch.int32)
+    with torch.no_grad():
+        y = lin(x, ids)
+    assert y.shape == shape[:-1] + (72,) and y.dtype == dtype
+    for plan in (None, ops.lora_pool_plan(torch.zeros(0, device="cuda", dtype=torch.int32), 3)):
+        lin.zero_grad(set_to_none=True)
+        xr = x.clone().requires_grad_()
+        y = lin(xr, ids, plan)
+        assert y.shape == shape[:-1] + (72,) and y.dtype == dtype
+        y.sum().backward()
+        assert xr.grad.shape == shape and xr.grad.dtype == dtype
+        for p in (lin.lora_A, lin.lora_B):
+            assert p.grad.shape == p.shape and (p.grad == 0).all()

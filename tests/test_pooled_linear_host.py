@@ -53,3 +53,12 @@ def test_pool_of_layers_without_a_bias():
     for mixed in ([layers[0], with_bias], [with_bias, layers[0]]):
         with pytest.raises(ValueError, match="bias"):
             lora.PooledLinear.from_merged(mixed)
+
+
+def test_cast_of_nothing():
+    """a batch without rows has no address"""
+    from ssrs_amd import _lib
+    L = _lib.lib()
+    assert L.mfnet_cast(None, 0, None, 1, 0, None) == 0
+    assert L.mfnet_cast(None, 0, None, 1, 8, None) == -1 and b"null" in L.mfnet_last_error()
+    assert L.mfnet_cast(None, 0, None, 1, 4, None) == -1 and b"multiple" in L.mfnet_last_error()
