@@ -1907,8 +1907,13 @@ def lora_pool(A, B, scale=None) -> LoraPool:
 
 class LoraPlan:
     """The rows of a batch grouped by adapter (lora_pool_plan): what the backward sums over an adapter's rows read. Depends on the row
-    indices alone: one plan serves every layer of a batch."""
-    __slots__ = ("ids", "M", "n", "offs", "perm", "base", "table")
+    indices alone: one plan serves every layer of a batch. It holds the indices as they were; older_than(ids) tells that the tensor
+    it was made of has been written to since."""
+    __slots__ = ("ids", "M", "n", "offs", "perm", "base", "table", "_source", "_version")
+
+    def older_than(self, ids):
+        s = self._source
+        return s is not None and self._version is not None and ids.data_ptr() == s.data_ptr() and s._version != self._version
 
 
 def _check_ids(name, ids, M):
@@ -1917,13 +1922,21 @@ def _check_ids(name, ids, M):
 
 
 def lora_pool_plan(ids, n) -> LoraPlan:
-    """ids int32 [M]: the adapter of every row (none if outside [0, n))."""
+    """ids int32 [M]: the adapter of every row (none if outside [0, n)). They may be written to afterwards: the plan holds a copy."""
     name = "lora_pool_plan"
     dev = _device_of(name, ids)
     _check_ids(name, ids, ids.shape[0] if ids.dim() else -1)
     if not 1 <= n <= 65535:
         _bad(name, f"n={n}: 1 .. 65535 adapters")
+    p = _lora_plan(ids + 0, n, dev)                              # (a kernel's copy: captured graphs hold kernels only)
+    p._source, p._version = ids, None if ids.is_inference() else ids._version
+    return p
+
+
+def _lora_plan(ids, n, dev):
+    """the plan of indices that nobody writes to while it lives"""
     p = LoraPlan()
+    p._source = p._version = None
     p.ids, p.M, p.n = ids, ids.shape[0], n
     chunks = _lib.lib().mfnet_lora_pool_chunks(p.M, n)
     p.table = torch.empty((max(chunks, 1), 4), dtype=torch.int32, device=ids.device)

@@ -637,7 +637,8 @@ class PooledLinear(nn.Linear):
     `scaling` [n] is a buffer; the factors are rounded to bf16 for the products, their gradients are fp32.
     checkpoint8: keep the input in 8 bits until the backward pass (ops.Ckpt8; in multiples of 8). A captured call reads the factors as
     they are at each replay, and the frozen weight as it was at capture. plan: ops.lora_pool_plan of the same
-    rows, to share one among the layers of a batch (None: the backward pass makes its own)."""
+    indices, row by row, to share one among the layers of a batch (None: the backward pass makes its own); of what it holds, the row and
+    adapter counts and a later write to its index tensor are checked, the indices themselves are the caller's to keep alike."""
 
     def __init__(self, in_features, out_features, n_adapters, r, lora_alpha=1, bias=True, checkpoint8=False):
         super().__init__(in_features, out_features, bias=bias)
@@ -692,6 +693,8 @@ class PooledLinear(nn.Linear):
             ids = ids.view(-1, *[1] * (len(rows) - 1)).expand(rows)
         if plan is not None and (plan.M != ids.numel() or plan.n != self.n_adapters):
             raise ValueError(f"the plan is of {plan.M} rows and {plan.n} adapters, not of {ids.numel()} and {self.n_adapters}")
+        if plan is not None and plan.older_than(ids):
+            raise ValueError("the plan is older than its row indices: they were written to after ops.lora_pool_plan")
         if torch.is_grad_enabled() and (self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad)):
             raise NotImplementedError("the shared projection of a lora.PooledLinear is frozen: its weight and bias get no gradients")
         if torch.is_grad_enabled() and any(t.requires_grad for t in (x, self.lora_A, self.lora_B)):
@@ -733,7 +736,7 @@ class _PooledLinear(torch.autograd.Function):
         x = kept if ctx.kept8 is None else ops.Ckpt8.of(kept, ctx.kept8)
         d2 = dout.reshape(-1, dout.shape[-1])
         d2 = d2 if d2.dtype == BF else ops.cast(d2.contiguous(), BF)
-        plan = ctx.plan if ctx.plan is not None else ops.lora_pool_plan(ids, lin.n_adapters)
+        plan = ctx.plan if ctx.plan is not None else ops._lora_plan(ids, lin.n_adapters, ids.get_device())      # (saved indices: autograd sees to it that they are the forward's)
         want_dx = ctx.needs_input_grad[0]
         dx, dA, dB = ops.lora_pool_bwd(d2, x, wT_bf16(lin.weight) if want_dx else None, ctx.pool, plan, down, want_dx=want_dx)
         if want_dx:

@@ -209,3 +209,43 @@ def test_batch_without_rows(shape, dtype, checkpoint8):
         assert xr.grad.shape == shape and xr.grad.dtype == dtype
         for p in (lin.lora_A, lin.lora_B):
             assert p.grad.shape == p.shape and (p.grad == 0).all()
+
+
+@pytest.mark.parametrize("M", [40, 700, 6000])
+def test_plan_holds_its_own_indices(M):
+    """a static index buffer that is refilled for the next batch between a plan and the backward passes that read it"""
+    from ssrs_amd import ops
+    g = torch.Generator().manual_seed(26)
+    n, K, N = 4, 136, 264
+    x, dy = _rows(g, M, K).bfloat16().cuda(), _rows(g, M, N).bfloat16().cuda()
+    w = _rows(g, N, K).bfloat16().cuda()
+    pool = ops.lora_pool(_rows(g, n, 6, K).cuda(), _rows(g, n, N, 6).cuda())
+    ids = torch.randint(-1, n, (M,), generator=g, dtype=torch.int32).cuda()
+    plan = ops.lora_pool_plan(ids, n)
+    down = ops.lora_pool_fwd(x, w, None, pool, ids, want_down=True)[1]
+    want = [t.clone() for t in ops.lora_pool_bwd(dy, x, w.t().contiguous(), pool, plan, down)]
+    ids.copy_(torch.randint(-1, n, (M,), generator=g, dtype=torch.int32))
+    assert all(torch.equal(a, b) for a, b in zip(ops.lora_pool_bwd(dy, x, w.t().contiguous(), pool, plan, down), want))
+
+
+def test_plan_older_than_its_indices_is_refused():
+    """the indices were written to after the plan was made of them: that plan is of other rows now"""
+    from ssrs_amd import ops
+    g, lin, ref = _twins(27)
+    x = _rows(g, 4, 10, 96).cuda()
+    ids = torch.randint(-1, 3, (40,), generator=g, dtype=torch.int32).cuda()
+    plan = ops.lora_pool_plan(ids, 3)
+    want = lin(x, ids.view(4, 10), plan)
+    assert torch.equal(want, ref(x, ids.view(4, 10)))
+    assert torch.equal(lin(x, ids.clone().view(4, 10), plan), want)           # (the same rows in another tensor)
+    ids.copy_(torch.randint(-1, 3, (40,), generator=g, dtype=torch.int32))
+    for bad in (ids.view(4, 10), ids.view(4, 10)[:, :]):
+        with pytest.raises(ValueError, match="plan"):
+            lin(x, bad, plan)
+    per_image = torch.randint(0, 3, (40,), generator=g, dtype=torch.int32).cuda()     # one index per image of one row
+    plan = ops.lora_pool_plan(per_image, 3)
+    one = x.view(40, 1, 96)
+    assert torch.equal(lin(one, per_image, plan), ref(one, per_image))
+    per_image.zero_()
+    with pytest.raises(ValueError, match="plan"):
+        lin(one, per_image, plan)
