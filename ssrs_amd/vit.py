@@ -697,9 +697,10 @@ class PooledLinear(nn.Linear):
             raise ValueError("the plan is older than its row indices: they were written to after ops.lora_pool_plan")
         if torch.is_grad_enabled() and (self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad)):
             raise NotImplementedError("the shared projection of a lora.PooledLinear is frozen: its weight and bias get no gradients")
+        ids = ids.reshape(-1).contiguous()
         if torch.is_grad_enabled() and any(t.requires_grad for t in (x, self.lora_A, self.lora_B)):
-            return _PooledLinear.apply(x, self, ids.reshape(-1), plan, self.lora_A, self.lora_B)
-        return self._product(x, ids.reshape(-1), False)[0].view(*rows, self.out_features)
+            return _PooledLinear.apply(x, self, ids, plan, self.lora_A, self.lora_B)
+        return self._product(x, ids, False)[0].view(*rows, self.out_features)
 
     def _factors(self, train):
         """the factors' images: kept while nothing writes to the factors; made anew (one launch) in a training step, whose optimizer

@@ -249,3 +249,19 @@ def test_plan_older_than_its_indices_is_refused():
     per_image.zero_()
     with pytest.raises(ValueError, match="plan"):
         lin(one, per_image, plan)
+
+
+def test_indices_with_a_stride():
+    """a column of a request table, every second entry, reversed dimensions: one index per row, however they lie"""
+    g, lin, ref = _twins(28)
+    table = torch.randint(-1, 3, (40, 3), generator=g, dtype=torch.int32).cuda()
+    x, dy = _rows(g, 40, 96).cuda(), _rows(g, 40, 72).cuda()
+    for ids in (table[:, 1], table.view(-1)[::3], table.t()[2], table[:1, 0].expand(40)):
+        assert not ids.is_contiguous()
+        with torch.no_grad():
+            assert torch.equal(lin(x, ids), ref(x, ids.contiguous()))
+        assert torch.equal(_dx(lin, x, ids, dy), _dx(ref, x, ids.contiguous(), dy))
+        assert torch.equal(lin(x.view(40, 1, 96), ids).view(40, 72), ref(x, ids.contiguous()))
+    ids = table.t()[:2]                                          # [2, 40] with strides (1, 3)
+    two = torch.stack([x, dy.new_zeros(40, 96)])
+    assert torch.equal(lin(two, ids), ref(two, ids.contiguous()))
