@@ -682,6 +682,9 @@ class PooledLinear(nn.Linear):
         return pool
 
     def forward(self, x, ids, plan=None):
+        if x.is_cuda and x.get_device() != ops._current_device():            # (launches, allocations and capture checks go by the current device)
+            with torch.cuda.device(x.get_device()):
+                return self.forward(x, ids, plan)
         if ops.FP32:
             raise NotImplementedError("lora.PooledLinear runs on the bf16 MFMA: it has no fp32 mode")
         if x.dtype not in (torch.float32, BF):

@@ -265,3 +265,35 @@ def test_indices_with_a_stride():
     ids = table.t()[:2]                                          # [2, 40] with strides (1, 3)
     two = torch.stack([x, dy.new_zeros(40, 96)])
     assert torch.equal(lin(two, ids), ref(two, ids.contiguous()))
+
+
+@pytest.mark.parametrize("train", [False, True])
+def test_launches_on_the_inputs_device(monkeypatch, train):
+    """another device is current: every launch of the call, the casts of x and of the weight among them, runs under the device of x"""
+    from ssrs_amd import ops
+    g, lin, ref = _twins(29)
+    x = _rows(g, 40, 96).cuda()
+    ids = torch.randint(-1, 3, (40,), generator=g, dtype=torch.int32).cuda()
+    with torch.set_grad_enabled(train):
+        want = ref(x, ids)
+    under, calls, real_device, real_call = [], [], torch.cuda.device, ops.call
+
+    class Device(real_device):
+        def __enter__(self):
+            under.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *exc):
+            under.pop()
+            return super().__exit__(*exc)
+
+    def call(name, *args):
+        calls.append((name, under[-1:] == [x.get_device()]))
+        return real_call(name, *args)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(ops, "_current_device", lambda: under[-1] if under else 7)
+    monkeypatch.setattr(ops, "call", call)
+    with torch.set_grad_enabled(train):
+        got = lin(x, ids)
+    assert torch.equal(got, want) and {"mfnet_cast", "mfnet_lora_pool_pack", "mfnet_lora_pool_fwd"} <= {name for name, _ in calls}
+    assert all(ok for _, ok in calls), calls
