@@ -1597,8 +1597,10 @@ def gather(pairs, accumulate=False):
 # ------------------------------------------------------------------------------------------ 8-bit activation checkpoints
 # The wrappers below are called with tensors of a few microseconds' work: their checks are written to cost about one (device indices
 # instead of device objects, messages formatted only when raised, one allocation for what belongs together).
-raw_stream = torch._C._cuda_getCurrentRawStream        # torch.cuda.current_stream(device).cuda_stream without the Stream object
-_current_device = torch._C._cuda_getDevice              # torch.cuda.current_device() of a process that holds device tensors
+# torch.cuda.current_stream(device).cuda_stream without the Stream object; torch.cuda.current_device() of a process that holds device
+# tensors (None in a torch without a GPU backend, where there are none)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _bad(name, what):

@@ -62,3 +62,25 @@ def test_cast_of_nothing():
     assert L.mfnet_cast(None, 0, None, 1, 0, None) == 0
     assert L.mfnet_cast(None, 0, None, 1, 8, None) == -1 and b"null" in L.mfnet_last_error()
     assert L.mfnet_cast(None, 0, None, 1, 4, None) == -1 and b"multiple" in L.mfnet_last_error()
+
+
+def test_import_with_a_torch_that_has_no_gpu_backend():
+    """ops is imported by code that runs on the host alone (state dicts, plans of rasters); only calls need the GPU backend"""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for n in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):\n"
+            "    delattr(torch._C, n)\n"
+            "from ssrs_amd import ops\n"
+            "from ssrs_amd.vit import PooledLinear\n"
+            "PooledLinear(64, 64, 2, 4)\n"
+            "try:\n"
+            "    ops.ckpt8_pack(torch.zeros(4, 64))\n"
+            "except ops.MfnetError as e:\n"
+            "    assert 'CPU tensor' in str(e)\n"
+            "else:\n"
+            "    raise SystemExit(1)\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
