@@ -330,8 +330,9 @@ class UNetFormer(nn.Module):
         self.decoder = Decoder(ec, decode_channels, dropout, window_size, num_classes)
         # what an MMLoRA encoder block keeps between its forward and its backward pass. "bf16" (default): the fp32 residual stream, the
         # LayerNorm outputs, lin1's output and GELU of it. "int8": the residual stream and lin1's output in 8 bits (ops.Ckpt8), the rest
-        # is made again - 2.6x less memory per block, the same forward, gradients that see the rounded activations. Choose before the
-        # first training step; fp32 mode keeps everything.
+        # is made again - 2.6x less memory per block, gradients that see the rounded activations, a forward of the same roundings whose
+        # fp32 sums (statistics, down products) are added in another order. Choose before the first training step; fp32 mode keeps
+        # everything.
         self.checkpoints = checkpoints or "bf16"
 
     @property

@@ -394,8 +394,8 @@ class _LoraMlpBranch(torch.autograd.Function):
             l2 = blk.mlp.lin2
             ln, mean, rstd, ck = ops.layernorm_fwd_ckpt8(h2, blk.norm2.weight, blk.norm2.bias, blk.norm2.eps)
             s1 = _down8(ln, l1.lora_Ax, l1.lora_Ay, half, l1.lora_wx.detach(), l1.lora_wy.detach())
-            pre = _mix_linear_fwd(ln, l1, half, False, None, s1)[0]
-            act, ckp = ops.gelu_fwd_ckpt8(pre)
+            act, pre, _ = _mix_linear_fwd(ln, l1, half, True, None, s1)      # GELU of the fp32 sums, as without checkpoints
+            ckp = ops.ckpt8_pack(pre)
             out, _, s2 = _mix_linear_fwd(act, l2, half, False, h2)
             ctx.save_for_backward(ck.buf, mean, rstd, ckp.buf, None, None, *s1, *s2)
             ctx.blk, ctx.kept8 = blk, (ck.shape, ckp.shape)
