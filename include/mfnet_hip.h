@@ -355,6 +355,9 @@ int mfnet_dwconv_bwd_data(const void* dy, int dy_dtype, const float* w, float* d
                           int64_t k, int ext, hipStream_t stream);
 int mfnet_dwconv_bwd_weight(const void* dy, int dy_dtype, const float* x, float* dw, float* dbias, int64_t B, int64_t H,
                             int64_t W, int64_t C, int64_t k, int ext, int slots, hipStream_t stream);
+/* Workgroups of mfnet_dwconv_bwd_weight over npix = B H W pixels (at most 1024): workgroup i adds into copy i % slots of dw / dbias, so with
+ * as many slots (1 .. 1024) every copy has one writer and the sum over the copies does not depend on the run. */
+int64_t mfnet_dwconv_bwd_weight_workgroups(int64_t npix, int64_t k);
 /* Several depthwise weight gradients in one launch (independent of the backward chain, collected by the host like
  * mfnet_gemm_tn_batch; what autograd computes node by node for the depthwise convs of unetformer_mmsam.py:52-84,117-131).
  * desc: 12 int64 per problem - dy, dy_dtype, x, dw, dbias (0: none), B, H, W, C, k, ext, slots. */
@@ -542,10 +545,10 @@ int64_t mfnet_layernorm_ckpt8_workspace_floats(int64_t rows, int64_t C);
  * writes all four from A [n][r][K] and B [n][N][r], fp32 or bf16, and copies scale [n] (NULL: ones). K and N are
  * multiples of 8, rows 16-byte aligned with strides that are multiples of 8; M < 2^27, n <= 65535. No call synchronises,
  * allocates or uses atomics; the same inputs give the same bits. An adapter's or a row's infinities and NaN reach only the rows of that
- * adapter, or that row, and their gradients. No output or workspace may overlap an input. */
+ * adapter, or that row, and their gradients, where an infinity may end as NaN. No output or workspace may overlap an input. */
 int mfnet_lora_pool_pack(const void* A, const void* B, int dtype, const float* scale, int64_t n, int64_t K, int64_t N, int r, int RP,
                          void* a_down, void* a_up, void* b_down, void* b_up, float* scale_out, hipStream_t stream);
-/* Rows grouped by adapter, ascending inside each: offs [n + 1], perm [M], and chunks of rows for the backward sums: base [n + 1], table
+/* Of one batch's ids, which the backward pass reads beside the plan and which stay as they are until then. Rows grouped by adapter, ascending inside each: offs [n + 1], perm [M], and chunks of rows for the backward sums: base [n + 1], table
  * [4 * mfnet_lora_pool_chunks(M, n)] int32 (16-byte aligned). Depends on ids alone: one per batch serves all of its layers. */
 int mfnet_lora_pool_plan(const int* ids, int64_t M, int64_t n, int* offs, int* perm, int* base, int* table, hipStream_t stream);
 int64_t mfnet_lora_pool_chunks(int64_t M, int64_t n);

@@ -144,6 +144,7 @@ _SIGS = {
 
 # host-side size helpers: name -> (restype, argtypes)
 _HELPERS = {
+    "mfnet_dwconv_bwd_weight_workgroups": (c_int64, [I64, I64]),
     "mfnet_layernorm_ckpt8_workspace_floats": (c_int64, [I64, I64]),
     "mfnet_lora_pool_chunks": (c_int64, [I64, I64]),
     "mfnet_lora_pool_image_elements": (c_int64, [I64, I]),

@@ -743,7 +743,7 @@ __device__ __forceinline__ void dw_tap_body(const void* __restrict__ dy, const f
       }
     }
     // same-address float atomics cost ~140 ns each on this chip: the workgroups spread over `slots` copies of dw / dbias
-    // that the caller sums (512 workgroups on one copy: 70 of the kernel's 110 us)
+    // that the caller sums (512 workgroups on one copy: 70 of the kernel's 110 us). A copy per workgroup: the same bits each run.
     const int sl = bid % slots;
     float* o = dw + ((int64_t)sl * p.C + 4 * cg) * kk + tap;
     atomicAdd(o, acc.x); atomicAdd(o + kk, acc.y); atomicAdd(o + 2 * kk, acc.z); atomicAdd(o + 3 * kk, acc.w);
@@ -895,6 +895,11 @@ static void dw_weight_geometry(int64_t npix, int64_t k, int* kind, int64_t* ppb,
   }
   *nwg = ceil_div64(npix, *ppb);
 }
+extern "C" int64_t mfnet_dwconv_bwd_weight_workgroups(int64_t npix, int64_t k) {
+  int kind; int64_t ppb, nwg = 0;
+  if (npix > 0) dw_weight_geometry(npix, k, &kind, &ppb, &nwg);
+  return nwg;
+}
 // desc: 12 int64 per problem - dy, dy_dtype, x, dw, dbias (0: none), B, H, W, C, k, ext, slots; per problem exactly
 // mfnet_dwconv_bwd_weight (dw / dbias are ADDED into).
 extern "C" int mfnet_dwconv_bwd_weight_batch(const int64_t* desc, int64_t n, hipStream_t stream) {
@@ -907,7 +912,7 @@ extern "C" int mfnet_dwconv_bwd_weight_batch(const int64_t* desc, int64_t n, hip
     for (int j = 0; j < b.n; ++j) {
       const int64_t* d = desc + 12 * (i0 + j);
       DwProb& q = b.q[j];
-      MF_CHECK_ARG(d[0] && d[2] && d[3] && d[11] >= 1 && d[11] <= 64 && (d[1] == MFNET_BF16 || d[1] == MFNET_F32), "dwconv_bwd_weight_batch: bad problem %lld", (long long)(i0 + j));
+      MF_CHECK_ARG(d[0] && d[2] && d[3] && d[11] >= 1 && d[11] <= 1024 && (d[1] == MFNET_BF16 || d[1] == MFNET_F32), "dwconv_bwd_weight_batch: bad problem %lld", (long long)(i0 + j));
       int rc = dw_check(&q.p, d[5], d[6], d[7], d[8], d[9], (int)d[10], "dwconv_bwd_weight_batch");
       if (rc) return rc;
       q.dy = (const void*)d[0]; q.bf16 = d[1] == MFNET_BF16; q.x = (const float*)d[2]; q.dw = (float*)d[3]; q.dbias = (float*)d[4]; q.slots = (int)d[11];
@@ -924,7 +929,7 @@ extern "C" int mfnet_dwconv_bwd_weight_batch(const int64_t* desc, int64_t n, hip
 }
 extern "C" int mfnet_dwconv_bwd_weight(const void* dy, int dy_dtype, const float* x, float* dw, float* dbias, int64_t B, int64_t H, int64_t W,
                                        int64_t C, int64_t k, int ext, int slots, hipStream_t stream) {
-  MF_CHECK_ARG(dy && x && dw && slots >= 1 && slots <= 64, "dwconv_bwd_weight: null pointer / slots not in [1, 64]");
+  MF_CHECK_ARG(dy && x && dw && slots >= 1 && slots <= 1024, "dwconv_bwd_weight: null pointer / slots not in [1, 1024]");
   DwParams p;
   int rc = dw_check(&p, B, H, W, C, k, ext, "dwconv_bwd_weight");
   if (rc) return rc;

@@ -1205,7 +1205,9 @@ def dwconv_bwd(dy, x, w, B, H, W, k, ext, want_bias=False):
     assert dy.is_contiguous() and x.is_contiguous() and x.dtype == torch.float32
     dx = torch.empty_like(x)
     tcall("mfnet_dwconv_bwd_data", dy.numel() * dy.element_size() + x.numel() * 4, 2.0 * x.numel() * k * k, dy.data_ptr(), _dt(dy), w.data_ptr(), dx.data_ptr(), B, H, W, C, k, 1 if ext else 0, _stream(x))
-    slots = 32                                           # copies of dw / db the workgroups spread their atomics over
+    # copies of dw / db the workgroups spread their atomics over: 32; in fp32 mode, whose runs are compared step by step, one each, so
+    # that the sum has one order (the small differences of these gradients grew to 1e-5 of the loss within five steps)
+    slots = int(_lib.lib().mfnet_dwconv_bwd_weight_workgroups(B * H * W, k)) if FP32 else 32
     dw = zeros((slots,) + tuple(w.shape), x.device)
     db = zeros((slots, C), x.device) if want_bias else None
     if TN_QUEUE is not None:
