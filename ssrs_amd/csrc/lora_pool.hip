@@ -9,10 +9,12 @@
 //
 // The factors are held as bf16 images padded to RP = 16, 32 or 64 ranks (mfnet_lora_pool_pack): "down" images for products that contract
 // over the long axis, "up" images for products that contract over the ranks, so that both are read as MFMA
-// operands in 16-byte pieces. fp32 factors of a product (down, p) are split into bf16 parts hi + lo (+ lo'), never rounded once.
+// operands in 16-byte pieces. Adapters given in fp32 are rounded to bf16 there, once. The fp32 factors that a call makes itself (down, p)
+// are split into bf16 parts hi + lo (+ lo').
 //
 // A workgroup that meets rows of several adapters multiplies all its rows with each adapter in turn and SELECTS the rows it belongs to:
-// a sum of zeros would let one adapter's infinities and NaN into another request's rows.
+// a sum of zeros would let one adapter's infinities and NaN into another request's rows. In its own rows an infinity may end as NaN: padded
+// ranks hold 0 * inf, the split inf - inf.
 #include "ckpt8.h"
 #include <math.h>
 #include <type_traits>
@@ -1377,7 +1379,8 @@ static int pool_products(PoolGemm& p, const void* image, const float* scale, con
   // One launch for both products saves the host 3 us, but every workgroup makes all down products again: it pays while they are few. us a
   // call, issued one by one (on the GPU alone): 16 rows, 768 -> 2304, rank 16: 11.4 (10.8) in one launch, 14.7 (7.1) in two; 8 rows,
   // 1280 -> 3840: 11.3 (10.8), 14.3 (8.1); 16 rows: 15.8 (16.1), 14.7 (8.6); 1 row, 1280 -> 5120, rank 32: 11.3 (10.6), 14.9 (10.0); 1 row,
-  // 5120 -> 1280, rank 16: 21.0 (21.5), 15.8 (15.5). (64 ranks: more registers than 16 waves have.)
+  // 5120 -> 1280, rank 16: 21.0 (21.5), 15.8 (15.5). (64 ranks: more registers than 16 waves have.) The rule goes by calls issued one by one:
+  // in a replayed graph two launches are the faster form wherever their time on the GPU is.
   const int64_t one_row = (int64_t)p.K * p.RP;
   if (p.M > 16 || p.RP > 32 || one_row > 40960 || p.M * one_row > (1 << 18)) {
     PoolDown d = {down, reinterpret_cast<bf16_t*>(down + p.M * p.RP), pool_few(p.M, p.N) ? 0 : p.out_f32 ? 3 : 2};

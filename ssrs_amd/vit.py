@@ -634,7 +634,8 @@ class PooledLinear(nn.Linear):
 
     forward(x, ids): x [..., in] fp32 or bf16, ids int32 - one per row (x.shape[:-1]) or one per entry of x's first dimension; an index
     outside [0, n) takes the projection alone. -> [..., out] of x's dtype. lora_A [n, r, in] and lora_B [n, out, r] are trainable,
-    `scaling` [n] is a buffer; the factors are rounded to bf16 for the products, their gradients are fp32.
+    `scaling` [n] is a buffer; the factors are rounded to bf16 for the products, their gradients are fp32; x's gradient is rounded to bf16
+    also where x is fp32.
     checkpoint8: keep the input in 8 bits until the backward pass (ops.Ckpt8; in multiples of 8). A captured call reads the factors as
     they are at each replay, and the frozen weight as it was at capture. plan: ops.lora_pool_plan of the same
     indices, row by row, to share one among the layers of a batch (None: the backward pass makes its own); of what it holds, the row and
