@@ -134,7 +134,9 @@ __device__ __forceinline__ void colreduce_finish(const ColRedParams& p, const in
   for (int c0 = 0; c0 < ncg; c0 += cpp) {
     const int cl = threadIdx.x % cpp, part = threadIdx.x / cpp, c4 = c0 + cl;
     float4 tot = F4ZERO;
-    const bool on = part < parts;                      // 256 % cpp != 0: the threads past the last whole part idle
+    // 256 % cpp != 0: the threads past the last whole part idle; and so do those past the last column group of the last pass (two sums of
+    // 516 .. 1020 columns: their loads left the workspace and their adds the output)
+    const bool on = part < parts && c4 < ncg;
     for (int sb = part; on && sb < splits; sb += 16 * parts) {
       float4 v[16];
 #pragma unroll
@@ -148,7 +150,7 @@ __device__ __forceinline__ void colreduce_finish(const ColRedParams& p, const in
     __syncthreads();
     if (on) red0[part * cpp + cl] = tot;
     __syncthreads();
-    if (part == 0) {
+    if (on && part == 0) {
       for (int k = 1; k < parts; ++k) tot = f4add(tot, red0[k * cpp + cl]);
       float* o = 4 * c4 < p.C ? p.out0 + g * p.C + 4 * c4 : p.out1 + g * p.C + 4 * c4 - p.C;
       o[0] += tot.x; o[1] += tot.y; o[2] += tot.z; o[3] += tot.w;
